@@ -24,7 +24,9 @@
  *      b  Q4_K of 3 to 16 rows (2 where K >= 8192); ttq_linear_forward_allreduce is of kinds a and b
  *         (rows too long for that kernel are of kind c instead: count 3 to 16 rows as both unless K is small)
  *      c  Q4_K from 17 rows, Q8_0 / Q6_K from 9, trellis from 65        d  every trellis call        e  ttq_decode_attention
- *    An expert layer (ttq_moe) has a workspace of its own and overlaps with anything but itself.
+ *    An expert layer (ttq_moe) or a paged-attention plan (ttq_paged) has a workspace of its own and overlaps with anything but
+ *    itself: two streams, or two captured graphs that may run at the same time, take two plans.  ttq_paged_append and ttq_sample
+ *    have no workspace and overlap with anything.
  *  - Device-pointer entry points are asynchronous on `stream`; *_host entry points copy in, run,
  *    copy out and synchronise before returning.
  *  - Shapes: W is [N = out_features][K = in_features]; x is [M][ldx] (ldx >= K, in elements);
@@ -51,6 +53,7 @@ typedef struct ttq_weight ttq_weight;
 typedef struct ttq_comm ttq_comm;
 typedef struct ttq_moe ttq_moe;
 typedef struct ttq_host_batch ttq_host_batch;
+typedef struct ttq_paged ttq_paged;
 
 typedef enum ttq_status {
     TTQ_OK = 0,
@@ -216,7 +219,8 @@ TTQ_API ttq_status ttq_host_batch_destroy(ttq_host_batch *batch);
 TTQ_API ttq_status ttq_host_sync(ttq_ctx *ctx);
 
 /* Synchronises `stream` and reports whether any kernel launched through this context since the last
- * check gave up a bounded device-side wait (TTQ_ERR_TIMEOUT; the flag is cleared).  The *_host entry
+ * check gave up a bounded device-side wait (TTQ_ERR_TIMEOUT; the flag is cleared) or met a page id or position outside
+ * a paged cache (TTQ_ERR_SHAPE; likewise).  The *_host entry
  * points perform this check themselves. */
 TTQ_API ttq_status ttq_device_status(ttq_ctx *ctx, void *stream);
 
@@ -349,6 +353,89 @@ TTQ_API ttq_status ttq_rope_kv_append(ttq_ctx *ctx, const void *qkv_dev, ttq_dty
 TTQ_API ttq_status ttq_decode_attention(ttq_ctx *ctx, const void *q_dev, const void *k_cache_dev, const void *v_cache_dev,
                                         ttq_dtype dt, int64_t B, int32_t hq, int32_t hkv, int32_t d, int64_t ctx_len,
                                         int64_t n_ctx, void *out_dev, void *stream);
+
+/* ---- paged key/value cache: append with rotation, attention of a ragged batch ---------------------
+ * The reference keeps one growing, contiguous cache per sequence (KVCache.append, attn.nim:97-104) and attends over it with
+ * scaled_dot_product_attention (attn.nim:56-88,149-189).  Here a layer's keys and values live in pages of `page_size` tokens
+ * that any sequence may own, and a call serves a ragged batch: prompts, pieces of prompts and single tokens together. */
+
+/* One layer's pages.  Element (page, head, slot, i) of K is at k_dev + page * page_stride + head * head_stride
+ * + slot * token_stride + i (strides in elements, any order of the three; the head dimension is contiguous), V alike. */
+typedef struct ttq_kv_pages {
+    void *k_dev, *v_dev; /* 16-byte aligned */
+    int64_t n_pages;
+    int64_t page_stride, head_stride, token_stride; /* multiples of 8 */
+} ttq_kv_pages;
+
+/* A ragged batch.  The rows q_start[b] .. q_start[b+1]-1 of the call's tokens are the newest of the kv_len[b] tokens of
+ * sequence b: its token i is at position kv_len[b] - (q_start[b+1] - q_start[b]) + i.  Rows from q_start[n_seqs] on belong to
+ * no sequence (a padded batch) and are left as they were; a sequence may bring no token.  All three arrays are int32 in
+ * device memory, so a captured graph follows their contents.
+ * With prefix_len > 0 every sequence begins with the same prefix_len tokens, whose pages are prefix_table[0 ..
+ * ceil(prefix_len / page_size) - 1]; kv_len counts them, the sequence's own table starts behind them: position p >= prefix_len is
+ * slot (p - prefix_len) % page_size of page block_table[b][(p - prefix_len) / page_size].
+ * Only table entries of pages with a visible (attention) or new (append) position are read, so pages that slid out of a window
+ * may have been given away.  A page id outside 0 .. n_pages-1 or a position outside the table or the cos / sin rows touches no
+ * memory; the call's results are then invalid and ttq_device_status reports TTQ_ERR_SHAPE. */
+typedef struct ttq_paged_batch {
+    int64_t n_seqs, n_tokens;   /* n_tokens: rows of qkv, q and out (at least q_start[n_seqs]) */
+    int64_t max_q;              /* most new tokens of any sequence: selects the kernel, results do not depend on it (0: unknown) */
+    const int32_t *q_start_dev;     /* [n_seqs + 1], ascending from 0 */
+    const int32_t *kv_len_dev;      /* [n_seqs] */
+    const int32_t *block_table_dev; /* [n_seqs][ld_table], the first table_len entries of a row are used */
+    int64_t table_len, ld_table;
+    int64_t prefix_len;
+    const int32_t *prefix_table_dev;
+} ttq_paged_batch;
+
+/* A plan: head geometry and the workspace of one attention call.  One plan serves all layers of a model.  dt: bf16 or f16;
+ * d = 64 or 128; hq a multiple of hkv; page_size a power of two, 16 to 1024.  max_seqs and max_tokens bound the batches;
+ * max_prefix_tokens (0: none) bounds the tokens of calls with a shared prefix, whose partial results take
+ * (d + 1) * 4 bytes per token and query head. */
+TTQ_API ttq_status ttq_paged_create(ttq_ctx *ctx, ttq_dtype dt, int32_t hq, int32_t hkv, int32_t d, int32_t page_size,
+                                    int64_t max_seqs, int64_t max_tokens, int64_t max_prefix_tokens, ttq_paged **out);
+TTQ_API ttq_status ttq_paged_destroy(ttq_paged *plan);
+
+/* For every token of the batch: the q and k heads of its fused qkv row [hq q heads | hkv k heads | hkv v heads] x d are
+ * normalised (x * rsqrt(mean(x^2) + eps) * weight[d] per head, where q_norm_dev / k_norm_dev are given; attn.nim:175-178),
+ * rotated in the rotate-half form (rope.nim:29-92) with row `position` of cos_dev / sin_dev ([n_rope][d], f32 or the
+ * plan's dtype), q goes to q_out [n_tokens][ld_q] (hq x d used), k and v into the sequence's pages.  fp32 arithmetic,
+ * rounded once.  Two tokens must not share a slot. */
+TTQ_API ttq_status ttq_paged_append(ttq_ctx *ctx, ttq_paged *plan, const ttq_kv_pages *kv, const ttq_paged_batch *batch,
+                                    const void *qkv_dev, int64_t ld_qkv, const void *q_norm_dev, const void *k_norm_dev, float eps,
+                                    const void *cos_dev, const void *sin_dev, ttq_dtype rope_dt, int64_t n_rope, void *q_out_dev,
+                                    int64_t ld_q, void *stream);
+
+/* Causal grouped-query attention of the batch's tokens over their sequences' pages (their own keys included: append first):
+ * out[t][h] = softmax_j(scale * q[t][h] . k[j][h / (hq/hkv)]) . v over the keys j <= p of a token at position p and, with
+ * window > 0, of those only j > p - window or j < sinks (the first tokens stay visible).  A row that sees no key gives zeros.
+ * q and out: [n_tokens][ld], hq x d used, 16-byte aligned rows of the plan's dtype.  Scores, softmax statistics and sums in
+ * fp32; the softmax weights enter the second product in the plan's dtype.  What the cache holds at positions that no token
+ * of a sequence sees is ignored, NaN included; keys and values that some token sees must be finite. */
+TTQ_API ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *plan, const ttq_kv_pages *kv, const ttq_paged_batch *batch,
+                                       const void *q_dev, int64_t ld_q, float scale, int64_t window, int64_t sinks,
+                                       void *out_dev, int64_t ld_out, void *stream);
+
+/* ---- sampling ---------------------------------------------------------------------------------------
+ * No reference counterpart (the reference has no sampler).  Settings of the rows: an array of M values in device memory, or
+ * NULL and one value for all. */
+typedef struct ttq_sampling {
+    const float *temperature_dev, *top_p_dev, *min_p_dev;
+    const int32_t *top_k_dev;
+    float temperature, top_p, min_p; /* where the array is NULL */
+    int32_t top_k;
+} ttq_sampling;
+
+/* ids[m] = the next token of logits row m [V] (f32, bf16 or f16), drawn with the random number u[m] in [0, 1).
+ * With w_i = exp((x_i - max x) / temperature) the tokens in descending order of x (equal logits: lowest index first) are cut to
+ * the first top_k (0 or less: all), of those to the shortest run that holds top_p of their weight (1 or more: all; at least
+ * one token stays), of those to w_i >= min_p.  The result is the first token, in the order of the vocabulary, at which the
+ * cumulative weight of what is left exceeds u[m] times its total.  temperature <= 0 or NaN: the token of the largest logit (lowest
+ * index).  NaN logits count as -inf, a row of nothing but -inf gives -1; where a logit is +inf only such tokens have weight.
+ * Weights are computed in 64 bits and summed as 2^-44 fixed point, so that the cuts fall where the definition has them and
+ * results do not depend on the order of summation.  Any M >= 0, V from 1 to 2^18. */
+TTQ_API ttq_status ttq_sample(ttq_ctx *ctx, const void *logits_dev, ttq_dtype dt, int64_t M, int64_t V, int64_t ld,
+                              const ttq_sampling *sampling, const float *u_dev, int64_t *ids_dev, void *stream);
 
 /* ---- mixture-of-experts layer (grouped quantized GEMM) -----------------------------------------
  * No reference counterpart: the reference has dense gated MLPs only

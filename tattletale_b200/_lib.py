@@ -35,6 +35,25 @@ class HostLinear(ctypes.Structure):
                 ("y_dt", ctypes.c_int32), ("ldy", ctypes.c_int64)]
 
 
+class KvPages(ctypes.Structure):
+    """``ttq_kv_pages``: one layer's pages."""
+    _fields_ = [("k_dev", ctypes.c_void_p), ("v_dev", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64)]
+
+
+class PagedBatchArgs(ctypes.Structure):
+    """``ttq_paged_batch``: a ragged batch over a paged cache."""
+    _fields_ = [("n_seqs", ctypes.c_int64), ("n_tokens", ctypes.c_int64), ("max_q", ctypes.c_int64), ("q_start_dev", ctypes.c_void_p),
+                ("kv_len_dev", ctypes.c_void_p), ("block_table_dev", ctypes.c_void_p), ("table_len", ctypes.c_int64), ("ld_table", ctypes.c_int64),
+                ("prefix_len", ctypes.c_int64), ("prefix_table_dev", ctypes.c_void_p)]
+
+
+class Sampling(ctypes.Structure):
+    """``ttq_sampling``: settings of the sampler, per row or for all rows."""
+    _fields_ = [("temperature_dev", ctypes.c_void_p), ("top_p_dev", ctypes.c_void_p), ("min_p_dev", ctypes.c_void_p), ("top_k_dev", ctypes.c_void_p),
+                ("temperature", ctypes.c_float), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32)]
+
+
 SIGNATURES = {
     "ttq_init": (_ci, [_ci, _pp]),
     "ttq_destroy": (_ci, [_vp]),
@@ -78,6 +97,13 @@ SIGNATURES = {
     "ttq_rope_kv_append": (_ci, [_vp, _vp, _ci, _i64, _i64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _vp, _vp, _vp, _vp, _vp,
                                  _i64, _i64, _vp]),
     "ttq_decode_attention": (_ci, [_vp, _vp, _vp, _vp, _ci, _i64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _i64, _i64, _vp, _vp]),
+    "ttq_paged_create": (_ci, [_vp, _ci, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _i64, _i64, _i64, _pp]),
+    "ttq_paged_destroy": (_ci, [_vp]),
+    "ttq_paged_append": (_ci, [_vp, _vp, ctypes.POINTER(KvPages), ctypes.POINTER(PagedBatchArgs), _vp, _i64, _vp, _vp, ctypes.c_float, _vp, _vp, _ci,
+                               _i64, _vp, _i64, _vp]),
+    "ttq_paged_attention": (_ci, [_vp, _vp, ctypes.POINTER(KvPages), ctypes.POINTER(PagedBatchArgs), _vp, _i64, ctypes.c_float, _i64, _i64, _vp, _i64,
+                                  _vp]),
+    "ttq_sample": (_ci, [_vp, _vp, _ci, _i64, _i64, _i64, ctypes.POINTER(Sampling), _vp, _vp, _vp]),
     "ttq_launch_count": (_i64, [_vp]),
     "ttq_device_status": (_ci, [_vp, _vp]),
     "ttq_trace_read": (_ci, [_vp, _vp, _i64, ctypes.POINTER(_i64)]),

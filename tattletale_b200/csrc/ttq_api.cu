@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "ttq_internal.cuh"
+#include "ttq_paged.cuh"
 
 using namespace ttq;
 
@@ -73,6 +74,16 @@ struct ttq_moe {
     float *part;                   // tensor-memory GEMM: partial sums of row tiles that are cut over several CTAs
     size_t part_bytes;
     int64_t n_arrivals;            // its counters (MoeRouting::arrivals)
+};
+
+// Paged attention: head geometry and the workspace of one call.
+struct ttq_paged {
+    ttq_ctx *ctx;
+    int dt, hq, hkv, d, page_size, page_shift;
+    int64_t max_seqs, max_tokens, max_prefix_tokens;
+    void *ws;            // one allocation: arrival counters, partial results, the shared prefix's results
+    unsigned *counters;
+    float *part, *pre_o, *pre_lse;
 };
 
 namespace {
@@ -1090,6 +1101,10 @@ ttq_status ttq_device_status(ttq_ctx *ctx, void *stream) {
     int host = 0;
     TTQ_CUDA(ctx, cudaMemcpyAsync(&host, ctx->dev_status, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     TTQ_CUDA(ctx, cudaStreamSynchronize((cudaStream_t)stream));
+    if (host == PAGED_BAD_INDEX) {  // no wait was given up: nothing to clear but the flag
+        TTQ_CUDA(ctx, cudaMemsetAsync(ctx->dev_status, 0, sizeof(int), (cudaStream_t)stream));
+        return fail(ctx, TTQ_ERR_SHAPE, "a page id or position was outside the paged cache; results of that call are invalid");
+    }
     if (host != 0) {
         ctx->host_status[0] = 0;
         cudaMemsetAsync(ctx->dev_status, 0, sizeof(int), (cudaStream_t)stream);
@@ -1544,6 +1559,238 @@ ttq_status ttq_decode_attention(ttq_ctx *ctx, const void *q_dev, const void *k_c
                                             (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "decode attention launch");
     ctx->launches += 2;
+    return TTQ_OK;
+}
+
+// ---- paged cache ----------------------------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+constexpr int64_t PAGED_MAX_SEQS = 1 << 20;
+
+// Makes the context's device current for the duration of a call.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t err;
+    explicit DeviceScope(int device) {
+        err = cudaGetDevice(&before);
+        if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+typedef CUresult (*TensorMapEncode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                    const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+TensorMapEncode tensor_map_encode() {
+    static const TensorMapEncode fn = []() -> TensorMapEncode {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+        return reinterpret_cast<TensorMapEncode>(p);
+    }();
+    return fn;
+}
+
+// Map of the pages as (element, slot, kv head, page), copied in boxes of 64 elements x `slots` slots, 128-byte swizzle.
+ttq_status paged_map(ttq_ctx *ctx, const ttq_paged *p, const ttq_kv_pages *kv, void *base, int slots, CUtensorMap *map) {
+    const TensorMapEncode encode = tensor_map_encode();
+    if (!encode) return fail(ctx, TTQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {(cuuint64_t)p->d, (cuuint64_t)p->page_size, (cuuint64_t)p->hkv, (cuuint64_t)kv->n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)kv->token_stride * 2, (cuuint64_t)kv->head_stride * 2, (cuuint64_t)kv->page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)slots, 1, 1}, unit[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, p->dt == TTQ_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box,
+                              unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ctx, TTQ_ERR_SHAPE, "the pages' strides cannot be mapped (cuTensorMapEncodeTiled: %d)", (int)r);
+    return TTQ_OK;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Checks of the pages and the batch that append and attention share; fills `a`.
+ttq_status paged_args(ttq_ctx *ctx, const ttq_paged *p, const ttq_kv_pages *kv, const ttq_paged_batch *bt, PagedArgs *a) {
+    if (!p || !kv || !bt) return fail(ctx, TTQ_ERR_INVALID_ARG, "plan, pages or batch is NULL");
+    if (p->ctx != ctx) return fail(ctx, TTQ_ERR_INVALID_ARG, "plan belongs to another context");
+    if (bt->n_seqs < 0 || bt->n_tokens < 0 || bt->max_q < 0 || bt->table_len < 0 || bt->prefix_len < 0) return fail(ctx, TTQ_ERR_SHAPE, "negative size");
+    if (bt->n_seqs > p->max_seqs) return fail(ctx, TTQ_ERR_LIMIT, "n_seqs=%lld exceeds max_seqs=%lld of the plan", (long long)bt->n_seqs, (long long)p->max_seqs);
+    if (bt->n_tokens > p->max_tokens)
+        return fail(ctx, TTQ_ERR_LIMIT, "n_tokens=%lld exceeds max_tokens=%lld of the plan", (long long)bt->n_tokens, (long long)p->max_tokens);
+    if (bt->n_seqs == 0 || bt->n_tokens == 0) return TTQ_OK;
+    if (!bt->q_start_dev || !bt->kv_len_dev || (bt->table_len > 0 && !bt->block_table_dev))
+        return fail(ctx, TTQ_ERR_INVALID_ARG, "q_start, kv_len or block_table is NULL");
+    if (bt->ld_table < bt->table_len) return fail(ctx, TTQ_ERR_SHAPE, "ld_table is smaller than table_len");
+    if (bt->prefix_len > 0 && !bt->prefix_table_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "prefix_table is NULL");
+    if (bt->prefix_len > INT32_MAX || bt->table_len > INT32_MAX / p->page_size)
+        return fail(ctx, TTQ_ERR_LIMIT, "prefix_len or table_len: positions are 32-bit");
+    if (!kv->k_dev || !kv->v_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "k or v pages pointer is NULL");
+    if (!aligned16(kv->k_dev) || !aligned16(kv->v_dev)) return fail(ctx, TTQ_ERR_INVALID_ARG, "the pages must be 16-byte aligned");
+    if (kv->n_pages < 1 || kv->n_pages > INT32_MAX - 1) return fail(ctx, TTQ_ERR_SHAPE, "n_pages=%lld out of range", (long long)kv->n_pages);
+    const int64_t st[3] = {kv->token_stride, kv->head_stride, kv->page_stride};
+    for (int64_t s : st)
+        if (s <= 0 || s % 8 || s >= (1ll << 39)) return fail(ctx, TTQ_ERR_SHAPE, "the pages' strides must be positive multiples of 8 elements below 2^39");
+    if (kv->token_stride < p->d || (p->hkv > 1 && kv->head_stride < p->d)) return fail(ctx, TTQ_ERR_SHAPE, "slots or heads of a page overlap");
+    memset(a, 0, sizeof(*a));
+    a->n_tokens = bt->n_tokens;
+    a->B = (int)bt->n_seqs;
+    a->q_start = bt->q_start_dev;
+    a->kv_len = bt->kv_len_dev;
+    a->block_table = bt->block_table_dev;
+    a->ld_table = bt->ld_table;
+    a->table_len = (int)bt->table_len;
+    a->prefix_len = (int)bt->prefix_len;
+    a->prefix_table = bt->prefix_table_dev;
+    a->hq = p->hq;
+    a->hkv = p->hkv;
+    a->G = p->hq / p->hkv;
+    a->page_shift = p->page_shift;
+    a->n_pages = (int)kv->n_pages;
+    a->status = ctx->dev_status;
+    a->sms = ctx->sms;
+    return TTQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+ttq_status ttq_paged_create(ttq_ctx *ctx, ttq_dtype dt, int32_t hq, int32_t hkv, int32_t d, int32_t page_size, int64_t max_seqs,
+                            int64_t max_tokens, int64_t max_prefix_tokens, ttq_paged **out) {
+    if (!ctx) return TTQ_ERR_INVALID_ARG;
+    if (!out) return fail(ctx, TTQ_ERR_INVALID_ARG, "out is NULL");
+    *out = nullptr;
+    if (dt != TTQ_DT_BF16 && dt != TTQ_DT_F16) return fail(ctx, TTQ_ERR_INVALID_ARG, "dtype must be bf16 or f16");
+    if (hq <= 0 || hkv <= 0 || hq % hkv || hq > 1024) return fail(ctx, TTQ_ERR_SHAPE, "bad head counts (hq=%d hkv=%d)", hq, hkv);
+    if (d != 64 && d != 128) return fail(ctx, TTQ_ERR_UNSUPPORTED, "paged attention serves head dimensions 64 and 128");
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+        return fail(ctx, TTQ_ERR_UNSUPPORTED, "page_size=%d: a power of two from 16 to 1024", page_size);
+    if (max_seqs < 1 || max_seqs > PAGED_MAX_SEQS) return fail(ctx, TTQ_ERR_SHAPE, "max_seqs=%lld out of range 1..2^20", (long long)max_seqs);
+    if (max_tokens < 1 || max_tokens > INT32_MAX / hq) return fail(ctx, TTQ_ERR_SHAPE, "max_tokens=%lld out of range", (long long)max_tokens);
+    if (max_prefix_tokens < 0 || max_prefix_tokens > max_tokens) return fail(ctx, TTQ_ERR_SHAPE, "max_prefix_tokens out of range 0..max_tokens");
+    DeviceScope dev(ctx->device);
+    if (dev.err != cudaSuccess) return cuda_fail(ctx, dev.err, "cudaSetDevice");
+    ttq_paged *p = new (std::nothrow) ttq_paged();
+    if (!p) return fail(ctx, TTQ_ERR_OOM, "host allocation failed");
+    p->ctx = ctx; p->dt = dt; p->hq = hq; p->hkv = hkv; p->d = d; p->page_size = page_size;
+    p->max_seqs = max_seqs; p->max_tokens = max_tokens; p->max_prefix_tokens = max_prefix_tokens;
+    while ((1 << p->page_shift) < page_size) p->page_shift++;
+    auto up256 = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t b_cnt = up256((size_t)paged_counters(ctx->sms) * sizeof(unsigned)), b_part = up256((size_t)paged_part_floats(d, ctx->sms) * sizeof(float));
+    const size_t rows = (size_t)max_prefix_tokens * hq;
+    const size_t b_o = up256(rows * d * sizeof(float)), b_lse = up256(rows * sizeof(float));
+    cudaError_t e = cudaMalloc(&p->ws, b_cnt + b_part + b_o + b_lse);
+    if (e == cudaSuccess) e = cudaMemset(p->ws, 0, b_cnt);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {
+        cudaFree(p->ws);
+        delete p;
+        return cuda_fail(ctx, e, "cudaMalloc(paged attention workspace)");
+    }
+    uint8_t *q = reinterpret_cast<uint8_t *>(p->ws);
+    p->counters = reinterpret_cast<unsigned *>(q); q += b_cnt;
+    p->part = reinterpret_cast<float *>(q); q += b_part;
+    p->pre_o = reinterpret_cast<float *>(q); q += b_o;
+    p->pre_lse = reinterpret_cast<float *>(q);
+    *out = p;
+    return TTQ_OK;
+}
+
+ttq_status ttq_paged_destroy(ttq_paged *p) {
+    if (!p) return TTQ_OK;
+    DeviceScope dev(p->ctx->device);
+    cudaFree(p->ws);
+    delete p;
+    return TTQ_OK;
+}
+
+ttq_status ttq_paged_append(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *kv, const ttq_paged_batch *bt, const void *qkv_dev, int64_t ld_qkv,
+                            const void *q_norm_dev, const void *k_norm_dev, float eps, const void *cos_dev, const void *sin_dev,
+                            ttq_dtype rope_dt, int64_t n_rope, void *q_out_dev, int64_t ld_q, void *stream) {
+    if (!ctx) return TTQ_ERR_INVALID_ARG;
+    PagedArgs a;
+    const ttq_status s = paged_args(ctx, p, kv, bt, &a);
+    if (s != TTQ_OK) return s;
+    if (bt->n_seqs == 0 || bt->n_tokens == 0) return TTQ_OK;
+    if (!qkv_dev || !cos_dev || !sin_dev || !q_out_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "a device pointer is NULL");
+    if (rope_dt != TTQ_DT_F32 && (int)rope_dt != p->dt) return fail(ctx, TTQ_ERR_INVALID_ARG, "cos and sin must be f32 or of the plan's dtype");
+    if (n_rope < 1 || n_rope > INT32_MAX) return fail(ctx, TTQ_ERR_SHAPE, "n_rope=%lld out of range", (long long)n_rope);
+    if (ld_qkv < (int64_t)(p->hq + 2 * p->hkv) * p->d || ld_q < (int64_t)p->hq * p->d || ld_qkv % 8 || ld_q % 8)
+        return fail(ctx, TTQ_ERR_SHAPE, "ld_qkv and ld_q must be multiples of 8 and hold the heads of a row");
+    if (!aligned16(qkv_dev) || !aligned16(cos_dev) || !aligned16(sin_dev) || !aligned16(q_out_dev) || !aligned16(q_norm_dev) || !aligned16(k_norm_dev))
+        return fail(ctx, TTQ_ERR_INVALID_ARG, "pointers must be 16-byte aligned");
+    DeviceScope dev(ctx->device);
+    if (dev.err != cudaSuccess) return cuda_fail(ctx, dev.err, "cudaSetDevice");
+    PagedAppend ap;
+    ap.qkv = qkv_dev; ap.q_norm = q_norm_dev; ap.k_norm = k_norm_dev; ap.cosv = cos_dev; ap.sinv = sin_dev;
+    ap.q_out = q_out_dev; ap.k = kv->k_dev; ap.v = kv->v_dev;
+    ap.ld_qkv = ld_qkv; ap.ld_q = ld_q; ap.page_stride = kv->page_stride; ap.head_stride = kv->head_stride; ap.token_stride = kv->token_stride;
+    ap.eps = eps; ap.dt = p->dt; ap.rope_dt = rope_dt; ap.n_rope = (int)n_rope; ap.d = p->d;
+    const cudaError_t e = launch_paged_append(a, ap, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "paged append launch");
+    ctx->launches++;
+    return TTQ_OK;
+}
+
+ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *kv, const ttq_paged_batch *bt, const void *q_dev, int64_t ld_q,
+                               float scale, int64_t window, int64_t sinks, void *out_dev, int64_t ld_out, void *stream) {
+    if (!ctx) return TTQ_ERR_INVALID_ARG;
+    PagedArgs a;
+    const ttq_status s = paged_args(ctx, p, kv, bt, &a);
+    if (s != TTQ_OK) return s;
+    if (window < 0 || sinks < 0) return fail(ctx, TTQ_ERR_SHAPE, "window and sinks must not be negative");
+    if (!(scale > 0.f) || scale > 1e30f) return fail(ctx, TTQ_ERR_INVALID_ARG, "scale must be positive and finite");
+    if (bt->n_seqs == 0 || bt->n_tokens == 0) return TTQ_OK;
+    if (!q_dev || !out_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "q or out pointer is NULL");
+    if (ld_q < (int64_t)p->hq * p->d || ld_out < (int64_t)p->hq * p->d || ld_q % 8 || ld_out % 8)
+        return fail(ctx, TTQ_ERR_SHAPE, "ld_q and ld_out must be multiples of 8 and hold the heads of a row");
+    if (!aligned16(q_dev) || !aligned16(out_dev)) return fail(ctx, TTQ_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
+    if (bt->prefix_len > 0 && bt->n_tokens > p->max_prefix_tokens)
+        return fail(ctx, TTQ_ERR_LIMIT, "n_tokens=%lld exceeds max_prefix_tokens=%lld of the plan", (long long)bt->n_tokens, (long long)p->max_prefix_tokens);
+    DeviceScope dev(ctx->device);
+    if (dev.err != cudaSuccess) return cuda_fail(ctx, dev.err, "cudaSetDevice");
+    a.q = q_dev; a.ld_q = ld_q; a.out = out_dev; a.ld_out = ld_out;
+    a.window = window > INT32_MAX ? 0 : (int)window;
+    a.sinks = sinks > INT32_MAX ? INT32_MAX : (int)sinks;
+    a.scale2 = scale * 1.4426950408889634f;
+    a.part = p->part;
+    a.counters = p->counters;
+    // the shared prefix for all rows first, then every sequence's own keys, which take the prefix's results in
+    for (int pass = bt->prefix_len > 0 ? 0 : 1; pass < 2; pass++) {
+        a.prefix_pass = pass == 0;
+        a.pre_o = bt->prefix_len > 0 ? p->pre_o : nullptr;
+        a.pre_lse = p->pre_lse;
+        PagedMaps maps;
+        ttq_status ms = paged_map(ctx, p, kv, kv->k_dev, 16, &maps.k);
+        if (ms == TTQ_OK) ms = paged_map(ctx, p, kv, kv->v_dev, 16, &maps.v);
+        if (ms != TTQ_OK) return ms;
+        const cudaError_t e = launch_paged_rows(a, p->dt, p->d, maps, (cudaStream_t)stream);
+        if (e != cudaSuccess) return cuda_fail(ctx, e, "paged attention launch");
+        ctx->launches++;
+    }
+    return TTQ_OK;
+}
+
+ttq_status ttq_sample(ttq_ctx *ctx, const void *logits_dev, ttq_dtype dt, int64_t M, int64_t V, int64_t ld, const ttq_sampling *sp,
+                      const float *u_dev, int64_t *ids_dev, void *stream) {
+    if (!ctx) return TTQ_ERR_INVALID_ARG;
+    if (M < 0 || V <= 0 || ld < V) return fail(ctx, TTQ_ERR_SHAPE, "bad size (M=%lld V=%lld ld=%lld)", (long long)M, (long long)V, (long long)ld);
+    if (V > (1 << 18)) return fail(ctx, TTQ_ERR_LIMIT, "V=%lld exceeds 2^18", (long long)V);
+    if (M > INT32_MAX / 16) return fail(ctx, TTQ_ERR_LIMIT, "M=%lld exceeds the grid", (long long)M);
+    if (!sp) return fail(ctx, TTQ_ERR_INVALID_ARG, "sampling settings are NULL");
+    if (!valid_dt(dt)) return fail(ctx, TTQ_ERR_INVALID_ARG, "unknown dtype %d", (int)dt);
+    if (M == 0) return TTQ_OK;
+    if (!logits_dev || !u_dev || !ids_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "a device pointer is NULL");
+    if ((reinterpret_cast<uintptr_t>(logits_dev) & (dt_size(dt) - 1)) || (reinterpret_cast<uintptr_t>(ids_dev) & 7))
+        return fail(ctx, TTQ_ERR_INVALID_ARG, "logits or ids are not aligned to their type");
+    DeviceScope dev(ctx->device);
+    if (dev.err != cudaSuccess) return cuda_fail(ctx, dev.err, "cudaSetDevice");
+    const cudaError_t e = launch_sample(logits_dev, dt, M, (int)V, ld, *sp, u_dev, ids_dev, ctx->sms, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "sampling launch");
+    ctx->launches++;
     return TTQ_OK;
 }
 

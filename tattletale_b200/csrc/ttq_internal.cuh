@@ -286,6 +286,10 @@ int64_t decode_attention_scratch_floats(int64_t B, int hq, int64_t n_ctx);
 cudaError_t launch_decode_attention(const void *q, const void *k_cache, const void *v_cache, int dt, int64_t B, int hq, int hkv, int d,
                                     int64_t ctx_len, int64_t n_ctx, float *part, void *out, cudaStream_t st);
 
+// Next tokens from logits (ttq_sample.cu).
+cudaError_t launch_sample(const void *logits, int dt, int64_t M, int V, int64_t ld, const ttq_sampling &s, const float *u, int64_t *ids, int sms,
+                          cudaStream_t st);
+
 // Routing and combination of a mixture-of-experts layer (ttq_moe.cu).
 struct MoeRouting {
     unsigned *arrivals;                // [n_arrivals] counters of the grouped GEMM; they and the counts behind them are cleared per call

@@ -36,6 +36,21 @@ type
     y_dt*: int32
     ldy*: int64
 
+  TtqPaged* {.importc: "ttq_paged", header: "ttq.h", incompleteStruct.} = object
+  TtqKvPages* {.importc: "ttq_kv_pages", header: "ttq.h", bycopy.} = object
+    k_dev*, v_dev*: pointer
+    n_pages*, page_stride*, head_stride*, token_stride*: int64
+  TtqPagedBatch* {.importc: "ttq_paged_batch", header: "ttq.h", bycopy.} = object
+    n_seqs*, n_tokens*, max_q*: int64
+    q_start_dev*, kv_len_dev*, block_table_dev*: ptr int32
+    table_len*, ld_table*, prefix_len*: int64
+    prefix_table_dev*: ptr int32
+  TtqSampling* {.importc: "ttq_sampling", header: "ttq.h", bycopy.} = object
+    temperature_dev*, top_p_dev*, min_p_dev*: ptr cfloat
+    top_k_dev*: ptr int32
+    temperature*, top_p*, min_p*: cfloat
+    top_k*: int32
+
 proc ttq_init(device: cint, ctx: ptr ptr TtqCtx): TtqStatus {.importc, cdecl, header: "ttq.h".}
 proc ttq_destroy(ctx: ptr TtqCtx): TtqStatus {.importc, cdecl, header: "ttq.h".}
 proc ttq_last_error(ctx: ptr TtqCtx): cstring {.importc, cdecl, header: "ttq.h".}
@@ -109,6 +124,18 @@ proc ttq_moe_destroy(moe: ptr TtqMoe): TtqStatus {.importc, cdecl, header: "ttq.
 proc ttq_moe_forward(ctx: ptr TtqCtx, moe: ptr TtqMoe, x: pointer, xDt: TtqDtype, T, ldx: int64, topkIds: ptr int32,
                      topkWeights: ptr cfloat, y: pointer, yDt: TtqDtype, ldy: int64,
                      stream: pointer): TtqStatus {.importc, cdecl, header: "ttq.h".}
+# paged cache: append with rotation, attention of a ragged batch; sampling
+proc ttq_paged_create(ctx: ptr TtqCtx, dt: TtqDtype, hq, hkv, d, pageSize: int32, maxSeqs, maxTokens, maxPrefixTokens: int64,
+                      plan: ptr ptr TtqPaged): TtqStatus {.importc, cdecl, header: "ttq.h".}
+proc ttq_paged_destroy(plan: ptr TtqPaged): TtqStatus {.importc, cdecl, header: "ttq.h".}
+proc ttq_paged_append(ctx: ptr TtqCtx, plan: ptr TtqPaged, kv: ptr TtqKvPages, batch: ptr TtqPagedBatch, qkv: pointer, ldQkv: int64,
+                      qNorm, kNorm: pointer, eps: cfloat, cosv, sinv: pointer, ropeDt: TtqDtype, nRope: int64, qOut: pointer,
+                      ldQ: int64, stream: pointer): TtqStatus {.importc, cdecl, header: "ttq.h".}
+proc ttq_paged_attention(ctx: ptr TtqCtx, plan: ptr TtqPaged, kv: ptr TtqKvPages, batch: ptr TtqPagedBatch, q: pointer, ldQ: int64,
+                         scale: cfloat, window, sinks: int64, outp: pointer, ldOut: int64,
+                         stream: pointer): TtqStatus {.importc, cdecl, header: "ttq.h".}
+proc ttq_sample(ctx: ptr TtqCtx, logits: pointer, dt: TtqDtype, M, V, ld: int64, sampling: ptr TtqSampling, u: ptr cfloat,
+                ids: ptr int64, stream: pointer): TtqStatus {.importc, cdecl, header: "ttq.h".}
 # introspection
 proc ttq_trace_read(ctx: ptr TtqCtx, outp: ptr uint64, maxEntries: int64, nEntries: ptr int64): TtqStatus {.importc, cdecl, header: "ttq.h".}
 proc ttq_launch_count(ctx: ptr TtqCtx): int64 {.importc, cdecl, header: "ttq.h".}
