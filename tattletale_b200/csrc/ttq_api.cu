@@ -1763,11 +1763,16 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
         a.prefix_pass = pass == 0;
         a.pre_o = bt->prefix_len > 0 ? p->pre_o : nullptr;
         a.pre_lse = p->pre_lse;
+        // few rows per kv head: the memory-bound kernel; from 17 on the tensor-memory kernel
+        const int64_t most = a.prefix_pass || bt->max_q == 0 ? bt->n_tokens : bt->max_q;
+        const bool few = most * a.G <= 16;
+        const int slots = few ? 16 : (p->page_size < 128 ? p->page_size : 128);
         PagedMaps maps;
-        ttq_status ms = paged_map(ctx, p, kv, kv->k_dev, 16, &maps.k);
-        if (ms == TTQ_OK) ms = paged_map(ctx, p, kv, kv->v_dev, 16, &maps.v);
+        ttq_status ms = paged_map(ctx, p, kv, kv->k_dev, slots, &maps.k);
+        if (ms == TTQ_OK) ms = paged_map(ctx, p, kv, kv->v_dev, slots, &maps.v);
         if (ms != TTQ_OK) return ms;
-        const cudaError_t e = launch_paged_rows(a, p->dt, p->d, maps, (cudaStream_t)stream);
+        const cudaError_t e = few ? launch_paged_rows(a, p->dt, p->d, maps, (cudaStream_t)stream)
+                                  : launch_paged_tc(a, p->dt, p->d, maps, slots, (cudaStream_t)stream);
         if (e != cudaSuccess) return cuda_fail(ctx, e, "paged attention launch");
         ctx->launches++;
     }

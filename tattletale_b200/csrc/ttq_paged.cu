@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     grid_launch_dependents();
     grid_dependency_wait();
 
-    const PagedShare sh = paged_share<ROWS_THREADS>(a, red, [&](int b, int min_pos) -> int64_t {
+    const PagedShare sh = paged_share<ROWS_THREADS>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
+        if (!ok) return 0;
         const PagedSeq s = paged_seq(a, b, min_pos);
         return s.n > 0 ? (int64_t)rows_items(a, s.n) * paged_units<ROWS_UNIT>(s).count : 0;
     });
@@ -552,7 +553,10 @@ cudaError_t launch_append_t(const AppendArgs &args, int per_cta, cudaStream_t st
 
 }  // namespace
 
-int64_t paged_part_floats(int d, int sms) { return (int64_t)2 * PAGED_ROWS16_CTAS * sms * ROWS_TILE * (d + 2); }
+int64_t paged_part_floats(int d, int sms) {
+    const int64_t rows = (int64_t)2 * PAGED_ROWS16_CTAS * sms * ROWS_TILE * (d + 2), tc = paged_tc_part_floats(d, sms);
+    return rows > tc ? rows : tc;
+}
 int64_t paged_counters(int sms) { return PAGED_ROWS16_CTAS * sms; }
 
 cudaError_t launch_paged_rows(const PagedArgs &a, int dt, int d, const PagedMaps &maps, cudaStream_t st) {

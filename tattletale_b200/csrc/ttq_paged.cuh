@@ -131,7 +131,7 @@ struct PagedShare {
     int min_pos;     // prefix pass: smallest position of any token
 };
 
-// Called by all THREADS of the CTA.  `cost(b)`: units of sequence b.  red: shared, at least THREADS / 32 + 4 int64.
+// Called by all THREADS of the CTA.  `cost(b, ok, min_pos)`: units of sequence b (ok false: none), whole warps at a time.  red: shared, at least THREADS / 32 + 4 int64.
 template <int THREADS, class Cost>
 __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *red, Cost &&cost) {
     constexpr int W = THREADS / 32;
@@ -158,7 +158,8 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
         int64_t running = 0;
         for (int base = 0; base < nb; base += THREADS) {
             const int b = base + tid;
-            int64_t c = b < nb ? cost(b, sh.min_pos) : 0, incl = c;
+            const int64_t c = cost(b, b < nb, sh.min_pos);
+            int64_t incl = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -288,6 +289,8 @@ struct PagedMaps {
 // One launch of a pass (own keys, or the shared prefix's).
 cudaError_t launch_paged_rows(const PagedArgs &a, int dt, int d, const PagedMaps &maps, cudaStream_t st);
 constexpr int PAGED_ROWS16_CTAS = 2;  // resident CTAs per SM of the kernel for few rows
+cudaError_t launch_paged_tc(const PagedArgs &a, int dt, int d, const PagedMaps &maps, int box_rows, cudaStream_t st);
+int64_t paged_tc_part_floats(int d, int sms);
 // Workspace of a plan: partial results in floats, arrival counters.
 int64_t paged_part_floats(int d, int sms);
 int64_t paged_counters(int sms);

@@ -1,0 +1,668 @@
+// Attention over a paged cache on the tensor cores (tcgen05): prompts, pieces of prompts, and rows of a whole batch against a shared
+// prefix.
+//
+// An item is a tile of up to 256 rows (tokens x query heads of one kv head), walked in units of 128 keys.  Its two halves of 128
+// rows are two streams that take turns: while the softmax of one runs on the CUDA cores, the tensor core multiplies for the other.
+//   S = Q K^T     128 x 128, Q and K in shared memory (K-major, 128-byte swizzle), S in tensor memory
+//   softmax       one thread per row: 128 scores from tensor memory, running maximum and sum in registers, weights in the 16-bit type
+//                 back into the columns that the scores had
+//   O += P V      P from tensor memory, V as it lies in its pages (keys as rows: the transposed operand form), O in tensor memory
+// An item of 128 rows or fewer gives both streams the same rows and every other unit of keys; the two results meet in tensor
+// memory, whose lanes the warps of both streams reach.  Tensor memory is full: 2 x 128 columns of scores, 2 x d of output.
+//
+// Warps 0-3 and 4-7: softmax of the two streams, and their rows' queries and results.  Warp 8 issues the products, warp 9 the
+// tiled copies of the pages into a ring of slots.  Products of one CTA execute in the order of issue, so the scores of unit
+// i + 1 may follow the product that reads the weights of unit i from the same columns, and a full score buffer means that
+// the output accumulator is at rest: the softmax warps rescale it in place, which they do only when the maximum has grown by 2^8.
+#include <climits>
+
+#include "ttq_devutil.cuh"
+#include "ttq_paged.cuh"
+
+namespace ttq {
+namespace {
+
+constexpr int TC_UNIT = 128;       // keys per unit
+constexpr int TC_ROWS = 128;       // rows per stream
+constexpr int TC_ITEM_ROWS = 2 * TC_ROWS;
+constexpr int TC_MMA_WARP = 8, TC_TMA_WARP = 9;
+constexpr int TC_THREADS = 320, TC_SOFTMAX_THREADS = 256;
+
+template <int D>
+struct TcCfg {
+    static constexpr int HALVES = D / 64;
+    static constexpr int HALF_BYTES = 128 * 128;               // 128 rows x 64 elements
+    static constexpr int SLOT_BYTES = HALVES * HALF_BYTES;     // a unit of K or of V; a stream's queries
+    static constexpr int SLOTS = D == 128 ? 5 : 10;
+    static constexpr int S_COL = 0, O_COL = 256;               // streams 128 columns, resp. D columns apart
+    // shared memory: queries, ring, then barriers and exchange
+    static constexpr int RING_AT = 2 * SLOT_BYTES;
+    static constexpr int BAR_AT = RING_AT + SLOTS * SLOT_BYTES;
+    static constexpr int N_BARS = 2 * SLOTS + 8 + 1;
+    static constexpr int ML_AT = BAR_AT + (N_BARS * 8 + 15) / 16 * 16;
+    static constexpr int MISC_AT = ML_AT + 2 * TC_ROWS * 8;
+    static constexpr int SMEM = MISC_AT + 16 * 8 + 16;
+};
+
+template <bool BF16>
+__host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_rows_are_k) {
+    return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (b_rows_are_k ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// V: element (key, column) of a unit is row `key` of 128 bytes in the half of its column.  As the transposed operand: 8-key groups
+// 1024 bytes apart (stride offset), 64-column blocks a half apart (leading offset), 128-byte swizzle.
+__device__ __forceinline__ uint64_t tc_desc_v(uint32_t addr, int half_bytes) {
+    const uint32_t lo = ((addr & 0x3ffffu) >> 4) | ((uint32_t)(half_bytes >> 4) << 16);
+    const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return ((uint64_t)hi << 32) | lo;
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32 columns of this thread's lane
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, float *v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+// the wait, through which the loaded registers pass
+__device__ __forceinline__ void tc_ld_wait32(float *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                   "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
+                   "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                   "+f"(v[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+        "%30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+        "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&t);
+    } else {
+        const __half2 t = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&t);
+    }
+}
+
+// Row tile rt of a sequence: its rows, and the keys that any of them sees.
+struct TcItem {
+    PagedSeq k;      // key_end, lo, sink of this item (the rest as the sequence's)
+    PagedUnits u;
+    int rows;        // valid rows, from row 256 rt on
+};
+__device__ __forceinline__ int tc_tiles(const PagedArgs &a, int n) { return (n * a.G + TC_ITEM_ROWS - 1) / TC_ITEM_ROWS; }
+__device__ __forceinline__ TcItem tc_item(const PagedArgs &a, const PagedSeq &s, int rt) {
+    TcItem it;
+    it.k = s;
+    it.rows = min(TC_ITEM_ROWS, s.n * a.G - rt * TC_ITEM_ROWS);
+    if (!a.prefix_pass) {
+        const int i0 = rt * TC_ITEM_ROWS / a.G, i1 = (rt * TC_ITEM_ROWS + it.rows - 1) / a.G;  // first and last token
+        it.k.key_end = max(0, min(s.key_end, s.pos0 + i1 + 1 - a.prefix_len));
+        it.k.lo = it.k.sink = 0;
+        if (a.window > 0) {
+            it.k.lo = max(0, min(it.k.key_end, s.pos0 + i0 - a.window + 1 - a.prefix_len));
+            it.k.sink = max(0, min(it.k.lo, a.sinks - a.prefix_len));
+        }
+    }
+    it.u = paged_units<TC_UNIT>(it.k);
+    return it;
+}
+// Units of one kv head's items of a sequence, by the whole warp (`s`: the same in all lanes).
+__device__ __forceinline__ int64_t tc_seq_units(const PagedArgs &a, const PagedSeq &s, int lane) {
+    const int nt = tc_tiles(a, s.n);
+    int64_t sum = 0;
+    for (int rt = lane; rt < nt; rt += 32) sum += tc_item(a, s, rt).u.count;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
+// Walk through the items of consecutive sequences: kv heads, and their row tiles.  Every warp walks for itself.
+struct TcWalk {
+    PagedSeq s;
+    TcItem it;
+    int b, head, rt, nt;
+    int unit;        // of the item
+    int64_t pos;     // number of that unit
+
+    __device__ __forceinline__ void enter(const PagedArgs &a, int min_pos) {
+        const int nb = a.prefix_pass ? 1 : a.B;
+        for (; b < nb; b++) {
+            s = paged_seq(a, b, min_pos);
+            if (s.n > 0) break;
+        }
+        nt = tc_tiles(a, s.n);
+        head = rt = unit = 0;
+        it = tc_item(a, s, 0);
+    }
+    // to the unit `off` units behind the sequence's first (the whole warp)
+    __device__ __forceinline__ void start(const PagedArgs &a, const PagedShare &sh, int lane) {
+        b = sh.b;
+        enter(a, sh.min_pos);
+        int64_t off = sh.u0 - sh.seq_u;
+        const int64_t per_head = tc_seq_units(a, s, lane);
+        head = (int)(off / per_head);
+        off -= head * per_head;
+        for (int base = 0;; base += 32) {
+            const int c = base + lane < nt ? tc_item(a, s, base + lane).u.count : 0;
+            int incl = c;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, off < incl);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                rt = base + l;
+                unit = (int)off - __shfl_sync(0xffffffffu, incl - c, l);
+                break;
+            }
+            if (base + 32 >= nt) break;  // (not reached)
+            off -= __shfl_sync(0xffffffffu, incl, 31);
+        }
+        it = tc_item(a, s, rt);
+        pos = sh.u0;
+    }
+    // units of this item in the share
+    __device__ __forceinline__ int here(const PagedShare &sh) const {
+        const int64_t left = sh.u1 - pos;
+        return (int)(left < it.u.count - unit ? left : it.u.count - unit);
+    }
+    __device__ __forceinline__ void next(const PagedArgs &a, const PagedShare &sh) {
+        pos += here(sh);
+        unit = 0;
+        if (pos >= sh.u1) return;
+        if (++rt == nt) {
+            rt = 0;
+            if (++head == a.hkv) {
+                b++;
+                enter(a, sh.min_pos);
+                return;
+            }
+        }
+        it = tc_item(a, s, rt);
+    }
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                                 const __grid_constant__ CUtensorMap vmap, int box_rows) {
+    using C = TcCfg<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = smem_u32(smem);
+    const uint32_t bars = base + C::BAR_AT;
+    const uint32_t kv_full = bars, kv_empty = kv_full + 8 * C::SLOTS, q_full = kv_empty + 8 * C::SLOTS, s_full = q_full + 16, p_full = s_full + 16,
+                   o_full = p_full + 16, fix_bar = o_full + 16;
+    float2 *ml = reinterpret_cast<float2 *>(smem + C::ML_AT);
+    int64_t *red = reinterpret_cast<int64_t *>(smem + C::MISC_AT);
+    volatile uint32_t *slot_word = reinterpret_cast<volatile uint32_t *>(smem + C::MISC_AT + 16 * 8);
+    volatile int *last_word = reinterpret_cast<volatile int *>(smem + C::MISC_AT + 16 * 8 + 4);
+    if (tid == 0) {
+        for (int i = 0; i < C::SLOTS; i++) {
+            mbar_init(kv_full + 8 * i, 1);
+            mbar_init(kv_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(q_full + 8 * i, 4);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 4);
+            mbar_init(o_full + 8 * i, 1);
+        }
+        mbar_init(fix_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const PagedShare sh = paged_share<TC_THREADS>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
+        PagedSeq s{};
+        if (ok) s = paged_seq(a, b, min_pos);
+        const int nt = ok ? tc_tiles(a, s.n) : 0;
+        int64_t units = 0;
+        if (nt <= 2)
+            for (int rt = 0; rt < nt; rt++) units += tc_item(a, s, rt).u.count;
+        // long prompts: the warp's lanes share the row tiles
+        for (unsigned many = __ballot_sync(0xffffffffu, nt > 2); many; many &= many - 1) {
+            const int l = __ffs(many) - 1;
+            PagedSeq t;
+            t.q0 = 0;
+            t.n = __shfl_sync(0xffffffffu, s.n, l);
+            t.pos0 = __shfl_sync(0xffffffffu, s.pos0, l);
+            t.key_end = __shfl_sync(0xffffffffu, s.key_end, l);
+            t.lo = __shfl_sync(0xffffffffu, s.lo, l);
+            t.sink = __shfl_sync(0xffffffffu, s.sink, l);
+            const int64_t sum = tc_seq_units(a, t, lane);
+            if (lane == l) units = sum;
+        }
+        return units * a.hkv;
+    });
+    if (sh.u0 >= sh.u1) return;
+    if (warp == TC_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)slot_word)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot_word;
+
+    TcWalk w;
+    w.start(a, sh, lane);
+
+    if (warp == TC_TMA_WARP) {
+        // ------------------------------------------------------------------------------------------ copies of the pages
+        int n = 0;  // slots filled so far
+        bool alive = true;
+        uint32_t fix_par = 0;
+        const int page_mask = (1 << a.page_shift) - 1;
+        // Unit i of the item into the next slot: boxes of box_rows slots of one page.  Boxes that no row sees are left out of K (their scores
+        // are masked) and are zeros in V; rows of a page that no row sees are zeroed in V, where a weight of zero would meet them.
+        int cache_first = -1, cache_b = -1, page_cache = 0;  // lane i: page number cache_first + i of the table of sequence cache_b
+        auto copy = [&](int i, bool is_v) {
+            const int k0 = paged_unit_index(w.it.u, i) * TC_UNIT;
+            const PagedSeq &k = w.it.k;
+            auto wanted = [&](int kb) { return kb < k.key_end && (kb + box_rows > k.lo || kb < k.sink); };
+            const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES, full = kv_full + 8 * (n % C::SLOTS);
+            if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
+            __syncwarp();
+            const bool fix = is_v && (k0 + TC_UNIT > k.key_end || (k0 < k.lo && k0 + TC_UNIT > k.sink));
+            const uint32_t bar = fix ? fix_bar : full;
+            int bytes = 0;
+            for (int r = 0; r < TC_UNIT; r += box_rows) bytes += is_v || wanted(k0 + r) ? box_rows * 128 * C::HALVES : 0;
+            if (elect_one()) {
+                if (bytes > 0) mbar_expect_tx(bar, (uint32_t)bytes);
+                else mbar_arrive(bar);
+            }
+            __syncwarp();
+            for (int r = 0; r < TC_UNIT; r += box_rows) {
+                const int kb = k0 + r;
+                int page = a.n_pages;  // beyond the last page: zeros
+                if (wanted(kb)) {
+                    const int idx = kb >> a.page_shift;
+                    if (cache_b != w.b || idx < cache_first || idx >= cache_first + 32) {
+                        cache_b = w.b;
+                        cache_first = idx;
+                        const int64_t last = (k.key_end - 1) >> a.page_shift;
+                        const int at = idx + lane;
+                        page_cache = -1;
+                        if (at <= last) page_cache = a.prefix_pass ? a.prefix_table[at] : a.block_table[(int64_t)w.b * a.ld_table + at];
+                    }
+                    page = __shfl_sync(0xffffffffu, page_cache, idx - cache_first);
+                    if (page < 0 || page >= a.n_pages) {
+                        page = a.n_pages;
+                        if (lane == 0) atomicOr(a.status, PAGED_BAD_INDEX);
+                    }
+                } else if (!is_v) {
+                    continue;
+                }
+                if (elect_one()) {
+#pragma unroll
+                    for (int h = 0; h < C::HALVES; h++)
+                        tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * 128), is_v ? &vmap : &kmap, 64 * h, kb & page_mask, w.head, page, bar);
+                }
+                __syncwarp();
+            }
+            if (fix) {
+                if (alive) alive = tc_wait(fix_bar, fix_par, a.status);
+                fix_par ^= 1u;
+                for (int r = lane / 8; r < TC_UNIT; r += 4) {
+                    const int key = k0 + r;
+                    if (key >= k.key_end || (key < k.lo && key >= k.sink)) {
+#pragma unroll
+                        for (int h = 0; h < C::HALVES; h++) sts128<0>(slot + (uint32_t)(h * C::HALF_BYTES + r * 128 + (lane & 7) * 16), 0u, 0u, 0u, 0u);
+                    }
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full);
+            }
+            n++;
+        };
+        while (true) {
+            const int m = w.here(sh), u0 = w.unit;
+            if (w.it.rows > TC_ROWS) {  // both streams take every unit
+                for (int i = 0; i < m; i++) {
+                    copy(u0 + i, false);
+                    copy(u0 + i, true);
+                }
+            } else {                    // stream 0 the even ones, stream 1 the odd ones
+                copy(u0, false);
+                if (m > 1) copy(u0 + 1, false);
+                for (int i = 0; i < m; i++) {
+                    copy(u0 + i, true);
+                    if (i + 2 < m) copy(u0 + i + 2, false);
+                }
+            }
+            w.next(a, sh);
+            if (w.pos >= sh.u1) break;
+        }
+        // the last copies have landed before the CTA may end: the product warp waits for every slot
+    } else if (warp == TC_MMA_WARP) {
+        // ------------------------------------------------------------------------------------------ products
+        bool alive = true;
+        int n = 0;                                   // slots consumed
+        uint32_t q_par = 0, p_par[2] = {0u, 0u};
+        constexpr uint32_t idesc_s = tc_idesc<BF16>(TC_UNIT, false), idesc_o = tc_idesc<BF16>(D, true);
+        auto slot_addr = [&](int i) { return base + C::RING_AT + (uint32_t)(i % C::SLOTS) * C::SLOT_BYTES; };
+        auto wait_slot = [&](int i) {
+            if (alive) alive = tc_wait(kv_full + 8 * (i % C::SLOTS), (uint32_t)((i / C::SLOTS) & 1), a.status);
+        };
+        // S of stream st from the K in slot i; `release`: the slot's last use
+        auto scores = [&](int st, int i, bool release) {
+            wait_slot(i);
+            __syncwarp();
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t d = tmem + C::S_COL + st * TC_UNIT;
+                const uint64_t qd = smem_desc_sw128(base + (uint32_t)st * C::SLOT_BYTES), kd = smem_desc_sw128(slot_addr(i));
+#pragma unroll
+                for (int h = 0; h < C::HALVES; h++)
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++)
+                        tc_mma_ss(d, qd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), kd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), idesc_s,
+                                  h + kk > 0 ? 1u : 0u);
+                umma_commit(s_full + 8 * st);
+                if (release) umma_commit(kv_empty + 8 * (i % C::SLOTS));
+            }
+            __syncwarp();
+        };
+        auto output = [&](int st, int i, bool first, bool last, bool release) {
+            if (alive) alive = tc_wait(p_full + 8 * st, p_par[st], a.status);
+            p_par[st] ^= 1u;
+            wait_slot(i);
+            __syncwarp();
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t d = tmem + C::O_COL + st * D, p = tmem + C::S_COL + st * TC_UNIT;
+                const uint64_t vd = tc_desc_v(slot_addr(i), C::HALF_BYTES);
+#pragma unroll
+                for (int kk = 0; kk < TC_UNIT / 16; kk++) tc_mma_ts(d, p + 8 * kk, vd + (uint64_t)(kk * 2048 >> 4), idesc_o, first && kk == 0 ? 0u : 1u);
+                if (release) umma_commit(kv_empty + 8 * (i % C::SLOTS));
+                if (last) umma_commit(o_full + 8 * st);
+            }
+            __syncwarp();
+        };
+        while (true) {
+            const int m = w.here(sh);
+            for (int st = 0; st < 2; st++)
+                if (alive) alive = tc_wait(q_full + 8 * st, q_par, a.status);
+            q_par ^= 1u;
+            if (w.it.rows > TC_ROWS) {
+                scores(0, n, false);
+                scores(1, n, true);
+                n++;
+                for (int i = 0; i < m; i++) {
+                    const bool more = i + 1 < m;
+                    output(0, n, i == 0, !more, false);
+                    if (more) scores(0, n + 1, false);
+                    output(1, n, i == 0, !more, true);
+                    if (more) scores(1, n + 1, true);
+                    n += more ? 2 : 1;
+                }
+            } else {
+                scores(0, n++, true);
+                if (m > 1) scores(1, n++, true);
+                for (int i = 0; i < m; i++) {
+                    output(i & 1, n++, i < 2, i + 2 >= m, true);
+                    if (i + 2 < m) scores(i & 1, n++, true);
+                }
+            }
+            w.next(a, sh);
+            if (w.pos >= sh.u1) break;
+        }
+    } else {
+        // ------------------------------------------------------------------------------------------ softmax: a thread per row
+        const int st = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the tensor memory's lanes
+        const uint32_t ts = tmem + C::S_COL + st * TC_UNIT + lanes, to = tmem + C::O_COL + st * D + lanes;
+        bool alive = true;
+        uint32_t s_par = 0, o_par = 0;
+        const int base_pos = a.prefix_pass ? 0 : a.prefix_len;
+        while (true) {
+            const int m = w.here(sh);
+            const bool joint = w.it.rows <= TC_ROWS;   // both streams work on the same rows
+            const int row0 = w.rt * TC_ITEM_ROWS + (joint ? 0 : st * TC_ROWS);
+            const int total_rows = w.s.n * a.G;
+            auto token_of = [&](int x, int &token, int &head) {
+                const int i = x / a.G;
+                token = w.s.q0 + i;
+                head = w.head * a.G + (x - i * a.G);
+            };
+            // queries into shared memory
+            for (int c = r; c < TC_ROWS * (D / 8); c += TC_ROWS) {
+                const int row = c / (D / 8), ch = c % (D / 8);
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (row0 + row < total_rows) {
+                    int token, head;
+                    token_of(row0 + row, token, head);
+                    v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (int64_t)token * a.ld_q + (int64_t)head * D + 8 * ch);
+                }
+                sts128<0>(base + (uint32_t)(st * C::SLOT_BYTES + (ch >> 3) * C::HALF_BYTES + row * 128 + (((ch & 7) ^ (row & 7)) << 4)), v.x, v.y, v.z, v.w);
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full + 8 * st);
+
+            const bool valid = row0 + r < total_rows;
+            int token = 0, head = 0, pos = -1;
+            if (valid) {
+                token_of(row0 + r, token, head);
+                pos = a.prefix_pass ? paged_row_pos(a, token) : w.s.pos0 + token - w.s.q0;
+            }
+            const int min_row = __reduce_min_sync(0xffffffffu, valid ? pos : INT_MAX), max_row = __reduce_max_sync(0xffffffffu, valid ? pos : -1);
+            float mx = -INFINITY, l = 0.f;  // running maximum of the scores (unscaled) and sum
+            const int step = joint ? 2 : 1;
+            for (int i = joint ? st : 0; i < m; i += step) {
+                const int k0 = paged_unit_index(w.it.u, w.unit + i) * TC_UNIT;
+                if (alive) alive = tc_wait(s_full + 8 * st, s_par, a.status);
+                s_par ^= 1u;
+                __syncwarp();
+                tc_fence_after();
+                float s[TC_UNIT];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc_ld32(ts + 32 * c, s + 32 * c);
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc_ld_wait32(s + 32 * c);
+                const int j0 = k0 + base_pos;
+                const bool whole = j0 + TC_UNIT - 1 <= min_row && k0 + TC_UNIT <= w.it.k.key_end && (a.window == 0 || j0 > max_row - a.window || j0 + TC_UNIT <= a.sinks);
+                if (!whole) {
+                    // key kk of the unit is visible from `from` to `to` and below `sink`
+                    const int end = min(pos - base_pos + 1, w.it.k.key_end) - k0, from = a.window > 0 ? pos - a.window + 1 - base_pos - k0 : INT_MIN,
+                              sink = a.sinks - base_pos - k0;
+#pragma unroll
+                    for (int kk = 0; kk < TC_UNIT; kk++)
+                        if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
+                }
+                float top = s[0];
+#pragma unroll
+                for (int kk = 1; kk < TC_UNIT; kk++) top = fmaxf(top, s[kk]);
+                const bool grow = (top - mx) * a.scale2 > 8.f || (mx == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float next = fmaxf(mx, top), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
+                    mx = next;
+                    l *= f;
+                    if (i >= step) {  // (the first unit starts the accumulator)
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            float o[32];
+                            tc_ld32(to + 32 * c, o);
+                            tc_ld_wait32(o);
+                            uint32_t q[32];
+#pragma unroll
+                            for (int x = 0; x < 32; x++) q[x] = __float_as_uint(o[x] * f);
+                            tc_st32(to + 32 * c, q);
+                        }
+                    }
+                }
+                const float off = mx == -INFINITY ? 0.f : mx * a.scale2;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t q[16];
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        const float e0 = ex2(fmaf(s[32 * c + 2 * x], a.scale2, -off)), e1 = ex2(fmaf(s[32 * c + 2 * x + 1], a.scale2, -off));
+                        l += e0 + e1;
+                        q[x] = pack2<BF16>(e0, e1);
+                    }
+                    tc_st16(ts + 16 * c, q);
+                }
+                tc_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * st);
+            }
+            // ---- results ----
+            const bool worked = !joint || m > st;
+            if (worked) {
+                if (alive) alive = tc_wait(o_full + 8 * st, o_par, a.status);
+                o_par ^= 1u;
+            }
+            __syncwarp();
+            tc_fence_after();
+            const float m2 = mx == -INFINITY ? -INFINITY : mx * a.scale2;
+            const int64_t item_start = w.pos - w.unit;
+            const bool complete = w.unit == 0 && m == w.it.u.count;
+            float M = m2, L = l, f0 = 1.f, f1 = 0.f;
+            if (joint) {
+                ml[st * TC_ROWS + r] = make_float2(m2, l);
+                tc_fence_before();
+                named_barrier(1, TC_SOFTMAX_THREADS);
+                tc_fence_after();
+                const float2 x = ml[r], y = ml[TC_ROWS + r];
+                M = fmaxf(x.x, y.x);
+                f0 = x.x == -INFINITY ? 0.f : ex2(x.x - M);
+                f1 = y.x == -INFINITY ? 0.f : ex2(y.x - M);
+                L = x.y * f0 + y.y * f1;
+            }
+            const int own_slot = 2 * blockIdx.x + (w.unit == 0 ? 1 : 0);
+            const int prow = joint ? r : st * TC_ROWS + r;
+            float *part = a.part + (int64_t)own_slot * TC_ITEM_ROWS * (D + 2);
+            // joint: each stream finishes half of the columns from both accumulators
+            const int c_first = joint ? st * (D / 64) : 0, c_last = joint ? c_first + D / 64 : D / 32;
+            for (int c = c_first; c < c_last; c++) {
+                float o[32];
+                if (joint) {
+                    float x[32];
+                    tc_ld32(tmem + C::O_COL + lanes + 32 * c, o);
+                    tc_ld_wait32(o);
+                    if (m > 1) {
+                        tc_ld32(tmem + C::O_COL + D + lanes + 32 * c, x);
+                        tc_ld_wait32(x);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = o[e] * f0 + x[e] * f1;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] *= f0;
+                    }
+                } else {
+                    tc_ld32(to + 32 * c, o);
+                    tc_ld_wait32(o);
+                }
+                if (valid) {
+                    if (complete) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float v[8];
+#pragma unroll
+                            for (int x = 0; x < 8; x++) v[x] = o[8 * e + x];
+                            paged_finish8<BF16>(a, D, token, head, 32 * c + 8 * e, M, L, v);
+                        }
+                    } else {
+                        float4 *dst = reinterpret_cast<float4 *>(part + (int64_t)prow * D + 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        if (c == c_first) *reinterpret_cast<float2 *>(part + (int64_t)TC_ITEM_ROWS * D + 2 * prow) = make_float2(M, L);
+                    }
+                }
+            }
+            tc_fence_before();
+            if (!complete) {
+                const int c0 = paged_owner(item_start, sh.total, sh.N), c1 = paged_owner(item_start + w.it.u.count - 1, sh.total, sh.N);
+                __threadfence();
+                named_barrier(1, TC_SOFTMAX_THREADS);
+                if (tid == 0) {
+                    const unsigned seen = atomicAdd(a.counters + c0, 1u);
+                    *last_word = seen == (unsigned)(c1 - c0);
+                    if (seen == (unsigned)(c1 - c0)) a.counters[c0] = 0;
+                }
+                named_barrier(1, TC_SOFTMAX_THREADS);
+                if (*last_word) {
+                    __threadfence();
+                    paged_merge<TC_SOFTMAX_THREADS, TC_ITEM_ROWS, BF16>(a, D, c0, c1, w.it.rows, [&](int x, int &t, int &h) { token_of(w.rt * TC_ITEM_ROWS + x, t, h); });
+                }
+            }
+            if (joint || !complete) named_barrier(1, TC_SOFTMAX_THREADS);  // the exchange, the accumulators and the flag are used again
+            w.next(a, sh);
+            if (w.pos >= sh.u1) break;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == TC_MMA_WARP)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+template <int D, bool BF16>
+cudaError_t launch_tc_t(const PagedArgs &a, const PagedMaps &maps, int box_rows, cudaStream_t st) {
+    using C = TcCfg<D>;
+    static_assert(C::SMEM <= 227 * 1024, "shared memory of a CTA");
+    auto kernel = paged_tc_kernel<D, BF16>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3((unsigned)a.sms), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, box_rows);
+}
+
+}  // namespace
+
+int64_t paged_tc_part_floats(int d, int sms) { return (int64_t)2 * sms * TC_ITEM_ROWS * (d + 2); }
+
+cudaError_t launch_paged_tc(const PagedArgs &a, int dt, int d, const PagedMaps &maps, int box_rows, cudaStream_t st) {
+    if (d == 128) return dt == TTQ_DT_BF16 ? launch_tc_t<128, true>(a, maps, box_rows, st) : launch_tc_t<128, false>(a, maps, box_rows, st);
+    return dt == TTQ_DT_BF16 ? launch_tc_t<64, true>(a, maps, box_rows, st) : launch_tc_t<64, false>(a, maps, box_rows, st);
+}
+
+}  // namespace ttq
