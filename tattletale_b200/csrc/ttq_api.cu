@@ -81,8 +81,8 @@ struct ttq_paged {
     ttq_ctx *ctx;
     int dt, hq, hkv, d, page_size, page_shift;
     int64_t max_seqs, max_tokens, max_prefix_tokens;
-    void *ws;            // one allocation: arrival counters, partial results, the shared prefix's results
-    unsigned *counters;
+    void *ws;            // one allocation: arrival counters, records of cut items, partial results, the shared prefix's results
+    unsigned *counters, *splits;
     float *part, *pre_o, *pre_lse;
 };
 
@@ -1679,10 +1679,10 @@ ttq_status ttq_paged_create(ttq_ctx *ctx, ttq_dtype dt, int32_t hq, int32_t hkv,
     p->max_seqs = max_seqs; p->max_tokens = max_tokens; p->max_prefix_tokens = max_prefix_tokens;
     while ((1 << p->page_shift) < page_size) p->page_shift++;
     auto up256 = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    const size_t b_cnt = up256((size_t)paged_counters(ctx->sms) * sizeof(unsigned)), b_part = up256((size_t)paged_part_floats(d, ctx->sms) * sizeof(float));
+    const size_t b_cnt = up256((size_t)paged_counters(ctx->sms) * sizeof(unsigned)), b_split = up256((size_t)paged_tc_words(ctx->sms) * sizeof(unsigned)), b_part = up256((size_t)paged_part_floats(d, ctx->sms) * sizeof(float));
     const size_t rows = (size_t)max_prefix_tokens * hq;
     const size_t b_o = up256(rows * d * sizeof(float)), b_lse = up256(rows * sizeof(float));
-    cudaError_t e = cudaMalloc(&p->ws, b_cnt + b_part + b_o + b_lse);
+    cudaError_t e = cudaMalloc(&p->ws, b_cnt + b_split + b_part + b_o + b_lse);
     if (e == cudaSuccess) e = cudaMemset(p->ws, 0, b_cnt);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e != cudaSuccess) {
@@ -1692,6 +1692,7 @@ ttq_status ttq_paged_create(ttq_ctx *ctx, ttq_dtype dt, int32_t hq, int32_t hkv,
     }
     uint8_t *q = reinterpret_cast<uint8_t *>(p->ws);
     p->counters = reinterpret_cast<unsigned *>(q); q += b_cnt;
+    p->splits = reinterpret_cast<unsigned *>(q); q += b_split;
     p->part = reinterpret_cast<float *>(q); q += b_part;
     p->pre_o = reinterpret_cast<float *>(q); q += b_o;
     p->pre_lse = reinterpret_cast<float *>(q);
@@ -1757,7 +1758,6 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
     a.sinks = sinks > INT32_MAX ? INT32_MAX : (int)sinks;
     a.scale2 = scale * 1.4426950408889634f;
     a.part = p->part;
-    a.counters = p->counters;
     // the shared prefix for all rows first, then every sequence's own keys, which take the prefix's results in
     for (int pass = bt->prefix_len > 0 ? 0 : 1; pass < 2; pass++) {
         a.prefix_pass = pass == 0;
@@ -1766,6 +1766,7 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
         // few rows per kv head: the memory-bound kernel; from 17 on the tensor-memory kernel
         const int64_t most = a.prefix_pass || bt->max_q == 0 ? bt->n_tokens : bt->max_q;
         const bool few = most * a.G <= 16;
+        a.counters = few ? p->counters : p->splits;
         const int slots = few ? 16 : (p->page_size < 128 ? p->page_size : 128);
         PagedMaps maps;
         ttq_status ms = paged_map(ctx, p, kv, kv->k_dev, slots, &maps.k);
@@ -1774,7 +1775,7 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
         const cudaError_t e = few ? launch_paged_rows(a, p->dt, p->d, maps, (cudaStream_t)stream)
                                   : launch_paged_tc(a, p->dt, p->d, maps, slots, (cudaStream_t)stream);
         if (e != cudaSuccess) return cuda_fail(ctx, e, "paged attention launch");
-        ctx->launches++;
+        ctx->launches += few ? 1 : 2;
     }
     return TTQ_OK;
 }

@@ -523,7 +523,14 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             __syncthreads();
             if (last_s) {
                 __threadfence();
-                paged_merge<ROWS_THREADS, ROWS_TILE, BF16>(a, D, c0, c1, rows, [&](int r, int &token, int &head) { row_of(cw.item, cw.s, r, token, head); });
+                for (int i = tid; i < rows * (D / 8); i += ROWS_THREADS) {
+                    const int r = i / (D / 8), col = i % (D / 8) * 8;
+                    float m, l, v[8];
+                    paged_gather8<ROWS_TILE>(a, D, c0, c1, r, col, m, l, v);
+                    int token, head;
+                    row_of(cw.item, cw.s, r, token, head);
+                    paged_finish8<BF16>(a, D, token, head, col, m, l, v);
+                }
             }
         }
         if (pos + 1 < sh.u1) {

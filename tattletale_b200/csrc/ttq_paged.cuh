@@ -6,9 +6,9 @@
 // units of a fixed number of keys.  All units of a call are numbered through -- sequence, row tile, kv head, unit -- and every CTA
 // takes an equal, contiguous share of the numbers, found from the lengths in device memory by each CTA for itself (a captured graph
 // follows them, the host never waits).  An item that one CTA sees whole is finished there; of an item cut by share borders
-// every CTA leaves a partial result (running maximum, sum, unnormalised output) in the plan's workspace, and the one that
-// arrives last adds them in the order of the keys: at most two partials per CTA whatever the batch looks like, one launch, and the
-// same bits every time.
+// every CTA leaves a partial result (running maximum, sum, unnormalised output) in the plan's workspace, at most two per CTA
+// whatever the batch looks like.  They are added in the order of the keys, hence to the same bits every time: by the CTA that
+// arrives last (few rows), or by a launch of its own (hundreds of rows).
 #pragma once
 
 #include <cuda.h>
@@ -36,7 +36,7 @@ struct PagedArgs {
     float scale2;               // scale * log2(e): scores and maxima are kept in units of log2
     float *pre_o, *pre_lse;     // [n_tokens][hq][d] normalised, [n_tokens][hq]; read by the other pass (nullptr: no prefix)
     float *part;                // partial results, two per CTA
-    unsigned *counters;         // arrivals, one per CTA, zero between launches
+    unsigned *counters;         // few rows: arrivals, one per CTA, zero between launches; else the records of cut items
     int *status;
     int sms;
 };
@@ -243,35 +243,30 @@ __device__ __forceinline__ void paged_finish8(const PagedArgs &a, int D, int tok
     *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Adds the partials of one item in the order of the keys and writes its rows; called by all THREADS of the CTA that arrived last.
-// part: [2 N][ROWS][D + 2] = (output, maximum, sum).  The item's units are in the shares of CTAs c0 .. c1; it starts in c0's
-// last segment (slot 2 c0 + 1) and continues in the first ones of the others (slots 2 c).
-template <int THREADS, int ROWS, bool BF16, class RowFn>
-__device__ __forceinline__ void paged_merge(const PagedArgs &a, int D, int c0, int c1, int rows, RowFn &&row_of) {
-    const int per_row = D / 8;
+// Adds the partials of eight results of one row in the order of the keys: maximum, sum and unnormalised output.
+// part: [2 N][ROWS][D + 2] = (outputs, then maximum and sum per row).  The item's units are in the shares of CTAs c0 .. c1; it starts
+// in c0's last segment (slot 2 c0 + 1) and continues in the first ones of the others (slots 2 c).
+template <int ROWS>
+__device__ __forceinline__ void paged_gather8(const PagedArgs &a, int D, int c0, int c1, int r, int col, float &m, float &l, float (&v)[8]) {
     const int64_t pitch = (int64_t)ROWS * (D + 2);
-    for (int i = threadIdx.x; i < rows * per_row; i += THREADS) {
-        const int r = i / per_row, col = (i % per_row) * 8;
-        const float *ml = a.part + (int64_t)ROWS * D + 2 * r;
-        float m = -INFINITY;
-        for (int c = c0; c <= c1; c++) m = fmaxf(m, __ldcg(ml + (2 * c + (c == c0)) * pitch));
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
-        if (m != -INFINITY) {
-            const float *o = a.part + (int64_t)r * D + col;
+    const float *ml = a.part + (int64_t)ROWS * D + 2 * r;
+    m = -INFINITY;
+#pragma unroll 8
+    for (int c = c0; c <= c1; c++) m = fmaxf(m, __ldcg(ml + (2 * c + (c == c0)) * pitch));
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = 0.f;
+    if (m == -INFINITY) return;
+    const float *o = a.part + (int64_t)r * D + col;
 #pragma unroll 4
-            for (int c = c0; c <= c1; c++) {
-                const int64_t at = (2 * c + (c == c0)) * pitch;
-                const float2 s = __ldcg(reinterpret_cast<const float2 *>(ml + at));
-                const float4 x = __ldcg(reinterpret_cast<const float4 *>(o + at)), y = __ldcg(reinterpret_cast<const float4 *>(o + at + 4));
-                const float w = ex2(s.x - m);
-                l = fmaf(w, s.y, l);
-                v[0] = fmaf(w, x.x, v[0]); v[1] = fmaf(w, x.y, v[1]); v[2] = fmaf(w, x.z, v[2]); v[3] = fmaf(w, x.w, v[3]);
-                v[4] = fmaf(w, y.x, v[4]); v[5] = fmaf(w, y.y, v[5]); v[6] = fmaf(w, y.z, v[6]); v[7] = fmaf(w, y.w, v[7]);
-            }
-        }
-        int token, head;
-        row_of(r, token, head);
-        paged_finish8<BF16>(a, D, token, head, col, m, l, v);
+    for (int c = c0; c <= c1; c++) {
+        const int64_t at = (2 * c + (c == c0)) * pitch;
+        const float2 s = __ldcg(reinterpret_cast<const float2 *>(ml + at));
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(o + at)), y = __ldcg(reinterpret_cast<const float4 *>(o + at + 4));
+        const float w = ex2(s.x - m);
+        l = fmaf(w, s.y, l);
+        v[0] = fmaf(w, x.x, v[0]); v[1] = fmaf(w, x.y, v[1]); v[2] = fmaf(w, x.z, v[2]); v[3] = fmaf(w, x.w, v[3]);
+        v[4] = fmaf(w, y.x, v[4]); v[5] = fmaf(w, y.y, v[5]); v[6] = fmaf(w, y.z, v[6]); v[7] = fmaf(w, y.w, v[7]);
     }
 }
 
@@ -291,7 +286,8 @@ cudaError_t launch_paged_rows(const PagedArgs &a, int dt, int d, const PagedMaps
 constexpr int PAGED_ROWS16_CTAS = 2;  // resident CTAs per SM of the kernel for few rows
 cudaError_t launch_paged_tc(const PagedArgs &a, int dt, int d, const PagedMaps &maps, int box_rows, cudaStream_t st);
 int64_t paged_tc_part_floats(int d, int sms);
-// Workspace of a plan: partial results in floats, arrival counters.
+int64_t paged_tc_words(int sms);  // records of cut items
+// Workspace of a plan: partial results in floats, arrival counters of the kernel for few rows.
 int64_t paged_part_floats(int d, int sms);
 int64_t paged_counters(int sms);
 struct PagedAppend {

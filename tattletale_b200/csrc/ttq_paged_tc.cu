@@ -11,7 +11,8 @@
 // memory, whose lanes the warps of both streams reach.  Tensor memory is full: 2 x 128 columns of scores, 2 x d of output.
 //
 // Warps 0-3 and 4-7: softmax of the two streams, and their rows' queries and results.  Warp 8 issues the products, warp 9 the
-// tiled copies of the pages into a ring of slots.  Products of one CTA execute in the order of issue, so the scores of unit
+// tiled copies of the pages into a ring of slots, warp 10 walks the batch and hands the other warps one record per item (they keep
+// their registers for scores); warp 11 only fills the warpgroup.  Products of one CTA execute in the order of issue, so the scores of unit
 // i + 1 may follow the product that reads the weights of unit i from the same columns, and a full score buffer means that
 // the output accumulator is at rest: the softmax warps rescale it in place, which they do only when the maximum has grown by 2^8.
 #include <climits>
@@ -25,8 +26,26 @@ namespace {
 constexpr int TC_UNIT = 128;       // keys per unit
 constexpr int TC_ROWS = 128;       // rows per stream
 constexpr int TC_ITEM_ROWS = 2 * TC_ROWS;
-constexpr int TC_MMA_WARP = 8, TC_TMA_WARP = 9;
-constexpr int TC_THREADS = 320, TC_SOFTMAX_THREADS = 256;
+constexpr int TC_MMA_WARP = 8, TC_TMA_WARP = 9, TC_WALK_WARP = 10;
+constexpr int TC_THREADS = 384, TC_SOFTMAX_THREADS = 256;
+// The block is launched with 168 registers a thread (65536 / 384, in steps of 8); a softmax thread, which holds a row of scores,
+// gets 208, a thread of the third warpgroup keeps 88: 8 x 208 + 4 x 88 = 12 x 168.
+constexpr int TC_SOFTMAX_REGS = 208, TC_OTHER_REGS = 88;
+
+// One item, or the part of it that is in this CTA's share.
+struct TcSeg {
+    int m;                    // units (0: the share ends)
+    int unit, u_sink, u_first;   // first unit; numbers of the item's units as PagedUnits has them
+    int key_end, lo, sink;
+    int rows, row0, total_rows;  // valid rows, number of the first one in the sequence, rows of the sequence
+    int b, head, q0, pos0;
+    int complete, slot;       // the item is whole; else where its partial goes
+};
+constexpr int TC_SEGS = 4, TC_SEG_READERS = 10;
+// An item that begins in one CTA's share and ends in CTA c1's (rows 0: none), left for the kernel that joins the parts.
+struct TcSplit {
+    int c1, rows, row0, q0, head;
+};
 
 template <int D>
 struct TcCfg {
@@ -38,9 +57,10 @@ struct TcCfg {
     // shared memory: queries, ring, then barriers and exchange
     static constexpr int RING_AT = 2 * SLOT_BYTES;
     static constexpr int BAR_AT = RING_AT + SLOTS * SLOT_BYTES;
-    static constexpr int N_BARS = 2 * SLOTS + 8 + 1;
+    static constexpr int N_BARS = 2 * SLOTS + 8 + 1 + 2 * TC_SEGS;
     static constexpr int ML_AT = BAR_AT + (N_BARS * 8 + 15) / 16 * 16;
-    static constexpr int MISC_AT = ML_AT + 2 * TC_ROWS * 8;
+    static constexpr int SEG_AT = ML_AT + 2 * TC_ROWS * 8;
+    static constexpr int MISC_AT = SEG_AT + (TC_SEGS * (int)sizeof(TcSeg) + 15) / 16 * 16;
     static constexpr int SMEM = MISC_AT + 16 * 8 + 16;
 };
 
@@ -236,11 +256,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
     const uint32_t base = smem_u32(smem);
     const uint32_t bars = base + C::BAR_AT;
     const uint32_t kv_full = bars, kv_empty = kv_full + 8 * C::SLOTS, q_full = kv_empty + 8 * C::SLOTS, s_full = q_full + 16, p_full = s_full + 16,
-                   o_full = p_full + 16, fix_bar = o_full + 16;
+                   o_full = p_full + 16, fix_bar = o_full + 16, seg_full = fix_bar + 8, seg_empty = seg_full + 8 * TC_SEGS;
     float2 *ml = reinterpret_cast<float2 *>(smem + C::ML_AT);
+    TcSeg *segs = reinterpret_cast<TcSeg *>(smem + C::SEG_AT);
     int64_t *red = reinterpret_cast<int64_t *>(smem + C::MISC_AT);
     volatile uint32_t *slot_word = reinterpret_cast<volatile uint32_t *>(smem + C::MISC_AT + 16 * 8);
-    volatile int *last_word = reinterpret_cast<volatile int *>(smem + C::MISC_AT + 16 * 8 + 4);
+    TcSplit *splits = reinterpret_cast<TcSplit *>(a.counters);
     if (tid == 0) {
         for (int i = 0; i < C::SLOTS; i++) {
             mbar_init(kv_full + 8 * i, 1);
@@ -253,6 +274,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             mbar_init(o_full + 8 * i, 1);
         }
         mbar_init(fix_bar, 1);
+        for (int i = 0; i < TC_SEGS; i++) {
+            mbar_init(seg_full + 8 * i, 1);
+            mbar_init(seg_empty + 8 * i, TC_SEG_READERS);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     grid_launch_dependents();
@@ -279,7 +304,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         }
         return units * a.hkv;
     });
-    if (sh.u0 >= sh.u1) return;
+    if (sh.u0 >= sh.u1) {
+        if (tid == 0) splits[blockIdx.x].rows = 0;
+        return;
+    }
     if (warp == TC_MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)slot_word)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -289,10 +317,200 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
     tc_fence_after();
     const uint32_t tmem = *slot_word;
 
-    TcWalk w;
-    w.start(a, sh, lane);
-
-    if (warp == TC_TMA_WARP) {
+    // a reader's next record, and its release
+    auto seg_wait = [&](int k) { return tc_wait(seg_full + 8 * (k % TC_SEGS), (uint32_t)((k / TC_SEGS) & 1), a.status); };
+    auto seg_done = [&](int k) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(seg_empty + 8 * (k % TC_SEGS));
+    };
+    if (warp < TC_MMA_WARP) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_SOFTMAX_REGS));
+        // ------------------------------------------------------------------------------------------ softmax: a thread per row
+        const int st = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the tensor memory's lanes
+        const uint32_t ts = tmem + C::S_COL + st * TC_UNIT + lanes, to = tmem + C::O_COL + st * D + lanes;
+        bool alive = true;
+        uint32_t s_par = 0, o_par = 0;
+        const int base_pos = a.prefix_pass ? 0 : a.prefix_len;
+        auto token_of = [&](const TcSeg &g, int x, int &token, int &head) {
+            const int i = x / a.G;
+            token = g.q0 + i;
+            head = g.head * a.G + (x - i * a.G);
+        };
+        auto first_row = [&](const TcSeg &g) { return g.row0 + (g.rows > TC_ROWS ? st * TC_ROWS : 0); };
+        // queries of an item into shared memory; the products that read the last item's are complete
+        auto load_queries = [&](const TcSeg &g) {
+            const int row0 = first_row(g), total_rows = g.total_rows;
+#pragma unroll 4
+            for (int c = r; c < TC_ROWS * (D / 8); c += TC_ROWS) {
+                const int row = c / (D / 8), ch = c % (D / 8);
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (row0 + row < total_rows) {
+                    int token, head;
+                    token_of(g, row0 + row, token, head);
+                    v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (int64_t)token * a.ld_q + (int64_t)head * D + 8 * ch);
+                }
+                sts128<0>(base + (uint32_t)(st * C::SLOT_BYTES + (ch >> 3) * C::HALF_BYTES + row * 128 + (((ch & 7) ^ (row & 7)) << 4)), v.x, v.y, v.z, v.w);
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full + 8 * st);
+        };
+        bool have = seg_wait(0);
+        if (have && segs[0].m > 0) load_queries(segs[0]);
+        for (int k = 0; have; k++) {
+            const TcSeg &g = segs[k % TC_SEGS];
+            const int m = g.m;
+            if (m == 0) break;
+            const bool joint = g.rows <= TC_ROWS;   // both streams work on the same rows
+            const bool valid = first_row(g) + r < g.total_rows;
+            int pos = -1;
+            if (valid) {
+                int token, head;
+                token_of(g, first_row(g) + r, token, head);
+                pos = a.prefix_pass ? paged_row_pos(a, token) : g.pos0 + token - g.q0;
+            }
+            const int min_row = __reduce_min_sync(0xffffffffu, valid ? pos : INT_MAX), max_row = __reduce_max_sync(0xffffffffu, valid ? pos : -1);
+            float mx = -INFINITY, l = 0.f;  // running maximum of the scores (unscaled) and sum
+            const int step = joint ? 2 : 1;
+            for (int i = joint ? st : 0; i < m; i += step) {
+                const int ui = g.unit + i, k0 = (ui < g.u_sink ? ui : g.u_first + ui - g.u_sink) * TC_UNIT;
+                if (alive) alive = tc_wait(s_full + 8 * st, s_par, a.status);
+                s_par ^= 1u;
+                __syncwarp();
+                tc_fence_after();
+                float s[TC_UNIT];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc_ld32(ts + 32 * c, s + 32 * c);
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc_ld_wait32(s + 32 * c);
+                const int j0 = k0 + base_pos;
+                const bool whole = j0 + TC_UNIT - 1 <= min_row && k0 + TC_UNIT <= g.key_end && (a.window == 0 || j0 > max_row - a.window || j0 + TC_UNIT <= a.sinks);
+                if (!whole) {
+                    // key kk of the unit is visible from `from` to `to` and below `sink`
+                    const int end = min(pos - base_pos + 1, g.key_end) - k0, from = a.window > 0 ? pos - a.window + 1 - base_pos - k0 : INT_MIN,
+                              sink = a.sinks - base_pos - k0;
+#pragma unroll
+                    for (int kk = 0; kk < TC_UNIT; kk++)
+                        if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
+                }
+                float top = s[0];
+#pragma unroll
+                for (int kk = 1; kk < TC_UNIT; kk++) top = fmaxf(top, s[kk]);
+                const bool grow = (top - mx) * a.scale2 > 8.f || (mx == -INFINITY && top > -INFINITY);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float next = fmaxf(mx, top), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
+                    mx = next;
+                    l *= f;
+                    if (i >= step) {  // (the first unit starts the accumulator)
+#pragma unroll
+                        for (int c = 0; c < D / 32; c++) {
+                            float o[32];
+                            tc_ld32(to + 32 * c, o);
+                            tc_ld_wait32(o);
+                            uint32_t q[32];
+#pragma unroll
+                            for (int x = 0; x < 32; x++) q[x] = __float_as_uint(o[x] * f);
+                            tc_st32(to + 32 * c, q);
+                        }
+                    }
+                }
+                const float off = mx == -INFINITY ? 0.f : mx * a.scale2;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t q[16];
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        const float e0 = ex2(fmaf(s[32 * c + 2 * x], a.scale2, -off)), e1 = ex2(fmaf(s[32 * c + 2 * x + 1], a.scale2, -off));
+                        l += e0 + e1;
+                        q[x] = pack2<BF16>(e0, e1);
+                    }
+                    tc_st16(ts + 16 * c, q);
+                }
+                tc_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * st);
+            }
+            // ---- results ----
+            const bool worked = !joint || m > st;
+            // the next item's first scores are computed under this one's end (a stream without a unit waits for the other: its queries'
+            // barrier may be one phase ahead of the product warp, not two)
+            auto prefetch = [&]() {
+                have = seg_wait(k + 1);
+                if (have && segs[(k + 1) % TC_SEGS].m > 0) load_queries(segs[(k + 1) % TC_SEGS]);
+            };
+            if (worked) {
+                prefetch();
+                if (alive) alive = tc_wait(o_full + 8 * st, o_par, a.status);
+                o_par ^= 1u;
+            }
+            __syncwarp();
+            tc_fence_after();
+            const float m2 = mx == -INFINITY ? -INFINITY : mx * a.scale2;
+            const bool complete = g.complete;
+            int token, head;
+            token_of(g, first_row(g) + r, token, head);
+            float M = m2, L = l, f0 = 1.f, f1 = 0.f;
+            if (joint) {
+                ml[st * TC_ROWS + r] = make_float2(m2, l);
+                tc_fence_before();
+                named_barrier(1, TC_SOFTMAX_THREADS);
+                tc_fence_after();
+                const float2 x = ml[r], y = ml[TC_ROWS + r];
+                M = fmaxf(x.x, y.x);
+                f0 = x.x == -INFINITY ? 0.f : ex2(x.x - M);
+                f1 = y.x == -INFINITY ? 0.f : ex2(y.x - M);
+                L = x.y * f0 + y.y * f1;
+            }
+            const int prow = joint ? r : st * TC_ROWS + r;
+            float *part = a.part + (int64_t)g.slot * TC_ITEM_ROWS * (D + 2);
+            // joint: each stream finishes half of the columns from both accumulators
+            const int c_first = joint ? st * (D / 64) : 0, c_last = joint ? c_first + D / 64 : D / 32;
+            for (int c = c_first; c < c_last; c++) {
+                float o[32];
+                if (joint) {
+                    float x[32];
+                    tc_ld32(tmem + C::O_COL + lanes + 32 * c, o);
+                    tc_ld_wait32(o);
+                    if (m > 1) {
+                        tc_ld32(tmem + C::O_COL + D + lanes + 32 * c, x);
+                        tc_ld_wait32(x);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = o[e] * f0 + x[e] * f1;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] *= f0;
+                    }
+                } else {
+                    tc_ld32(to + 32 * c, o);
+                    tc_ld_wait32(o);
+                }
+                if (valid) {
+                    if (complete) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float v[8];
+#pragma unroll
+                            for (int x = 0; x < 8; x++) v[x] = o[8 * e + x];
+                            paged_finish8<BF16>(a, D, token, head, 32 * c + 8 * e, M, L, v);
+                        }
+                    } else {
+                        float4 *dst = reinterpret_cast<float4 *>(part + (int64_t)prow * D + 32 * c);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        if (c == c_first) *reinterpret_cast<float2 *>(part + (int64_t)TC_ITEM_ROWS * D + 2 * prow) = make_float2(M, L);
+                    }
+                }
+            }
+            tc_fence_before();
+            if (joint) named_barrier(1, TC_SOFTMAX_THREADS);  // the exchange and the other's accumulator are used again
+            if (!worked) prefetch();
+            seg_done(k);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_OTHER_REGS));
+        if (warp == TC_TMA_WARP) {
         // ------------------------------------------------------------------------------------------ copies of the pages
         int n = 0;  // slots filled so far
         bool alive = true;
@@ -300,15 +518,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         const int page_mask = (1 << a.page_shift) - 1;
         // Unit i of the item into the next slot: boxes of box_rows slots of one page.  Boxes that no row sees are left out of K (their scores
         // are masked) and are zeros in V; rows of a page that no row sees are zeroed in V, where a weight of zero would meet them.
+        int key_end = 0, lo = 0, sink = 0, u_sink = 0, u_first = 0, head = 0, seq = 0;
         int cache_first = -1, cache_b = -1, page_cache = 0;  // lane i: page number cache_first + i of the table of sequence cache_b
         auto copy = [&](int i, bool is_v) {
-            const int k0 = paged_unit_index(w.it.u, i) * TC_UNIT;
-            const PagedSeq &k = w.it.k;
-            auto wanted = [&](int kb) { return kb < k.key_end && (kb + box_rows > k.lo || kb < k.sink); };
+            const int k0 = (i < u_sink ? i : u_first + i - u_sink) * TC_UNIT;
+            auto wanted = [&](int kb) { return kb < key_end && (kb + box_rows > lo || kb < sink); };
             const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES, full = kv_full + 8 * (n % C::SLOTS);
             if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
             __syncwarp();
-            const bool fix = is_v && (k0 + TC_UNIT > k.key_end || (k0 < k.lo && k0 + TC_UNIT > k.sink));
+            const bool fix = is_v && (k0 + TC_UNIT > key_end || (k0 < lo && k0 + TC_UNIT > sink));
             const uint32_t bar = fix ? fix_bar : full;
             int bytes = 0;
             for (int r = 0; r < TC_UNIT; r += box_rows) bytes += is_v || wanted(k0 + r) ? box_rows * 128 * C::HALVES : 0;
@@ -322,13 +540,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 int page = a.n_pages;  // beyond the last page: zeros
                 if (wanted(kb)) {
                     const int idx = kb >> a.page_shift;
-                    if (cache_b != w.b || idx < cache_first || idx >= cache_first + 32) {
-                        cache_b = w.b;
+                    if (cache_b != seq || idx < cache_first || idx >= cache_first + 32) {
+                        cache_b = seq;
                         cache_first = idx;
-                        const int64_t last = (k.key_end - 1) >> a.page_shift;
+                        const int64_t last = (key_end - 1) >> a.page_shift;
                         const int at = idx + lane;
                         page_cache = -1;
-                        if (at <= last) page_cache = a.prefix_pass ? a.prefix_table[at] : a.block_table[(int64_t)w.b * a.ld_table + at];
+                        if (at <= last) page_cache = a.prefix_pass ? a.prefix_table[at] : a.block_table[(int64_t)seq * a.ld_table + at];
                     }
                     page = __shfl_sync(0xffffffffu, page_cache, idx - cache_first);
                     if (page < 0 || page >= a.n_pages) {
@@ -341,7 +559,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 if (elect_one()) {
 #pragma unroll
                     for (int h = 0; h < C::HALVES; h++)
-                        tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * 128), is_v ? &vmap : &kmap, 64 * h, kb & page_mask, w.head, page, bar);
+                        tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * 128), is_v ? &vmap : &kmap, 64 * h, kb & page_mask, head, page, bar);
                 }
                 __syncwarp();
             }
@@ -350,7 +568,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 fix_par ^= 1u;
                 for (int r = lane / 8; r < TC_UNIT; r += 4) {
                     const int key = k0 + r;
-                    if (key >= k.key_end || (key < k.lo && key >= k.sink)) {
+                    if (key >= key_end || (key < lo && key >= sink)) {
 #pragma unroll
                         for (int h = 0; h < C::HALVES; h++) sts128<0>(slot + (uint32_t)(h * C::HALF_BYTES + r * 128 + (lane & 7) * 16), 0u, 0u, 0u, 0u);
                     }
@@ -361,14 +579,22 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             }
             n++;
         };
-        while (true) {
-            const int m = w.here(sh), u0 = w.unit;
-            if (w.it.rows > TC_ROWS) {  // both streams take every unit
+        for (int k = 0; seg_wait(k); k++) {
+            const TcSeg &g = segs[k % TC_SEGS];
+            const int m = g.m;
+            if (m == 0) break;
+            key_end = g.key_end; lo = g.lo; sink = g.sink;
+            u_sink = g.u_sink; u_first = g.u_first;
+            head = g.head; seq = g.b;
+            const int u0 = g.unit;
+            const bool pair = g.rows > TC_ROWS;
+            seg_done(k);
+            if (pair) {   // both streams take every unit
                 for (int i = 0; i < m; i++) {
                     copy(u0 + i, false);
                     copy(u0 + i, true);
                 }
-            } else {                    // stream 0 the even ones, stream 1 the odd ones
+            } else {      // stream 0 the even ones, stream 1 the odd ones
                 copy(u0, false);
                 if (m > 1) copy(u0 + 1, false);
                 for (int i = 0; i < m; i++) {
@@ -376,8 +602,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     if (i + 2 < m) copy(u0 + i + 2, false);
                 }
             }
-            w.next(a, sh);
-            if (w.pos >= sh.u1) break;
         }
         // the last copies have landed before the CTA may end: the product warp waits for every slot
     } else if (warp == TC_MMA_WARP) {
@@ -425,12 +649,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             }
             __syncwarp();
         };
-        while (true) {
-            const int m = w.here(sh);
+        for (int k = 0; seg_wait(k); k++) {
+            const TcSeg &g = segs[k % TC_SEGS];
+            const int m = g.m;
+            if (m == 0) break;
+            const bool pair = g.rows > TC_ROWS;
+            seg_done(k);
             for (int st = 0; st < 2; st++)
                 if (alive) alive = tc_wait(q_full + 8 * st, q_par, a.status);
             q_par ^= 1u;
-            if (w.it.rows > TC_ROWS) {
+            if (pair) {
                 scores(0, n, false);
                 scores(1, n, true);
                 n++;
@@ -450,193 +678,38 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     if (i + 2 < m) scores(i & 1, n++, true);
                 }
             }
-            w.next(a, sh);
-            if (w.pos >= sh.u1) break;
         }
-    } else {
-        // ------------------------------------------------------------------------------------------ softmax: a thread per row
-        const int st = warp >> 2, r = tid & 127;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the tensor memory's lanes
-        const uint32_t ts = tmem + C::S_COL + st * TC_UNIT + lanes, to = tmem + C::O_COL + st * D + lanes;
-        bool alive = true;
-        uint32_t s_par = 0, o_par = 0;
-        const int base_pos = a.prefix_pass ? 0 : a.prefix_len;
-        while (true) {
-            const int m = w.here(sh);
-            const bool joint = w.it.rows <= TC_ROWS;   // both streams work on the same rows
-            const int row0 = w.rt * TC_ITEM_ROWS + (joint ? 0 : st * TC_ROWS);
-            const int total_rows = w.s.n * a.G;
-            auto token_of = [&](int x, int &token, int &head) {
-                const int i = x / a.G;
-                token = w.s.q0 + i;
-                head = w.head * a.G + (x - i * a.G);
-            };
-            // queries into shared memory
-            for (int c = r; c < TC_ROWS * (D / 8); c += TC_ROWS) {
-                const int row = c / (D / 8), ch = c % (D / 8);
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (row0 + row < total_rows) {
-                    int token, head;
-                    token_of(row0 + row, token, head);
-                    v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (int64_t)token * a.ld_q + (int64_t)head * D + 8 * ch);
+    } else if (warp == TC_WALK_WARP) {
+        // ------------------------------------------------------------------------------------------ the batch, item by item
+        TcWalk w;
+        w.start(a, sh, lane);
+        for (int k = 0;; k++) {
+            if (k >= TC_SEGS && !tc_wait(seg_empty + 8 * (k % TC_SEGS), (uint32_t)((k / TC_SEGS - 1) & 1), a.status)) break;
+            const bool end = w.pos >= sh.u1;
+            if (lane == 0) {
+                TcSeg g{};
+                if (!end) {
+                    g.m = w.here(sh);
+                    g.unit = w.unit; g.u_sink = w.it.u.sink; g.u_first = w.it.u.first;
+                    g.key_end = w.it.k.key_end; g.lo = w.it.k.lo; g.sink = w.it.k.sink;
+                    g.rows = w.it.rows; g.row0 = w.rt * TC_ITEM_ROWS; g.total_rows = w.s.n * a.G;
+                    g.b = w.b; g.head = w.head; g.q0 = w.s.q0; g.pos0 = w.s.pos0;
+                    const int64_t first = w.pos - w.unit;
+                    g.complete = g.m == w.it.u.count;
+                    g.slot = 2 * (int)blockIdx.x + (w.unit == 0 ? 1 : 0);
+                    // an item that begins here and goes on elsewhere is the share's last
+                    if (w.unit == 0 && !g.complete)
+                        splits[blockIdx.x] = {paged_owner(first + w.it.u.count - 1, sh.total, sh.N), g.rows, g.row0, g.q0, g.head};
+                    else if (w.pos + g.m >= sh.u1)
+                        splits[blockIdx.x].rows = 0;
                 }
-                sts128<0>(base + (uint32_t)(st * C::SLOT_BYTES + (ch >> 3) * C::HALF_BYTES + row * 128 + (((ch & 7) ^ (row & 7)) << 4)), v.x, v.y, v.z, v.w);
-            }
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full + 8 * st);
-
-            const bool valid = row0 + r < total_rows;
-            int token = 0, head = 0, pos = -1;
-            if (valid) {
-                token_of(row0 + r, token, head);
-                pos = a.prefix_pass ? paged_row_pos(a, token) : w.s.pos0 + token - w.s.q0;
-            }
-            const int min_row = __reduce_min_sync(0xffffffffu, valid ? pos : INT_MAX), max_row = __reduce_max_sync(0xffffffffu, valid ? pos : -1);
-            float mx = -INFINITY, l = 0.f;  // running maximum of the scores (unscaled) and sum
-            const int step = joint ? 2 : 1;
-            for (int i = joint ? st : 0; i < m; i += step) {
-                const int k0 = paged_unit_index(w.it.u, w.unit + i) * TC_UNIT;
-                if (alive) alive = tc_wait(s_full + 8 * st, s_par, a.status);
-                s_par ^= 1u;
-                __syncwarp();
-                tc_fence_after();
-                float s[TC_UNIT];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_ld32(ts + 32 * c, s + 32 * c);
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_ld_wait32(s + 32 * c);
-                const int j0 = k0 + base_pos;
-                const bool whole = j0 + TC_UNIT - 1 <= min_row && k0 + TC_UNIT <= w.it.k.key_end && (a.window == 0 || j0 > max_row - a.window || j0 + TC_UNIT <= a.sinks);
-                if (!whole) {
-                    // key kk of the unit is visible from `from` to `to` and below `sink`
-                    const int end = min(pos - base_pos + 1, w.it.k.key_end) - k0, from = a.window > 0 ? pos - a.window + 1 - base_pos - k0 : INT_MIN,
-                              sink = a.sinks - base_pos - k0;
-#pragma unroll
-                    for (int kk = 0; kk < TC_UNIT; kk++)
-                        if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
-                }
-                float top = s[0];
-#pragma unroll
-                for (int kk = 1; kk < TC_UNIT; kk++) top = fmaxf(top, s[kk]);
-                const bool grow = (top - mx) * a.scale2 > 8.f || (mx == -INFINITY && top > -INFINITY);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float next = fmaxf(mx, top), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
-                    mx = next;
-                    l *= f;
-                    if (i >= step) {  // (the first unit starts the accumulator)
-#pragma unroll
-                        for (int c = 0; c < D / 32; c++) {
-                            float o[32];
-                            tc_ld32(to + 32 * c, o);
-                            tc_ld_wait32(o);
-                            uint32_t q[32];
-#pragma unroll
-                            for (int x = 0; x < 32; x++) q[x] = __float_as_uint(o[x] * f);
-                            tc_st32(to + 32 * c, q);
-                        }
-                    }
-                }
-                const float off = mx == -INFINITY ? 0.f : mx * a.scale2;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t q[16];
-#pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const float e0 = ex2(fmaf(s[32 * c + 2 * x], a.scale2, -off)), e1 = ex2(fmaf(s[32 * c + 2 * x + 1], a.scale2, -off));
-                        l += e0 + e1;
-                        q[x] = pack2<BF16>(e0, e1);
-                    }
-                    tc_st16(ts + 16 * c, q);
-                }
-                tc_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * st);
-            }
-            // ---- results ----
-            const bool worked = !joint || m > st;
-            if (worked) {
-                if (alive) alive = tc_wait(o_full + 8 * st, o_par, a.status);
-                o_par ^= 1u;
+                segs[k % TC_SEGS] = g;
+                mbar_arrive(seg_full + 8 * (k % TC_SEGS));
             }
             __syncwarp();
-            tc_fence_after();
-            const float m2 = mx == -INFINITY ? -INFINITY : mx * a.scale2;
-            const int64_t item_start = w.pos - w.unit;
-            const bool complete = w.unit == 0 && m == w.it.u.count;
-            float M = m2, L = l, f0 = 1.f, f1 = 0.f;
-            if (joint) {
-                ml[st * TC_ROWS + r] = make_float2(m2, l);
-                tc_fence_before();
-                named_barrier(1, TC_SOFTMAX_THREADS);
-                tc_fence_after();
-                const float2 x = ml[r], y = ml[TC_ROWS + r];
-                M = fmaxf(x.x, y.x);
-                f0 = x.x == -INFINITY ? 0.f : ex2(x.x - M);
-                f1 = y.x == -INFINITY ? 0.f : ex2(y.x - M);
-                L = x.y * f0 + y.y * f1;
-            }
-            const int own_slot = 2 * blockIdx.x + (w.unit == 0 ? 1 : 0);
-            const int prow = joint ? r : st * TC_ROWS + r;
-            float *part = a.part + (int64_t)own_slot * TC_ITEM_ROWS * (D + 2);
-            // joint: each stream finishes half of the columns from both accumulators
-            const int c_first = joint ? st * (D / 64) : 0, c_last = joint ? c_first + D / 64 : D / 32;
-            for (int c = c_first; c < c_last; c++) {
-                float o[32];
-                if (joint) {
-                    float x[32];
-                    tc_ld32(tmem + C::O_COL + lanes + 32 * c, o);
-                    tc_ld_wait32(o);
-                    if (m > 1) {
-                        tc_ld32(tmem + C::O_COL + D + lanes + 32 * c, x);
-                        tc_ld_wait32(x);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = o[e] * f0 + x[e] * f1;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] *= f0;
-                    }
-                } else {
-                    tc_ld32(to + 32 * c, o);
-                    tc_ld_wait32(o);
-                }
-                if (valid) {
-                    if (complete) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float v[8];
-#pragma unroll
-                            for (int x = 0; x < 8; x++) v[x] = o[8 * e + x];
-                            paged_finish8<BF16>(a, D, token, head, 32 * c + 8 * e, M, L, v);
-                        }
-                    } else {
-                        float4 *dst = reinterpret_cast<float4 *>(part + (int64_t)prow * D + 32 * c);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                        if (c == c_first) *reinterpret_cast<float2 *>(part + (int64_t)TC_ITEM_ROWS * D + 2 * prow) = make_float2(M, L);
-                    }
-                }
-            }
-            tc_fence_before();
-            if (!complete) {
-                const int c0 = paged_owner(item_start, sh.total, sh.N), c1 = paged_owner(item_start + w.it.u.count - 1, sh.total, sh.N);
-                __threadfence();
-                named_barrier(1, TC_SOFTMAX_THREADS);
-                if (tid == 0) {
-                    const unsigned seen = atomicAdd(a.counters + c0, 1u);
-                    *last_word = seen == (unsigned)(c1 - c0);
-                    if (seen == (unsigned)(c1 - c0)) a.counters[c0] = 0;
-                }
-                named_barrier(1, TC_SOFTMAX_THREADS);
-                if (*last_word) {
-                    __threadfence();
-                    paged_merge<TC_SOFTMAX_THREADS, TC_ITEM_ROWS, BF16>(a, D, c0, c1, w.it.rows, [&](int x, int &t, int &h) { token_of(w.rt * TC_ITEM_ROWS + x, t, h); });
-                }
-            }
-            if (joint || !complete) named_barrier(1, TC_SOFTMAX_THREADS);  // the exchange, the accumulators and the flag are used again
+            if (end) break;
             w.next(a, sh);
-            if (w.pos >= sh.u1) break;
+        }
         }
     }
     tc_fence_before();
@@ -646,6 +719,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// Joins the parts of the items that share borders have cut: CTA (c, y) takes 256 groups of eight results of the item that begins in
+// share c, one thread each.  A launch of its own, since a single CTA reads the parts of a widely cut item (two hundred rows against a
+// long prefix: 2 MB) at a hundred GB/s: 95 us of 187 us when the last CTA to arrive did it (48 decode rows, prefix of 12345).
+constexpr int TC_JOIN_THREADS = 256;
+template <int D, bool BF16>
+__global__ void __launch_bounds__(TC_JOIN_THREADS) paged_tc_join_kernel(const __grid_constant__ PagedArgs a) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int c0 = blockIdx.x;
+    const TcSplit sp = reinterpret_cast<const TcSplit *>(a.counters)[c0];
+    const int i = blockIdx.y * TC_JOIN_THREADS + threadIdx.x, r = i / (D / 8), col = i % (D / 8) * 8;
+    if (r >= sp.rows) return;
+    float m, l, v[8];
+    paged_gather8<TC_ITEM_ROWS>(a, D, c0, sp.c1, r, col, m, l, v);
+    const int x = sp.row0 + r, t = x / a.G;
+    paged_finish8<BF16>(a, D, sp.q0 + t, sp.head * a.G + (x - t * a.G), col, m, l, v);
+}
+
 template <int D, bool BF16>
 cudaError_t launch_tc_t(const PagedArgs &a, const PagedMaps &maps, int box_rows, cudaStream_t st) {
     using C = TcCfg<D>;
@@ -653,11 +744,14 @@ cudaError_t launch_tc_t(const PagedArgs &a, const PagedMaps &maps, int box_rows,
     auto kernel = paged_tc_kernel<D, BF16>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3((unsigned)a.sms), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, box_rows);
+    const cudaError_t r = launch_pdl(kernel, dim3((unsigned)a.sms), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, box_rows);
+    if (r != cudaSuccess) return r;
+    return launch_pdl(paged_tc_join_kernel<D, BF16>, dim3((unsigned)a.sms, TC_ITEM_ROWS * D / 8 / TC_JOIN_THREADS), dim3(TC_JOIN_THREADS), 0, st, a);
 }
 
 }  // namespace
 
+int64_t paged_tc_words(int sms) { return (int64_t)sms * (sizeof(TcSplit) / 4); }
 int64_t paged_tc_part_floats(int d, int sms) { return (int64_t)2 * sms * TC_ITEM_ROWS * (d + 2); }
 
 cudaError_t launch_paged_tc(const PagedArgs &a, int dt, int d, const PagedMaps &maps, int box_rows, cudaStream_t st) {
