@@ -1610,6 +1610,20 @@ ttq_status paged_map(ttq_ctx *ctx, const ttq_paged *p, const ttq_kv_pages *kv, v
     return TTQ_OK;
 }
 
+// Map of the query rows as (element, head, token), copied in boxes of 64 elements x the G heads of a kv head x `tokens`.
+ttq_status paged_query_map(ttq_ctx *ctx, const ttq_paged *p, const void *q, int64_t ld, int64_t n_tokens, int tokens, CUtensorMap *map) {
+    const TensorMapEncode encode = tensor_map_encode();
+    if (!encode) return fail(ctx, TTQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[3] = {(cuuint64_t)p->d, (cuuint64_t)p->hq, (cuuint64_t)n_tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)p->d * 2, (cuuint64_t)ld * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)(p->hq / p->hkv), (cuuint32_t)tokens}, unit[3] = {1, 1, 1};
+    const CUresult r = encode(map, p->dt == TTQ_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(q), dims,
+                              strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ctx, TTQ_ERR_SHAPE, "the query rows cannot be mapped (cuTensorMapEncodeTiled: %d)", (int)r);
+    return TTQ_OK;
+}
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Checks of the pages and the batch that append and attention share; fills `a`.
@@ -1746,7 +1760,7 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
     if (!(scale > 0.f) || scale > 1e30f) return fail(ctx, TTQ_ERR_INVALID_ARG, "scale must be positive and finite");
     if (bt->n_seqs == 0 || bt->n_tokens == 0) return TTQ_OK;
     if (!q_dev || !out_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "q or out pointer is NULL");
-    if (ld_q < (int64_t)p->hq * p->d || ld_out < (int64_t)p->hq * p->d || ld_q % 8 || ld_out % 8)
+    if (ld_q < (int64_t)p->hq * p->d || ld_out < (int64_t)p->hq * p->d || ld_q % 8 || ld_out % 8 || ld_q >= (1ll << 39))
         return fail(ctx, TTQ_ERR_SHAPE, "ld_q and ld_out must be multiples of 8 and hold the heads of a row");
     if (!aligned16(q_dev) || !aligned16(out_dev)) return fail(ctx, TTQ_ERR_INVALID_ARG, "q and out must be 16-byte aligned");
     if (bt->prefix_len > 0 && bt->n_tokens > p->max_prefix_tokens)
@@ -1765,12 +1779,13 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
         a.pre_lse = p->pre_lse;
         // few rows per kv head: the memory-bound kernel; from 17 on the tensor-memory kernel
         const int64_t most = a.prefix_pass || bt->max_q == 0 ? bt->n_tokens : bt->max_q;
-        const bool few = most * a.G <= 16;
+        const bool few = most * a.G <= 16 || a.G > 128;
         a.counters = few ? p->counters : p->splits;
         const int slots = few ? 16 : (p->page_size < 128 ? p->page_size : 128);
         PagedMaps maps;
         ttq_status ms = paged_map(ctx, p, kv, kv->k_dev, slots, &maps.k);
         if (ms == TTQ_OK) ms = paged_map(ctx, p, kv, kv->v_dev, slots, &maps.v);
+        if (ms == TTQ_OK && !few) ms = paged_query_map(ctx, p, q_dev, ld_q, bt->n_tokens, 128 / a.G, &maps.q);
         if (ms != TTQ_OK) return ms;
         const cudaError_t e = few ? launch_paged_rows(a, p->dt, p->d, maps, (cudaStream_t)stream)
                                   : launch_paged_tc(a, p->dt, p->d, maps, slots, (cudaStream_t)stream);

@@ -279,7 +279,7 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *m
 }
 
 struct PagedMaps {
-    CUtensorMap k, v;
+    CUtensorMap k, v, q;  // q: the tensor-memory kernel only
 };
 // One launch of a pass (own keys, or the shared prefix's).
 cudaError_t launch_paged_rows(const PagedArgs &a, int dt, int d, const PagedMaps &maps, cudaStream_t st);

@@ -1,18 +1,19 @@
 // Attention over a paged cache on the tensor cores (tcgen05): prompts, pieces of prompts, and rows of a whole batch against a shared
 // prefix.
 //
-// An item is a tile of up to 256 rows (tokens x query heads of one kv head), walked in units of 128 keys.  Its two halves of 128
-// rows are two streams that take turns: while the softmax of one runs on the CUDA cores, the tensor core multiplies for the other.
+// An item is a tile of up to 2 x 128 rows -- twice floor(128 / G) tokens times the G query heads of one kv head -- walked in units of
+// 128 keys.  Its two halves are two streams that take turns: while the softmax of one runs on the CUDA cores, the tensor core multiplies for the other.
 //   S = Q K^T     128 x 128, Q and K in shared memory (K-major, 128-byte swizzle), S in tensor memory
 //   softmax       one thread per row: 128 scores from tensor memory, running maximum and sum in registers, weights in the 16-bit type
 //                 back into the columns that the scores had
 //   O += P V      P from tensor memory, V as it lies in its pages (keys as rows: the transposed operand form), O in tensor memory
-// An item of 128 rows or fewer gives both streams the same rows and every other unit of keys; the two results meet in tensor
+// An item of one half gives both streams the same rows and every other unit of keys; the two results meet in tensor
 // memory, whose lanes the warps of both streams reach.  Tensor memory is full: 2 x 128 columns of scores, 2 x d of output.
 //
-// Warps 0-3 and 4-7: softmax of the two streams, and their rows' queries and results.  Warp 8 issues the products, warp 9 the
-// tiled copies of the pages into a ring of slots, warp 10 walks the batch and hands the other warps one record per item (they keep
-// their registers for scores); warp 11 only fills the warpgroup.  Products of one CTA execute in the order of issue, so the scores of unit
+// Warps 0-3 and 4-7: softmax of the two streams, and their rows' results.  Warp 8 issues the products, warp 9 the tiled copies of the
+// pages into a ring of slots, warp 11 those of the queries (one copy per stream and 64 columns: the G heads of a run of tokens
+// are the rows of a tile as they lie), warp 10 walks the batch and hands the other warps one record per item, so that they keep their
+// registers for scores.  Products of one CTA execute in the order of issue, so the scores of unit
 // i + 1 may follow the product that reads the weights of unit i from the same columns, and a full score buffer means that
 // the output accumulator is at rest: the softmax warps rescale it in place, which they do only when the maximum has grown by 2^8.
 #include <climits>
@@ -26,6 +27,7 @@ namespace {
 constexpr int TC_UNIT = 128;       // keys per unit
 constexpr int TC_ROWS = 128;       // rows per stream
 constexpr int TC_ITEM_ROWS = 2 * TC_ROWS;
+constexpr int TC_QUERY_WARP = 11;
 constexpr int TC_MMA_WARP = 8, TC_TMA_WARP = 9, TC_WALK_WARP = 10;
 constexpr int TC_THREADS = 384, TC_SOFTMAX_THREADS = 256;
 // The block is launched with 168 registers a thread (65536 / 384, in steps of 8); a softmax thread, which holds a row of scores,
@@ -37,15 +39,17 @@ struct TcSeg {
     int m;                    // units (0: the share ends)
     int unit, u_sink, u_first;   // first unit; numbers of the item's units as PagedUnits has them
     int key_end, lo, sink;
-    int rows, row0, total_rows;  // valid rows, number of the first one in the sequence, rows of the sequence
+    int pair;                 // the streams have rows of their own
+    int tok0, n;              // first token of the item, tokens of the sequence
     int b, head, q0, pos0;
     int complete, slot;       // the item is whole; else where its partial goes
 };
-constexpr int TC_SEGS = 4, TC_SEG_READERS = 10;
+constexpr int TC_SEGS = 4, TC_SEG_READERS = 11;
 // An item that begins in one CTA's share and ends in CTA c1's (rows 0: none), left for the kernel that joins the parts.
 struct TcSplit {
-    int c1, rows, row0, q0, head;
+    int c1, rows, tok0, n, q0, head;
 };
+__device__ __forceinline__ int tc_tokens(const PagedArgs &a) { return TC_ROWS / a.G; }  // of a stream
 
 template <int D>
 struct TcCfg {
@@ -57,7 +61,7 @@ struct TcCfg {
     // shared memory: queries, ring, then barriers and exchange
     static constexpr int RING_AT = 2 * SLOT_BYTES;
     static constexpr int BAR_AT = RING_AT + SLOTS * SLOT_BYTES;
-    static constexpr int N_BARS = 2 * SLOTS + 8 + 1 + 2 * TC_SEGS;
+    static constexpr int N_BARS = 2 * SLOTS + 10 + 1 + 2 * TC_SEGS;
     static constexpr int ML_AT = BAR_AT + (N_BARS * 8 + 15) / 16 * 16;
     static constexpr int SEG_AT = ML_AT + 2 * TC_ROWS * 8;
     static constexpr int MISC_AT = SEG_AT + (TC_SEGS * (int)sizeof(TcSeg) + 15) / 16 * 16;
@@ -93,6 +97,13 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// rows of a stream's queries: (element of the head, head, token)
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap *map, int x, int head, int token, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
+        "r"(head), "r"(token), "r"(bar)
+        : "memory");
+}
 // 32 columns of this thread's lane
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, float *v) {
     uint32_t r[32];
@@ -117,16 +128,6 @@ __device__ __forceinline__ void tc_ld_wait32(float *v) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
-        "%30, %31, %32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
 __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(r[0]),
@@ -146,23 +147,76 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     }
 }
 
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]),
+          "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+// ---- pairs of floats -----------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair on the FMA pipe, x <= 127: x = n + f, |f| <= 1/2; 2^f by a polynomial of degree 4 with p(0) = 1 (least maximal relative
+// error under that condition, 2.8e-6, found by iterated weighted least squares); n added to the exponent.  Below -127, -inf
+// among them: zero.  The special-function unit alone (16 results a clock and SM) would need as long for a unit's
+// weights as the tensor core for its products; every TC_POLY_EVERY-th pair takes this way.
+constexpr int TC_POLY_EVERY = 4;
+__device__ __forceinline__ void ex2_poly(uint64_t x, float &e0, float &e1) {
+    constexpr float BIG = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
+    float x0, x1;
+    f2_split(x, x0, x1);
+    x = f2(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+    const uint64_t t = add2(x, f2(BIG, BIG)), n = add2(t, f2(-BIG, -BIG)), f = fma2(n, f2(-1.f, -1.f), x);
+    uint64_t p = fma2(f, f2(0.00958285f, 0.00958285f), f2(0.05590643f, 0.05590643f));
+    p = fma2(p, f, f2(0.24024099f, 0.24024099f));
+    p = fma2(p, f, f2(0.69312419f, 0.69312419f));
+    p = fma2(p, f, f2(1.f, 1.f));
+    float p0, p1, t0, t1;
+    f2_split(p, p0, p1);
+    f2_split(t, t0, t1);
+    e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
 // Row tile rt of a sequence: its rows, and the keys that any of them sees.
 struct TcItem {
     PagedSeq k;      // key_end, lo, sink of this item (the rest as the sequence's)
     PagedUnits u;
-    int rows;        // valid rows, from row 256 rt on
+    int tok0, tokens;
 };
-__device__ __forceinline__ int tc_tiles(const PagedArgs &a, int n) { return (n * a.G + TC_ITEM_ROWS - 1) / TC_ITEM_ROWS; }
+__device__ __forceinline__ int tc_tiles(const PagedArgs &a, int n) { return (n + 2 * tc_tokens(a) - 1) / (2 * tc_tokens(a)); }
 __device__ __forceinline__ TcItem tc_item(const PagedArgs &a, const PagedSeq &s, int rt) {
     TcItem it;
     it.k = s;
-    it.rows = min(TC_ITEM_ROWS, s.n * a.G - rt * TC_ITEM_ROWS);
+    it.tok0 = rt * 2 * tc_tokens(a);
+    it.tokens = min(2 * tc_tokens(a), s.n - it.tok0);
     if (!a.prefix_pass) {
-        const int i0 = rt * TC_ITEM_ROWS / a.G, i1 = (rt * TC_ITEM_ROWS + it.rows - 1) / a.G;  // first and last token
-        it.k.key_end = max(0, min(s.key_end, s.pos0 + i1 + 1 - a.prefix_len));
+        it.k.key_end = max(0, min(s.key_end, s.pos0 + it.tok0 + it.tokens - a.prefix_len));
         it.k.lo = it.k.sink = 0;
         if (a.window > 0) {
-            it.k.lo = max(0, min(it.k.key_end, s.pos0 + i0 - a.window + 1 - a.prefix_len));
+            it.k.lo = max(0, min(it.k.key_end, s.pos0 + it.tok0 - a.window + 1 - a.prefix_len));
             it.k.sink = max(0, min(it.k.lo, a.sinks - a.prefix_len));
         }
     }
@@ -249,14 +303,15 @@ struct TcWalk {
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ CUtensorMap kmap,
-                                                                 const __grid_constant__ CUtensorMap vmap, int box_rows) {
+                                                                 const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
+                                                                 int box_rows) {
     using C = TcCfg<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = smem_u32(smem);
     const uint32_t bars = base + C::BAR_AT;
     const uint32_t kv_full = bars, kv_empty = kv_full + 8 * C::SLOTS, q_full = kv_empty + 8 * C::SLOTS, s_full = q_full + 16, p_full = s_full + 16,
-                   o_full = p_full + 16, fix_bar = o_full + 16, seg_full = fix_bar + 8, seg_empty = seg_full + 8 * TC_SEGS;
+                   o_full = p_full + 16, q_empty = o_full + 16, fix_bar = q_empty + 16, seg_full = fix_bar + 8, seg_empty = seg_full + 8 * TC_SEGS;
     float2 *ml = reinterpret_cast<float2 *>(smem + C::ML_AT);
     TcSeg *segs = reinterpret_cast<TcSeg *>(smem + C::SEG_AT);
     int64_t *red = reinterpret_cast<int64_t *>(smem + C::MISC_AT);
@@ -268,7 +323,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             mbar_init(kv_empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(q_full + 8 * i, 4);
+            mbar_init(q_full + 8 * i, 1);
+            mbar_init(q_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_full + 8 * i, 4);
             mbar_init(o_full + 8 * i, 1);
@@ -329,47 +385,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         const int st = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the tensor memory's lanes
         const uint32_t ts = tmem + C::S_COL + st * TC_UNIT + lanes, to = tmem + C::O_COL + st * D + lanes;
+        const int r_tok = r / a.G, r_head = r - r_tok * a.G;
+        const int base_pos = a.prefix_pass ? 0 : a.prefix_len;
+        const uint64_t scale_2 = f2(a.scale2, a.scale2);
         bool alive = true;
         uint32_t s_par = 0, o_par = 0;
-        const int base_pos = a.prefix_pass ? 0 : a.prefix_len;
-        auto token_of = [&](const TcSeg &g, int x, int &token, int &head) {
-            const int i = x / a.G;
-            token = g.q0 + i;
-            head = g.head * a.G + (x - i * a.G);
-        };
-        auto first_row = [&](const TcSeg &g) { return g.row0 + (g.rows > TC_ROWS ? st * TC_ROWS : 0); };
-        // queries of an item into shared memory; the products that read the last item's are complete
-        auto load_queries = [&](const TcSeg &g) {
-            const int row0 = first_row(g), total_rows = g.total_rows;
-#pragma unroll 4
-            for (int c = r; c < TC_ROWS * (D / 8); c += TC_ROWS) {
-                const int row = c / (D / 8), ch = c % (D / 8);
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (row0 + row < total_rows) {
-                    int token, head;
-                    token_of(g, row0 + row, token, head);
-                    v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (int64_t)token * a.ld_q + (int64_t)head * D + 8 * ch);
-                }
-                sts128<0>(base + (uint32_t)(st * C::SLOT_BYTES + (ch >> 3) * C::HALF_BYTES + row * 128 + (((ch & 7) ^ (row & 7)) << 4)), v.x, v.y, v.z, v.w);
-            }
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_full + 8 * st);
-        };
-        bool have = seg_wait(0);
-        if (have && segs[0].m > 0) load_queries(segs[0]);
-        for (int k = 0; have; k++) {
+        for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
             const int m = g.m;
             if (m == 0) break;
-            const bool joint = g.rows <= TC_ROWS;   // both streams work on the same rows
-            const bool valid = first_row(g) + r < g.total_rows;
+            const bool joint = !g.pair;   // both streams work on the same rows
+            const int tok = g.tok0 + (joint ? 0 : st * tc_tokens(a)) + r_tok;
+            const bool valid = r_tok < tc_tokens(a) && tok < g.n;
             int pos = -1;
-            if (valid) {
-                int token, head;
-                token_of(g, first_row(g) + r, token, head);
-                pos = a.prefix_pass ? paged_row_pos(a, token) : g.pos0 + token - g.q0;
-            }
+            if (valid) pos = a.prefix_pass ? paged_row_pos(a, g.q0 + tok) : g.pos0 + tok;
             const int min_row = __reduce_min_sync(0xffffffffu, valid ? pos : INT_MAX), max_row = __reduce_max_sync(0xffffffffu, valid ? pos : -1);
             float mx = -INFINITY, l = 0.f;  // running maximum of the scores (unscaled) and sum
             const int step = joint ? 2 : 1;
@@ -394,38 +423,57 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     for (int kk = 0; kk < TC_UNIT; kk++)
                         if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
                 }
-                float top = s[0];
+                float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int kk = 1; kk < TC_UNIT; kk++) top = fmaxf(top, s[kk]);
+                for (int kk = 4; kk < TC_UNIT - 4; kk += 8)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) tops[x] = max3(tops[x], s[kk + x], s[kk + 4 + x]);
+#pragma unroll
+                for (int x = 0; x < 4; x++) tops[x] = fmaxf(tops[x], s[TC_UNIT - 4 + x]);
+                const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
                 const bool grow = (top - mx) * a.scale2 > 8.f || (mx == -INFINITY && top > -INFINITY);
                 if (__any_sync(0xffffffffu, grow)) {
                     const float next = fmaxf(mx, top), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
                     mx = next;
                     l *= f;
                     if (i >= step) {  // (the first unit starts the accumulator)
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; c++) {
+                            float o[16];
+                            tc_ld16(to + 16 * c, o);
+                            uint32_t q[16];
 #pragma unroll
-                        for (int c = 0; c < D / 32; c++) {
-                            float o[32];
-                            tc_ld32(to + 32 * c, o);
-                            tc_ld_wait32(o);
-                            uint32_t q[32];
-#pragma unroll
-                            for (int x = 0; x < 32; x++) q[x] = __float_as_uint(o[x] * f);
-                            tc_st32(to + 32 * c, q);
+                            for (int x = 0; x < 16; x++) q[x] = __float_as_uint(o[x] * f);
+                            tc_st16(to + 16 * c, q);
                         }
                     }
                 }
-                const float off = mx == -INFINITY ? 0.f : mx * a.scale2;
+                const float off = mx == -INFINITY ? 0.f : -mx * a.scale2;
+                const uint64_t off_2 = f2(off, off);
+                uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     uint32_t q[16];
 #pragma unroll
                     for (int x = 0; x < 16; x++) {
-                        const float e0 = ex2(fmaf(s[32 * c + 2 * x], a.scale2, -off)), e1 = ex2(fmaf(s[32 * c + 2 * x + 1], a.scale2, -off));
-                        l += e0 + e1;
+                        const uint64_t y = fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale_2, off_2);
+                        float e0, e1;
+                        if (x % TC_POLY_EVERY == TC_POLY_EVERY - 1) {
+                            ex2_poly(y, e0, e1);
+                        } else {
+                            f2_split(y, e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                        }
+                        sums[x & 1] = add2(sums[x & 1], f2(e0, e1));
                         q[x] = pack2<BF16>(e0, e1);
                     }
                     tc_st16(ts + 16 * c, q);
+                }
+                {
+                    float x, y;
+                    f2_split(add2(sums[0], sums[1]), x, y);
+                    l += x + y;
                 }
                 tc_st_wait();
                 tc_fence_before();
@@ -433,15 +481,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 if (lane == 0) mbar_arrive(p_full + 8 * st);
             }
             // ---- results ----
-            const bool worked = !joint || m > st;
-            // the next item's first scores are computed under this one's end (a stream without a unit waits for the other: its queries'
-            // barrier may be one phase ahead of the product warp, not two)
-            auto prefetch = [&]() {
-                have = seg_wait(k + 1);
-                if (have && segs[(k + 1) % TC_SEGS].m > 0) load_queries(segs[(k + 1) % TC_SEGS]);
-            };
-            if (worked) {
-                prefetch();
+            if (!joint || m > st) {
                 if (alive) alive = tc_wait(o_full + 8 * st, o_par, a.status);
                 o_par ^= 1u;
             }
@@ -449,8 +489,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             tc_fence_after();
             const float m2 = mx == -INFINITY ? -INFINITY : mx * a.scale2;
             const bool complete = g.complete;
-            int token, head;
-            token_of(g, first_row(g) + r, token, head);
+            const int token = g.q0 + tok, head = g.head * a.G + r_head;
             float M = m2, L = l, f0 = 1.f, f1 = 0.f;
             if (joint) {
                 ml[st * TC_ROWS + r] = make_float2(m2, l);
@@ -467,6 +506,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             float *part = a.part + (int64_t)g.slot * TC_ITEM_ROWS * (D + 2);
             // joint: each stream finishes half of the columns from both accumulators
             const int c_first = joint ? st * (D / 64) : 0, c_last = joint ? c_first + D / 64 : D / 32;
+#pragma unroll 1
             for (int c = c_first; c < c_last; c++) {
                 float o[32];
                 if (joint) {
@@ -505,7 +545,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             }
             tc_fence_before();
             if (joint) named_barrier(1, TC_SOFTMAX_THREADS);  // the exchange and the other's accumulator are used again
-            if (!worked) prefetch();
             seg_done(k);
         }
     } else {
@@ -587,7 +626,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             u_sink = g.u_sink; u_first = g.u_first;
             head = g.head; seq = g.b;
             const int u0 = g.unit;
-            const bool pair = g.rows > TC_ROWS;
+            const bool pair = g.pair;
             seg_done(k);
             if (pair) {   // both streams take every unit
                 for (int i = 0; i < m; i++) {
@@ -608,14 +647,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         // ------------------------------------------------------------------------------------------ products
         bool alive = true;
         int n = 0;                                   // slots consumed
-        uint32_t q_par = 0, p_par[2] = {0u, 0u};
+        uint32_t q_par[2] = {0u, 0u}, p_par[2] = {0u, 0u};
         constexpr uint32_t idesc_s = tc_idesc<BF16>(TC_UNIT, false), idesc_o = tc_idesc<BF16>(D, true);
         auto slot_addr = [&](int i) { return base + C::RING_AT + (uint32_t)(i % C::SLOTS) * C::SLOT_BYTES; };
         auto wait_slot = [&](int i) {
             if (alive) alive = tc_wait(kv_full + 8 * (i % C::SLOTS), (uint32_t)((i / C::SLOTS) & 1), a.status);
         };
-        // S of stream st from the K in slot i; `release`: the slot's last use
-        auto scores = [&](int st, int i, bool release) {
+        // S of stream st from the K in slot i; `release`: the slot's last use, `last`: the queries'
+        auto scores = [&](int st, int i, bool release, bool last) {
             wait_slot(i);
             __syncwarp();
             tc_fence_after();
@@ -629,6 +668,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                         tc_mma_ss(d, qd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), kd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), idesc_s,
                                   h + kk > 0 ? 1u : 0u);
                 umma_commit(s_full + 8 * st);
+                if (last) umma_commit(q_empty + 8 * st);
                 if (release) umma_commit(kv_empty + 8 * (i % C::SLOTS));
             }
             __syncwarp();
@@ -653,30 +693,57 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             const TcSeg &g = segs[k % TC_SEGS];
             const int m = g.m;
             if (m == 0) break;
-            const bool pair = g.rows > TC_ROWS;
+            const bool pair = g.pair;
             seg_done(k);
-            for (int st = 0; st < 2; st++)
-                if (alive) alive = tc_wait(q_full + 8 * st, q_par, a.status);
-            q_par ^= 1u;
+            const int streams = pair || m > 1 ? 2 : 1;
+            for (int st = 0; st < streams; st++) {
+                if (alive) alive = tc_wait(q_full + 8 * st, q_par[st], a.status);
+                q_par[st] ^= 1u;
+            }
             if (pair) {
-                scores(0, n, false);
-                scores(1, n, true);
+                scores(0, n, false, m == 1);
+                scores(1, n, true, m == 1);
                 n++;
                 for (int i = 0; i < m; i++) {
                     const bool more = i + 1 < m;
                     output(0, n, i == 0, !more, false);
-                    if (more) scores(0, n + 1, false);
+                    if (more) scores(0, n + 1, false, i + 2 == m);
                     output(1, n, i == 0, !more, true);
-                    if (more) scores(1, n + 1, true);
+                    if (more) scores(1, n + 1, true, i + 2 == m);
                     n += more ? 2 : 1;
                 }
             } else {
-                scores(0, n++, true);
-                if (m > 1) scores(1, n++, true);
+                scores(0, n++, true, m <= 2);
+                if (m > 1) scores(1, n++, true, m <= 3);
                 for (int i = 0; i < m; i++) {
                     output(i & 1, n++, i < 2, i + 2 >= m, true);
-                    if (i + 2 < m) scores(i & 1, n++, true);
+                    if (i + 2 < m) scores(i & 1, n++, true, i + 4 >= m);
                 }
+            }
+        }
+    } else if (warp == TC_QUERY_WARP) {
+        // ------------------------------------------------------------------------------------------ queries
+        bool alive = true;
+        int used[2] = {0, 0};
+        const uint32_t bytes = (uint32_t)(tc_tokens(a) * a.G * 128 * C::HALVES);
+        for (int k = 0; seg_wait(k); k++) {
+            const TcSeg &g = segs[k % TC_SEGS];
+            const int m = g.m, token = g.q0 + g.tok0, head = g.head * a.G;
+            const bool pair = g.pair;
+            if (m == 0) break;
+            seg_done(k);
+            // (a stream without a unit gets none: the product warp waits for none)
+            for (int st = 0; st < (pair || m > 1 ? 2 : 1); st++) {
+                if (used[st] > 0 && alive) alive = tc_wait(q_empty + 8 * st, (uint32_t)((used[st] - 1) & 1), a.status);
+                used[st]++;
+                __syncwarp();
+                if (elect_one()) {
+                    mbar_expect_tx(q_full + 8 * st, bytes);
+#pragma unroll
+                    for (int h = 0; h < C::HALVES; h++)
+                        tma_load_rows(base + (uint32_t)(st * C::SLOT_BYTES + h * C::HALF_BYTES), &qmap, 64 * h, head, token + (pair ? st * tc_tokens(a) : 0), q_full + 8 * st);
+                }
+                __syncwarp();
             }
         }
     } else if (warp == TC_WALK_WARP) {
@@ -692,14 +759,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     g.m = w.here(sh);
                     g.unit = w.unit; g.u_sink = w.it.u.sink; g.u_first = w.it.u.first;
                     g.key_end = w.it.k.key_end; g.lo = w.it.k.lo; g.sink = w.it.k.sink;
-                    g.rows = w.it.rows; g.row0 = w.rt * TC_ITEM_ROWS; g.total_rows = w.s.n * a.G;
+                    g.pair = w.it.tokens > tc_tokens(a);
+                    g.tok0 = w.it.tok0; g.n = w.s.n;
                     g.b = w.b; g.head = w.head; g.q0 = w.s.q0; g.pos0 = w.s.pos0;
                     const int64_t first = w.pos - w.unit;
                     g.complete = g.m == w.it.u.count;
                     g.slot = 2 * (int)blockIdx.x + (w.unit == 0 ? 1 : 0);
                     // an item that begins here and goes on elsewhere is the share's last
                     if (w.unit == 0 && !g.complete)
-                        splits[blockIdx.x] = {paged_owner(first + w.it.u.count - 1, sh.total, sh.N), g.rows, g.row0, g.q0, g.head};
+                        splits[blockIdx.x] = {paged_owner(first + w.it.u.count - 1, sh.total, sh.N), g.pair ? TC_ITEM_ROWS : TC_ROWS, g.tok0, g.n, g.q0, g.head};
                     else if (w.pos + g.m >= sh.u1)
                         splits[blockIdx.x].rows = 0;
                 }
@@ -731,10 +799,11 @@ __global__ void __launch_bounds__(TC_JOIN_THREADS) paged_tc_join_kernel(const __
     const TcSplit sp = reinterpret_cast<const TcSplit *>(a.counters)[c0];
     const int i = blockIdx.y * TC_JOIN_THREADS + threadIdx.x, r = i / (D / 8), col = i % (D / 8) * 8;
     if (r >= sp.rows) return;
+    const int rr = r % TC_ROWS, t = rr / a.G, tok = sp.tok0 + r / TC_ROWS * tc_tokens(a) + t;
+    if (t >= tc_tokens(a) || tok >= sp.n) return;
     float m, l, v[8];
     paged_gather8<TC_ITEM_ROWS>(a, D, c0, sp.c1, r, col, m, l, v);
-    const int x = sp.row0 + r, t = x / a.G;
-    paged_finish8<BF16>(a, D, sp.q0 + t, sp.head * a.G + (x - t * a.G), col, m, l, v);
+    paged_finish8<BF16>(a, D, sp.q0 + tok, sp.head * a.G + (rr - t * a.G), col, m, l, v);
 }
 
 template <int D, bool BF16>
@@ -744,7 +813,7 @@ cudaError_t launch_tc_t(const PagedArgs &a, const PagedMaps &maps, int box_rows,
     auto kernel = paged_tc_kernel<D, BF16>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
-    const cudaError_t r = launch_pdl(kernel, dim3((unsigned)a.sms), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, box_rows);
+    const cudaError_t r = launch_pdl(kernel, dim3((unsigned)a.sms), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, maps.q, box_rows);
     if (r != cudaSuccess) return r;
     return launch_pdl(paged_tc_join_kernel<D, BF16>, dim3((unsigned)a.sms, TC_ITEM_ROWS * D / 8 / TC_JOIN_THREADS), dim3(TC_JOIN_THREADS), 0, st, a);
 }
