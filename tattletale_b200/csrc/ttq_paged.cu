@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     grid_launch_dependents();
     grid_dependency_wait();
 
-    const PagedShare sh = paged_share<ROWS_THREADS>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
+    const PagedShare sh = paged_share<ROWS_THREADS, 1>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
         if (!ok) return 0;
         const PagedSeq s = paged_seq(a, b, min_pos);
         return s.n > 0 ? (int64_t)rows_items(a, s.n) * paged_units<ROWS_UNIT>(s).count : 0;

@@ -3,7 +3,7 @@
 //
 // The rows of a sequence that attend with one kv head are its new tokens times the G = hq / hkv query heads of that kv head, row
 // r = token r / G, head r % G: K and V are read once for all of them.  An item is a tile of such rows; its keys are walked in
-// units of a fixed number of keys.  All units of a call are numbered through -- sequence, row tile, kv head, unit -- and every CTA
+// units of a fixed number of keys.  All units of a call are numbered through (the tensor-memory kernel: weighted) -- sequence, row tile, kv head, unit -- and every CTA
 // takes an equal, contiguous share of the numbers, found from the lengths in device memory by each CTA for itself (a captured graph
 // follows them, the host never waits).  An item that one CTA sees whole is finished there; of an item cut by share borders
 // every CTA leaves a partial result (running maximum, sum, unnormalised output) in the plan's workspace, at most two per CTA
@@ -131,8 +131,14 @@ struct PagedShare {
     int min_pos;     // prefix pass: smallest position of any token
 };
 
+// Shares of at least MIN_SHARE numbers each, at most one per CTA.
+template <int MIN_SHARE>
+__device__ __forceinline__ int paged_shares(int64_t total) {
+    const int64_t most = total / MIN_SHARE;
+    return total == 0 ? 0 : (int)(most < 1 ? 1 : (most < gridDim.x ? most : gridDim.x));
+}
 // Called by all THREADS of the CTA.  `cost(b, ok, min_pos)`: units of sequence b (ok false: none), whole warps at a time.  red: shared, at least THREADS / 32 + 4 int64.
-template <int THREADS, class Cost>
+template <int THREADS, int MIN_SHARE, class Cost>
 __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *red, Cost &&cost) {
     constexpr int W = THREADS / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -174,7 +180,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
             }
             if (nb <= THREADS) {
                 total = chunk;
-                sh.N = (int)(total < gridDim.x ? total : gridDim.x);
+                sh.N = paged_shares<MIN_SHARE>(total);
                 u0 = (int)blockIdx.x < sh.N ? total * blockIdx.x / sh.N : total;
                 pass = 1;
             }
@@ -188,7 +194,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
         }
         if (pass == 0) {
             total = running;
-            sh.N = (int)(total < gridDim.x ? total : gridDim.x);
+            sh.N = paged_shares<MIN_SHARE>(total);
             u0 = (int)blockIdx.x < sh.N ? total * blockIdx.x / sh.N : total;
         }
     }

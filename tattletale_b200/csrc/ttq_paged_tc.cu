@@ -10,10 +10,11 @@
 // An item of one half gives both streams the same rows and every other unit of keys; the two results meet in tensor
 // memory, whose lanes the warps of both streams reach.  Tensor memory is full: 2 x 128 columns of scores, 2 x d of output.
 //
-// Warps 0-3 and 4-7: softmax of the two streams, and their rows' results.  Warp 8 issues the products, warp 9 the tiled copies of the
-// pages into a ring of slots, warp 11 those of the queries (one copy per stream and 64 columns: the G heads of a run of tokens
-// are the rows of a tile as they lie), warp 10 walks the batch and hands the other warps one record per item, so that they keep their
-// registers for scores.  Products of one CTA execute in the order of issue, so the scores of unit
+// Warps 0-3 and 4-7: softmax of the two streams, and their rows' results.  Warps 8 and 11 issue the streams' products -- one
+// warp for both would leave the tensor core idle during its waits, since the issue of a product blocks until the queue before it has
+// drained -- warp 9 the tiled copies of the pages into a ring of slots.  Warp 10 walks the batch, hands the other warps one
+// record per item, so that they keep their registers for scores, and copies the queries (one copy per stream and 64 columns: the
+// G heads of a run of tokens are the rows of a tile as they lie).  Products of one CTA execute in the order of issue, so the scores of unit
 // i + 1 may follow the product that reads the weights of unit i from the same columns, and a full score buffer means that
 // the output accumulator is at rest: the softmax warps rescale it in place, which they do only when the maximum has grown by 2^8.
 #include <climits>
@@ -27,8 +28,7 @@ namespace {
 constexpr int TC_UNIT = 128;       // keys per unit
 constexpr int TC_ROWS = 128;       // rows per stream
 constexpr int TC_ITEM_ROWS = 2 * TC_ROWS;
-constexpr int TC_QUERY_WARP = 11;
-constexpr int TC_MMA_WARP = 8, TC_TMA_WARP = 9, TC_WALK_WARP = 10;
+constexpr int TC_MMA_WARP = 8, TC_TMA_WARP = 9, TC_WALK_WARP = 10, TC_MMA1_WARP = 11;
 constexpr int TC_THREADS = 384, TC_SOFTMAX_THREADS = 256;
 // The block is launched with 168 registers a thread (65536 / 384, in steps of 8); a softmax thread, which holds a row of scores,
 // gets 208, a thread of the third warpgroup keeps 88: 8 x 208 + 4 x 88 = 12 x 168.
@@ -44,7 +44,7 @@ struct TcSeg {
     int b, head, q0, pos0;
     int complete, slot;       // the item is whole; else where its partial goes
 };
-constexpr int TC_SEGS = 4, TC_SEG_READERS = 11;
+constexpr int TC_SEGS = 4, TC_SEG_READERS = 11;  // (8 softmax warps, copies, two product warps)
 // An item that begins in one CTA's share and ends in CTA c1's (rows 0: none), left for the kernel that joins the parts.
 struct TcSplit {
     int c1, rows, tok0, n, q0, head;
@@ -56,11 +56,12 @@ struct TcCfg {
     static constexpr int HALVES = D / 64;
     static constexpr int HALF_BYTES = 128 * 128;               // 128 rows x 64 elements
     static constexpr int SLOT_BYTES = HALVES * HALF_BYTES;     // a unit of K or of V; a stream's queries
-    static constexpr int SLOTS = D == 128 ? 5 : 10;
+    static constexpr int SLOTS = D == 128 ? 4 : 8;             // a fifth (tenth) changed nothing; its room is the results'
     static constexpr int S_COL = 0, O_COL = 256;               // streams 128 columns, resp. D columns apart
-    // shared memory: queries, ring, then barriers and exchange
+    // shared memory: queries, ring, 4 KB per softmax warp through which results leave, then barriers and exchange
     static constexpr int RING_AT = 2 * SLOT_BYTES;
-    static constexpr int BAR_AT = RING_AT + SLOTS * SLOT_BYTES;
+    static constexpr int OUT_AT = RING_AT + SLOTS * SLOT_BYTES;
+    static constexpr int BAR_AT = OUT_AT + 8 * 4096;
     static constexpr int N_BARS = 2 * SLOTS + 10 + 1 + 2 * TC_SEGS;
     static constexpr int ML_AT = BAR_AT + (N_BARS * 8 + 15) / 16 * 16;
     static constexpr int SEG_AT = ML_AT + 2 * TC_ROWS * 8;
@@ -178,33 +179,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of a pair on the FMA pipe, x <= 127: x = n + f, |f| <= 1/2; 2^f by a polynomial of degree 4 with p(0) = 1 (least maximal relative
-// error under that condition, 2.8e-6, found by iterated weighted least squares); n added to the exponent.  Below -127, -inf
-// among them: zero.  The special-function unit alone (16 results a clock and SM) would need as long for a unit's
-// weights as the tensor core for its products; every TC_POLY_EVERY-th pair takes this way.
-constexpr int TC_POLY_EVERY = 4;
-__device__ __forceinline__ void ex2_poly(uint64_t x, float &e0, float &e1) {
-    constexpr float BIG = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits
-    float x0, x1;
-    f2_split(x, x0, x1);
-    x = f2(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
-    const uint64_t t = add2(x, f2(BIG, BIG)), n = add2(t, f2(-BIG, -BIG)), f = fma2(n, f2(-1.f, -1.f), x);
-    uint64_t p = fma2(f, f2(0.00958285f, 0.00958285f), f2(0.05590643f, 0.05590643f));
-    p = fma2(p, f, f2(0.24024099f, 0.24024099f));
-    p = fma2(p, f, f2(0.69312419f, 0.69312419f));
-    p = fma2(p, f, f2(1.f, 1.f));
-    float p0, p1, t0, t1;
-    f2_split(p, p0, p1);
-    f2_split(t, t0, t1);
-    e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-    e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
+// How the work is numbered: a unit of keys counts once for an item of one stream, twice for one of two; an item's start and end
+// count like TC_ITEM_WEIGHT of them.
+constexpr int TC_PAIR_WEIGHT = 2, TC_ITEM_WEIGHT = 4;
 // Row tile rt of a sequence: its rows, and the keys that any of them sees.
 struct TcItem {
     PagedSeq k;      // key_end, lo, sink of this item (the rest as the sequence's)
     PagedUnits u;
     int tok0, tokens;
+    int weight, size;   // numbers of a unit and of the whole item
+    // units whose number is below p; unit i stands at TC_ITEM_WEIGHT + i * weight
+    __device__ __forceinline__ int units_before(int p) const { return max(0, min(u.count, (p - TC_ITEM_WEIGHT + weight - 1) / weight)); }
 };
 __device__ __forceinline__ int tc_tiles(const PagedArgs &a, int n) { return (n + 2 * tc_tokens(a) - 1) / (2 * tc_tokens(a)); }
 __device__ __forceinline__ TcItem tc_item(const PagedArgs &a, const PagedSeq &s, int rt) {
@@ -221,13 +206,15 @@ __device__ __forceinline__ TcItem tc_item(const PagedArgs &a, const PagedSeq &s,
         }
     }
     it.u = paged_units<TC_UNIT>(it.k);
+    it.weight = it.tokens > tc_tokens(a) ? TC_PAIR_WEIGHT : 1;
+    it.size = TC_ITEM_WEIGHT + it.u.count * it.weight;
     return it;
 }
-// Units of one kv head's items of a sequence, by the whole warp (`s`: the same in all lanes).
+// Numbers of one kv head's items of a sequence, by the whole warp (`s`: the same in all lanes).
 __device__ __forceinline__ int64_t tc_seq_units(const PagedArgs &a, const PagedSeq &s, int lane) {
     const int nt = tc_tiles(a, s.n);
     int64_t sum = 0;
-    for (int rt = lane; rt < nt; rt += 32) sum += tc_item(a, s, rt).u.count;
+    for (int rt = lane; rt < nt; rt += 32) sum += tc_item(a, s, rt).size;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum;
@@ -238,8 +225,8 @@ struct TcWalk {
     PagedSeq s;
     TcItem it;
     int b, head, rt, nt;
-    int unit;        // of the item
-    int64_t pos;     // number of that unit
+    int at;          // number within the item
+    int64_t pos;     // the same, of the call
 
     __device__ __forceinline__ void enter(const PagedArgs &a, int min_pos) {
         const int nb = a.prefix_pass ? 1 : a.B;
@@ -248,10 +235,10 @@ struct TcWalk {
             if (s.n > 0) break;
         }
         nt = tc_tiles(a, s.n);
-        head = rt = unit = 0;
+        head = rt = at = 0;
         it = tc_item(a, s, 0);
     }
-    // to the unit `off` units behind the sequence's first (the whole warp)
+    // to the share's first number (the whole warp)
     __device__ __forceinline__ void start(const PagedArgs &a, const PagedShare &sh, int lane) {
         b = sh.b;
         enter(a, sh.min_pos);
@@ -260,7 +247,7 @@ struct TcWalk {
         head = (int)(off / per_head);
         off -= head * per_head;
         for (int base = 0;; base += 32) {
-            const int c = base + lane < nt ? tc_item(a, s, base + lane).u.count : 0;
+            const int c = base + lane < nt ? tc_item(a, s, base + lane).size : 0;
             int incl = c;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -271,7 +258,7 @@ struct TcWalk {
             if (hit) {
                 const int l = __ffs(hit) - 1;
                 rt = base + l;
-                unit = (int)off - __shfl_sync(0xffffffffu, incl - c, l);
+                at = (int)off - __shfl_sync(0xffffffffu, incl - c, l);
                 break;
             }
             if (base + 32 >= nt) break;  // (not reached)
@@ -280,14 +267,14 @@ struct TcWalk {
         it = tc_item(a, s, rt);
         pos = sh.u0;
     }
-    // units of this item in the share
+    // numbers of this item in the share
     __device__ __forceinline__ int here(const PagedShare &sh) const {
         const int64_t left = sh.u1 - pos;
-        return (int)(left < it.u.count - unit ? left : it.u.count - unit);
+        return (int)(left < it.size - at ? left : it.size - at);
     }
     __device__ __forceinline__ void next(const PagedArgs &a, const PagedShare &sh) {
         pos += here(sh);
-        unit = 0;
+        at = 0;
         if (pos >= sh.u1) return;
         if (++rt == nt) {
             rt = 0;
@@ -320,7 +307,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
     if (tid == 0) {
         for (int i = 0; i < C::SLOTS; i++) {
             mbar_init(kv_full + 8 * i, 1);
-            mbar_init(kv_empty + 8 * i, 1);
+            mbar_init(kv_empty + 8 * i, 2);  // one arrival per stream, two of the only one that takes the slot
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(q_full + 8 * i, 1);
@@ -338,13 +325,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
     }
     grid_launch_dependents();
     grid_dependency_wait();
-    const PagedShare sh = paged_share<TC_THREADS>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
+    const PagedShare sh = paged_share<TC_THREADS, TC_PAIR_WEIGHT>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
         PagedSeq s{};
         if (ok) s = paged_seq(a, b, min_pos);
         const int nt = ok ? tc_tiles(a, s.n) : 0;
         int64_t units = 0;
         if (nt <= 2)
-            for (int rt = 0; rt < nt; rt++) units += tc_item(a, s, rt).u.count;
+            for (int rt = 0; rt < nt; rt++) units += tc_item(a, s, rt).size;
         // long prompts: the warp's lanes share the row tiles
         for (unsigned many = __ballot_sync(0xffffffffu, nt > 2); many; many &= many - 1) {
             const int l = __ffs(many) - 1;
@@ -458,13 +445,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     for (int x = 0; x < 16; x++) {
                         const uint64_t y = fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale_2, off_2);
                         float e0, e1;
-                        if (x % TC_POLY_EVERY == TC_POLY_EVERY - 1) {
-                            ex2_poly(y, e0, e1);
-                        } else {
-                            f2_split(y, e0, e1);
-                            e0 = ex2(e0);
-                            e1 = ex2(e1);
-                        }
+                        f2_split(y, e0, e1);
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
                         sums[x & 1] = add2(sums[x & 1], f2(e0, e1));
                         q[x] = pack2<BF16>(e0, e1);
                     }
@@ -502,46 +485,87 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 f1 = y.x == -INFINITY ? 0.f : ex2(y.x - M);
                 L = x.y * f0 + y.y * f1;
             }
-            const int prow = joint ? r : st * TC_ROWS + r;
+            // what the row's accumulator is multiplied by (0: the other stream's too), and its share of the shared prefix's result
+            float w0 = f0, w1 = f1, wp = 0.f;
+            if (complete) {
+                float inv = L > 0.f ? 1.f / L : 0.f;
+                if (a.prefix_pass) {
+                    if (valid && (!joint || st == 0)) a.pre_lse[(int64_t)token * a.hq + head] = L > 0.f ? M + log2f(L) : -INFINITY;
+                } else if (a.pre_o != nullptr && valid) {
+                    const float lse = a.pre_lse[(int64_t)token * a.hq + head];
+                    if (lse != -INFINITY) {
+                        const float top = fmaxf(M, lse), own = M == -INFINITY ? 0.f : ex2(M - top), pre = ex2(lse - top);
+                        inv = 1.f / (L * own + pre);
+                        wp = pre * inv;
+                        inv *= own;
+                    }
+                }
+                w0 *= inv;
+                w1 *= inv;
+            }
             float *part = a.part + (int64_t)g.slot * TC_ITEM_ROWS * (D + 2);
-            // joint: each stream finishes half of the columns from both accumulators
+            if (!complete && valid && (!joint || st == 0))
+                *reinterpret_cast<float2 *>(part + (int64_t)TC_ITEM_ROWS * D + 2 * (joint ? r : st * TC_ROWS + r)) = make_float2(M, L);
+            // 32 columns at a time through the warp's 4 KB (16-byte chunks, swizzled), then four rows of 128 bytes per instruction: a store by
+            // the row's own thread would touch 32 lines.  Joint: each stream finishes half of the columns from both accumulators.
+            const uint32_t stage = base + C::OUT_AT + (uint32_t)warp * 4096u;
             const int c_first = joint ? st * (D / 64) : 0, c_last = joint ? c_first + D / 64 : D / 32;
+            const int my_token = valid ? token : -1, width = complete && !a.prefix_pass ? 2 : 4;
+            uint8_t *dst[8];    // where this lane's part of rows 4 e + lane / 8 goes
+            float pw[8];
+            int prow[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int rr = 4 * e + (lane >> 3), t = __shfl_sync(0xffffffffu, my_token, rr), hd = __shfl_sync(0xffffffffu, head, rr);
+                pw[e] = __shfl_sync(0xffffffffu, wp, rr);
+                prow[e] = t * a.hq + hd;
+                uint8_t *row;
+                if (!complete) row = reinterpret_cast<uint8_t *>(part + (int64_t)((joint ? 0 : st * TC_ROWS) + (warp & 3) * 32 + rr) * D);
+                else if (a.prefix_pass) row = reinterpret_cast<uint8_t *>(a.pre_o + (int64_t)prow[e] * D);
+                else row = reinterpret_cast<uint8_t *>(reinterpret_cast<uint16_t *>(a.out) + (int64_t)t * a.ld_out + (int64_t)hd * D);
+                dst[e] = t < 0 ? nullptr : row + 4 * (lane & 7) * width;
+            }
+            const bool with_prefix = __any_sync(0xffffffffu, wp != 0.f);
 #pragma unroll 1
             for (int c = c_first; c < c_last; c++) {
                 float o[32];
-                if (joint) {
+                tc_ld32(joint ? tmem + C::O_COL + lanes + 32 * c : to + 32 * c, o);
+                tc_ld_wait32(o);
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] *= w0;
+                if (joint && m > 1) {
                     float x[32];
-                    tc_ld32(tmem + C::O_COL + lanes + 32 * c, o);
-                    tc_ld_wait32(o);
-                    if (m > 1) {
-                        tc_ld32(tmem + C::O_COL + D + lanes + 32 * c, x);
-                        tc_ld_wait32(x);
+                    tc_ld32(tmem + C::O_COL + D + lanes + 32 * c, x);
+                    tc_ld_wait32(x);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = o[e] * f0 + x[e] * f1;
-                    } else {
+                    for (int e = 0; e < 32; e++) o[e] = fmaf(x[e], w1, o[e]);
+                }
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] *= f0;
-                    }
+                for (int e = 0; e < 8; e++) sts128f<0>(stage + lane * 128 + ((e ^ (lane & 7)) << 4), o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                __syncwarp();
+                float4 v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = lds128f<0>(stage + (4 * e + (lane >> 3)) * 128 + (((lane & 7) ^ ((4 * e + (lane >> 3)) & 7)) << 4));
+                if (with_prefix) {
+                    float4 x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (dst[e] != nullptr && pw[e] != 0.f) x[e] = *reinterpret_cast<const float4 *>(a.pre_o + (int64_t)prow[e] * D + 32 * c + 4 * (lane & 7));
+                        else x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        v[e] = make_float4(fmaf(x[e].x, pw[e], v[e].x), fmaf(x[e].y, pw[e], v[e].y), fmaf(x[e].z, pw[e], v[e].z), fmaf(x[e].w, pw[e], v[e].w));
+                }
+                if (width == 2) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (dst[e] != nullptr) *reinterpret_cast<uint2 *>(dst[e] + 64 * c) = make_uint2(pack2<BF16>(v[e].x, v[e].y), pack2<BF16>(v[e].z, v[e].w));
                 } else {
-                    tc_ld32(to + 32 * c, o);
-                    tc_ld_wait32(o);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (dst[e] != nullptr) *reinterpret_cast<float4 *>(dst[e] + 128 * c) = v[e];
                 }
-                if (valid) {
-                    if (complete) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float v[8];
-#pragma unroll
-                            for (int x = 0; x < 8; x++) v[x] = o[8 * e + x];
-                            paged_finish8<BF16>(a, D, token, head, 32 * c + 8 * e, M, L, v);
-                        }
-                    } else {
-                        float4 *dst = reinterpret_cast<float4 *>(part + (int64_t)prow * D + 32 * c);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                        if (c == c_first) *reinterpret_cast<float2 *>(part + (int64_t)TC_ITEM_ROWS * D + 2 * prow) = make_float2(M, L);
-                    }
-                }
+                __syncwarp();
             }
             tc_fence_before();
             if (joint) named_barrier(1, TC_SOFTMAX_THREADS);  // the exchange and the other's accumulator are used again
@@ -559,49 +583,52 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         // are masked) and are zeros in V; rows of a page that no row sees are zeroed in V, where a weight of zero would meet them.
         int key_end = 0, lo = 0, sink = 0, u_sink = 0, u_first = 0, head = 0, seq = 0;
         int cache_first = -1, cache_b = -1, page_cache = 0;  // lane i: page number cache_first + i of the table of sequence cache_b
+        const int boxes = TC_UNIT / box_rows;
+        auto visible = [&](int from, int rows) { return from < key_end && (from + rows > lo || from < sink); };
         auto copy = [&](int i, bool is_v) {
-            const int k0 = (i < u_sink ? i : u_first + i - u_sink) * TC_UNIT;
-            auto wanted = [&](int kb) { return kb < key_end && (kb + box_rows > lo || kb < sink); };
+            const int k0 = (i < u_sink ? i : u_first + i - u_sink) * TC_UNIT, idx = k0 >> a.page_shift;
+            if (cache_b != seq || idx < cache_first || idx + boxes > cache_first + 32) {
+                cache_b = seq;
+                cache_first = idx;
+                const int at = idx + lane;
+                page_cache = a.n_pages;  // beyond the last page: zeros
+                if (at <= (key_end - 1) >> a.page_shift) {
+                    page_cache = a.prefix_pass ? a.prefix_table[at] : a.block_table[(int64_t)seq * a.ld_table + at];
+                    if (page_cache < 0 || page_cache >= a.n_pages) {
+                        page_cache = a.n_pages;
+                        if (visible(at << a.page_shift, page_mask + 1)) atomicOr(a.status, PAGED_BAD_INDEX);
+                    }
+                }
+            }
+            int page[8];
+            uint32_t wanted = 0;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                page[r] = __shfl_sync(0xffffffffu, page_cache, (idx - cache_first + r) & 31);
+                if (r < boxes) {
+                    if (visible(k0 + r * box_rows, box_rows)) wanted |= 1u << r;
+                    else page[r] = a.n_pages;
+                }
+            }
+            if (is_v) wanted = (1u << boxes) - 1u;
             const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES, full = kv_full + 8 * (n % C::SLOTS);
-            if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
-            __syncwarp();
             const bool fix = is_v && (k0 + TC_UNIT > key_end || (k0 < lo && k0 + TC_UNIT > sink));
             const uint32_t bar = fix ? fix_bar : full;
-            int bytes = 0;
-            for (int r = 0; r < TC_UNIT; r += box_rows) bytes += is_v || wanted(k0 + r) ? box_rows * 128 * C::HALVES : 0;
+            if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
+            __syncwarp();
             if (elect_one()) {
-                if (bytes > 0) mbar_expect_tx(bar, (uint32_t)bytes);
+                if (wanted) mbar_expect_tx(bar, (uint32_t)(__popc(wanted) * box_rows * 128 * C::HALVES));
                 else mbar_arrive(bar);
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+                    if (wanted >> r & 1u) {
+#pragma unroll
+                        for (int h = 0; h < C::HALVES; h++)
+                            tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * box_rows * 128), is_v ? &vmap : &kmap, 64 * h, (k0 + r * box_rows) & page_mask,
+                                          head, page[r], bar);
+                    }
             }
             __syncwarp();
-            for (int r = 0; r < TC_UNIT; r += box_rows) {
-                const int kb = k0 + r;
-                int page = a.n_pages;  // beyond the last page: zeros
-                if (wanted(kb)) {
-                    const int idx = kb >> a.page_shift;
-                    if (cache_b != seq || idx < cache_first || idx >= cache_first + 32) {
-                        cache_b = seq;
-                        cache_first = idx;
-                        const int64_t last = (key_end - 1) >> a.page_shift;
-                        const int at = idx + lane;
-                        page_cache = -1;
-                        if (at <= last) page_cache = a.prefix_pass ? a.prefix_table[at] : a.block_table[(int64_t)seq * a.ld_table + at];
-                    }
-                    page = __shfl_sync(0xffffffffu, page_cache, idx - cache_first);
-                    if (page < 0 || page >= a.n_pages) {
-                        page = a.n_pages;
-                        if (lane == 0) atomicOr(a.status, PAGED_BAD_INDEX);
-                    }
-                } else if (!is_v) {
-                    continue;
-                }
-                if (elect_one()) {
-#pragma unroll
-                    for (int h = 0; h < C::HALVES; h++)
-                        tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * 128), is_v ? &vmap : &kmap, 64 * h, kb & page_mask, head, page, bar);
-                }
-                __syncwarp();
-            }
             if (fix) {
                 if (alive) alive = tc_wait(fix_bar, fix_par, a.status);
                 fix_par ^= 1u;
@@ -643,51 +670,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             }
         }
         // the last copies have landed before the CTA may end: the product warp waits for every slot
-    } else if (warp == TC_MMA_WARP) {
-        // ------------------------------------------------------------------------------------------ products
+    } else if (warp == TC_MMA_WARP || warp == TC_MMA1_WARP) {
+        // ------------------------------------------------------------------------------------------ products of a stream
+        const int st = warp == TC_MMA_WARP ? 0 : 1;
         bool alive = true;
-        int n = 0;                                   // slots consumed
-        uint32_t q_par[2] = {0u, 0u}, p_par[2] = {0u, 0u};
+        int n = 0;                       // slots that earlier items took
+        uint32_t q_par = 0u, p_par = 0u;
         constexpr uint32_t idesc_s = tc_idesc<BF16>(TC_UNIT, false), idesc_o = tc_idesc<BF16>(D, true);
+        const uint32_t sc = tmem + C::S_COL + st * TC_UNIT, o = tmem + C::O_COL + st * D;
+        const uint64_t qd = smem_desc_sw128(base + (uint32_t)st * C::SLOT_BYTES);
         auto slot_addr = [&](int i) { return base + C::RING_AT + (uint32_t)(i % C::SLOTS) * C::SLOT_BYTES; };
         auto wait_slot = [&](int i) {
             if (alive) alive = tc_wait(kv_full + 8 * (i % C::SLOTS), (uint32_t)((i / C::SLOTS) & 1), a.status);
-        };
-        // S of stream st from the K in slot i; `release`: the slot's last use, `last`: the queries'
-        auto scores = [&](int st, int i, bool release, bool last) {
-            wait_slot(i);
-            __syncwarp();
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t d = tmem + C::S_COL + st * TC_UNIT;
-                const uint64_t qd = smem_desc_sw128(base + (uint32_t)st * C::SLOT_BYTES), kd = smem_desc_sw128(slot_addr(i));
-#pragma unroll
-                for (int h = 0; h < C::HALVES; h++)
-#pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        tc_mma_ss(d, qd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), kd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), idesc_s,
-                                  h + kk > 0 ? 1u : 0u);
-                umma_commit(s_full + 8 * st);
-                if (last) umma_commit(q_empty + 8 * st);
-                if (release) umma_commit(kv_empty + 8 * (i % C::SLOTS));
-            }
-            __syncwarp();
-        };
-        auto output = [&](int st, int i, bool first, bool last, bool release) {
-            if (alive) alive = tc_wait(p_full + 8 * st, p_par[st], a.status);
-            p_par[st] ^= 1u;
-            wait_slot(i);
-            __syncwarp();
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t d = tmem + C::O_COL + st * D, p = tmem + C::S_COL + st * TC_UNIT;
-                const uint64_t vd = tc_desc_v(slot_addr(i), C::HALF_BYTES);
-#pragma unroll
-                for (int kk = 0; kk < TC_UNIT / 16; kk++) tc_mma_ts(d, p + 8 * kk, vd + (uint64_t)(kk * 2048 >> 4), idesc_o, first && kk == 0 ? 0u : 1u);
-                if (release) umma_commit(kv_empty + 8 * (i % C::SLOTS));
-                if (last) umma_commit(o_full + 8 * st);
-            }
-            __syncwarp();
         };
         for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
@@ -695,45 +689,66 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             if (m == 0) break;
             const bool pair = g.pair;
             seg_done(k);
-            const int streams = pair || m > 1 ? 2 : 1;
-            for (int st = 0; st < streams; st++) {
-                if (alive) alive = tc_wait(q_full + 8 * st, q_par[st], a.status);
-                q_par[st] ^= 1u;
+            // Slots in the order of the copies: K V K V ... for a pair, K K V K V K ... V V otherwise
+            auto v_slot = [&](int i) { return n + (pair ? 2 * i + 1 : min(m, 2) + i + min(i, max(0, m - 2))); };
+            auto k_slot = [&](int i) { return pair ? n + 2 * i : (i < 2 ? n + i : v_slot(i - 2) + 1); };
+            const int first = pair ? 0 : st, step = pair ? 1 : 2;
+            if (first < m) {
+                if (alive) alive = tc_wait(q_full + 8 * st, q_par, a.status);
+                q_par ^= 1u;
             }
-            if (pair) {
-                scores(0, n, false, m == 1);
-                scores(1, n, true, m == 1);
-                n++;
-                for (int i = 0; i < m; i++) {
-                    const bool more = i + 1 < m;
-                    output(0, n, i == 0, !more, false);
-                    if (more) scores(0, n + 1, false, i + 2 == m);
-                    output(1, n, i == 0, !more, true);
-                    if (more) scores(1, n + 1, true, i + 2 == m);
-                    n += more ? 2 : 1;
+            for (int i = first - step; i < m; i += step) {
+                // O += P V of unit i, then S = Q K^T of the next one
+                const bool with_v = i >= first, with_k = i + step < m;
+                const int vs = with_v ? v_slot(i) : 0, ks = with_k ? k_slot(i + step) : 0;
+                if (with_v) wait_slot(vs);
+                if (with_k) wait_slot(ks);
+                if (with_v) {
+                    if (alive) alive = tc_wait(p_full + 8 * st, p_par, a.status);
+                    p_par ^= 1u;
                 }
-            } else {
-                scores(0, n++, true, m <= 2);
-                if (m > 1) scores(1, n++, true, m <= 3);
-                for (int i = 0; i < m; i++) {
-                    output(i & 1, n++, i < 2, i + 2 >= m, true);
-                    if (i + 2 < m) scores(i & 1, n++, true, i + 4 >= m);
+                __syncwarp();
+                tc_fence_after();
+                if (elect_one()) {
+                    if (with_v) {
+                        const uint64_t vd = tc_desc_v(slot_addr(vs), C::HALF_BYTES);
+#pragma unroll
+                        for (int kk = 0; kk < TC_UNIT / 16; kk++)
+                            tc_mma_ts(o, sc + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, i == first && kk == 0 ? 0u : 1u);
+                        if (!with_k) umma_commit(o_full + 8 * st);
+                        umma_commit(kv_empty + 8 * (vs % C::SLOTS));
+                        if (!pair) umma_commit(kv_empty + 8 * (vs % C::SLOTS));
+                    }
+                    if (with_k) {
+                        const uint64_t kd = smem_desc_sw128(slot_addr(ks));
+#pragma unroll
+                        for (int h = 0; h < C::HALVES; h++)
+#pragma unroll
+                            for (int kk = 0; kk < 4; kk++)
+                                tc_mma_ss(sc, qd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), kd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), idesc_s,
+                                          h + kk > 0 ? 1u : 0u);
+                        umma_commit(s_full + 8 * st);
+                        if (i + 2 * step >= m) umma_commit(q_empty + 8 * st);
+                        umma_commit(kv_empty + 8 * (ks % C::SLOTS));
+                        if (!pair) umma_commit(kv_empty + 8 * (ks % C::SLOTS));
+                    }
                 }
+                __syncwarp();
             }
+            n += 2 * m;
         }
-    } else if (warp == TC_QUERY_WARP) {
-        // ------------------------------------------------------------------------------------------ queries
+    } else if (warp == TC_WALK_WARP) {
+        // ------------------------------------------------------------------------------------------ the batch, item by item
+        TcWalk w;
+        w.start(a, sh, lane);
+        if (lane == 0) splits[blockIdx.x].rows = 0;
         bool alive = true;
         int used[2] = {0, 0};
         const uint32_t bytes = (uint32_t)(tc_tokens(a) * a.G * 128 * C::HALVES);
-        for (int k = 0; seg_wait(k); k++) {
+        // Queries of item k, once the scores of the last item are complete.  A stream without a unit gets none.
+        auto queries = [&](int k) {
             const TcSeg &g = segs[k % TC_SEGS];
-            const int m = g.m, token = g.q0 + g.tok0, head = g.head * a.G;
-            const bool pair = g.pair;
-            if (m == 0) break;
-            seg_done(k);
-            // (a stream without a unit gets none: the product warp waits for none)
-            for (int st = 0; st < (pair || m > 1 ? 2 : 1); st++) {
+            for (int st = 0; st < (g.m == 0 ? 0 : (g.pair || g.m > 1 ? 2 : 1)); st++) {
                 if (used[st] > 0 && alive) alive = tc_wait(q_empty + 8 * st, (uint32_t)((used[st] - 1) & 1), a.status);
                 used[st]++;
                 __syncwarp();
@@ -741,42 +756,47 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     mbar_expect_tx(q_full + 8 * st, bytes);
 #pragma unroll
                     for (int h = 0; h < C::HALVES; h++)
-                        tma_load_rows(base + (uint32_t)(st * C::SLOT_BYTES + h * C::HALF_BYTES), &qmap, 64 * h, head, token + (pair ? st * tc_tokens(a) : 0), q_full + 8 * st);
+                        tma_load_rows(base + (uint32_t)(st * C::SLOT_BYTES + h * C::HALF_BYTES), &qmap, 64 * h, g.head * a.G,
+                                      g.q0 + g.tok0 + (g.pair ? st * tc_tokens(a) : 0), q_full + 8 * st);
                 }
                 __syncwarp();
             }
-        }
-    } else if (warp == TC_WALK_WARP) {
-        // ------------------------------------------------------------------------------------------ the batch, item by item
-        TcWalk w;
-        w.start(a, sh, lane);
-        for (int k = 0;; k++) {
-            if (k >= TC_SEGS && !tc_wait(seg_empty + 8 * (k % TC_SEGS), (uint32_t)((k / TC_SEGS - 1) & 1), a.status)) break;
+        };
+        for (int k = 0;;) {
             const bool end = w.pos >= sh.u1;
+            const int first = end ? 0 : w.it.units_before(w.at), units = end ? 0 : w.it.units_before(w.at + w.here(sh)) - first;
+            if (!end && units == 0) {  // (only numbers that stand for no unit)
+                w.next(a, sh);
+                continue;
+            }
+            if (k >= TC_SEGS && alive) alive = tc_wait(seg_empty + 8 * (k % TC_SEGS), (uint32_t)((k / TC_SEGS - 1) & 1), a.status);
+            if (!alive) break;
             if (lane == 0) {
                 TcSeg g{};
                 if (!end) {
-                    g.m = w.here(sh);
-                    g.unit = w.unit; g.u_sink = w.it.u.sink; g.u_first = w.it.u.first;
+                    g.m = units;
+                    g.unit = first; g.u_sink = w.it.u.sink; g.u_first = w.it.u.first;
                     g.key_end = w.it.k.key_end; g.lo = w.it.k.lo; g.sink = w.it.k.sink;
                     g.pair = w.it.tokens > tc_tokens(a);
                     g.tok0 = w.it.tok0; g.n = w.s.n;
                     g.b = w.b; g.head = w.head; g.q0 = w.s.q0; g.pos0 = w.s.pos0;
-                    const int64_t first = w.pos - w.unit;
-                    g.complete = g.m == w.it.u.count;
-                    g.slot = 2 * (int)blockIdx.x + (w.unit == 0 ? 1 : 0);
+                    g.complete = units == w.it.u.count;
+                    g.slot = 2 * (int)blockIdx.x + (first == 0 ? 1 : 0);
                     // an item that begins here and goes on elsewhere is the share's last
-                    if (w.unit == 0 && !g.complete)
-                        splits[blockIdx.x] = {paged_owner(first + w.it.u.count - 1, sh.total, sh.N), g.pair ? TC_ITEM_ROWS : TC_ROWS, g.tok0, g.n, g.q0, g.head};
-                    else if (w.pos + g.m >= sh.u1)
-                        splits[blockIdx.x].rows = 0;
+                    if (first == 0 && !g.complete)
+                        splits[blockIdx.x] = {paged_owner(w.pos - w.at + TC_ITEM_WEIGHT + (int64_t)(w.it.u.count - 1) * w.it.weight, sh.total, sh.N),
+                                              g.pair ? TC_ITEM_ROWS : TC_ROWS, g.tok0, g.n, g.q0, g.head};
                 }
                 segs[k % TC_SEGS] = g;
                 mbar_arrive(seg_full + 8 * (k % TC_SEGS));
             }
             __syncwarp();
+            // the queries of the item before, one record behind (the ring keeps a record until the last reader is done with it, and the
+            // products of an item wait for its queries)
+            if (k > 0) queries(k - 1);
             if (end) break;
             w.next(a, sh);
+            k++;
         }
         }
     }
