@@ -3,20 +3,23 @@
 //
 // An item is a tile of up to 2 x 128 rows -- twice floor(128 / G) tokens times the G query heads of one kv head -- walked in units of
 // 128 keys.  Its two halves are two streams that take turns: while the softmax of one runs on the CUDA cores, the tensor core multiplies for the other.
-//   S = Q K^T     128 x 128, Q and K in shared memory (K-major, 128-byte swizzle), S in tensor memory
-//   softmax       one thread per row: 128 scores from tensor memory, running maximum and sum in registers, weights in the 16-bit type
+//   S = Q K^T     128 rows x 64 keys (half a unit), Q and K in shared memory (K-major, 128-byte swizzle), S in one of the stream's two
+//                 score buffers in tensor memory
+//   softmax       one thread per row: 64 scores from tensor memory, running maximum and sum in registers, weights in the 16-bit type
 //                 back into the columns that the scores had
 //   O += P V      P from tensor memory, V as it lies in its pages (keys as rows: the transposed operand form), O in tensor memory
+// The scores of half j + 1 are complete while the softmax works on half j.  With one buffer of 128 keys per stream the
+// softmax waited for product and product for softmax in turn: 4260 clocks per unit and stream pair instead of
 // An item of one half gives both streams the same rows and every other unit of keys; the two results meet in tensor
-// memory, whose lanes the warps of both streams reach.  Tensor memory is full: 2 x 128 columns of scores, 2 x d of output.
+// memory, whose lanes the warps of both streams reach.  Tensor memory is full: 2 x 2 x 64 columns of scores, 2 x d of output.
 //
 // Warps 0-3 and 4-7: softmax of the two streams, and their rows' results.  Warps 8 and 11 issue the streams' products -- one
 // warp for both would leave the tensor core idle during its waits, since the issue of a product blocks until the queue before it has
 // drained -- warp 9 the tiled copies of the pages into a ring of slots.  Warp 10 walks the batch, hands the other warps one
 // record per item, so that they keep their registers for scores, and copies the queries (one copy per stream and 64 columns: the
-// G heads of a run of tokens are the rows of a tile as they lie).  Products of one CTA execute in the order of issue, so the scores of unit
-// i + 1 may follow the product that reads the weights of unit i from the same columns, and a full score buffer means that
-// the output accumulator is at rest: the softmax warps rescale it in place, which they do only when the maximum has grown by 2^8.
+// G heads of a run of tokens are the rows of a tile as they lie).  Products of one stream execute in the order of issue, so the scores of half
+// j + 2 may follow the product that reads the weights of half j from the same columns.  The softmax warps rescale the output in
+// place, which they do only when the maximum has grown by 2^8 and once the last product that they asked for is complete.
 #include <climits>
 
 #include "ttq_devutil.cuh"
@@ -25,7 +28,8 @@
 namespace ttq {
 namespace {
 
-constexpr int TC_UNIT = 128;       // keys per unit
+constexpr int TC_UNIT = 128;       // keys per unit (of copies and of shares)
+constexpr int TC_HALF = 64;        // keys per product
 constexpr int TC_ROWS = 128;       // rows per stream
 constexpr int TC_ITEM_ROWS = 2 * TC_ROWS;
 constexpr int TC_MMA_WARP = 8, TC_TMA_WARP = 9, TC_WALK_WARP = 10, TC_MMA1_WARP = 11;
@@ -62,7 +66,7 @@ struct TcCfg {
     static constexpr int RING_AT = 2 * SLOT_BYTES;
     static constexpr int OUT_AT = RING_AT + SLOTS * SLOT_BYTES;
     static constexpr int BAR_AT = OUT_AT + 8 * 4096;
-    static constexpr int N_BARS = 2 * SLOTS + 10 + 1 + 2 * TC_SEGS;
+    static constexpr int N_BARS = 2 * SLOTS + 14 + 1 + 2 * TC_SEGS;
     static constexpr int ML_AT = BAR_AT + (N_BARS * 8 + 15) / 16 * 16;
     static constexpr int SEG_AT = ML_AT + 2 * TC_ROWS * 8;
     static constexpr int MISC_AT = SEG_AT + (TC_SEGS * (int)sizeof(TcSeg) + 15) / 16 * 16;
@@ -297,8 +301,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = smem_u32(smem);
     const uint32_t bars = base + C::BAR_AT;
-    const uint32_t kv_full = bars, kv_empty = kv_full + 8 * C::SLOTS, q_full = kv_empty + 8 * C::SLOTS, s_full = q_full + 16, p_full = s_full + 16,
-                   o_full = p_full + 16, q_empty = o_full + 16, fix_bar = q_empty + 16, seg_full = fix_bar + 8, seg_empty = seg_full + 8 * TC_SEGS;
+    const uint32_t kv_full = bars, kv_empty = kv_full + 8 * C::SLOTS, q_full = kv_empty + 8 * C::SLOTS, s_full = q_full + 16, p_full = s_full + 32,
+                   o_full = p_full + 32, q_empty = o_full + 16, fix_bar = q_empty + 16, seg_full = fix_bar + 8, seg_empty = seg_full + 8 * TC_SEGS;
     float2 *ml = reinterpret_cast<float2 *>(smem + C::ML_AT);
     TcSeg *segs = reinterpret_cast<TcSeg *>(smem + C::SEG_AT);
     int64_t *red = reinterpret_cast<int64_t *>(smem + C::MISC_AT);
@@ -312,8 +316,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         for (int i = 0; i < 2; i++) {
             mbar_init(q_full + 8 * i, 1);
             mbar_init(q_empty + 8 * i, 1);
-            mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 4);
+            for (int h = 0; h < 2; h++) {
+                mbar_init(s_full + 8 * (2 * i + h), 1);
+                mbar_init(p_full + 8 * (2 * i + h), 4);
+            }
             mbar_init(o_full + 8 * i, 1);
         }
         mbar_init(fix_bar, 1);
@@ -371,12 +377,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         // ------------------------------------------------------------------------------------------ softmax: a thread per row
         const int st = warp >> 2, r = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's quarter of the tensor memory's lanes
-        const uint32_t ts = tmem + C::S_COL + st * TC_UNIT + lanes, to = tmem + C::O_COL + st * D + lanes;
+        const uint32_t tsc = tmem + C::S_COL + st * TC_UNIT + lanes, to = tmem + C::O_COL + st * D + lanes;
         const int r_tok = r / a.G, r_head = r - r_tok * a.G;
         const int base_pos = a.prefix_pass ? 0 : a.prefix_len;
         const uint64_t scale_2 = f2(a.scale2, a.scale2);
         bool alive = true;
-        uint32_t s_par = 0, o_par = 0;
+        uint32_t halves = 0, par[2] = {0u, 0u};  // halves done so far; parities of the buffers
         for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
             const int m = g.m;
@@ -388,86 +394,91 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             if (valid) pos = a.prefix_pass ? paged_row_pos(a, g.q0 + tok) : g.pos0 + tok;
             const int min_row = __reduce_min_sync(0xffffffffu, valid ? pos : INT_MAX), max_row = __reduce_max_sync(0xffffffffu, valid ? pos : -1);
             float mx = -INFINITY, l = 0.f;  // running maximum of the scores (unscaled) and sum
-            const int step = joint ? 2 : 1;
-            for (int i = joint ? st : 0; i < m; i += step) {
-                const int ui = g.unit + i, k0 = (ui < g.u_sink ? ui : g.u_first + ui - g.u_sink) * TC_UNIT;
-                if (alive) alive = tc_wait(s_full + 8 * st, s_par, a.status);
-                s_par ^= 1u;
-                __syncwarp();
-                tc_fence_after();
-                float s[TC_UNIT];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_ld32(ts + 32 * c, s + 32 * c);
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_ld_wait32(s + 32 * c);
-                const int j0 = k0 + base_pos;
-                const bool whole = j0 + TC_UNIT - 1 <= min_row && k0 + TC_UNIT <= g.key_end && (a.window == 0 || j0 > max_row - a.window || j0 + TC_UNIT <= a.sinks);
-                if (!whole) {
-                    // key kk of the unit is visible from `from` to `to` and below `sink`
-                    const int end = min(pos - base_pos + 1, g.key_end) - k0, from = a.window > 0 ? pos - a.window + 1 - base_pos - k0 : INT_MIN,
-                              sink = a.sinks - base_pos - k0;
-#pragma unroll
-                    for (int kk = 0; kk < TC_UNIT; kk++)
-                        if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
-                }
-                float tops[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int kk = 4; kk < TC_UNIT - 4; kk += 8)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) tops[x] = max3(tops[x], s[kk + x], s[kk + 4 + x]);
-#pragma unroll
-                for (int x = 0; x < 4; x++) tops[x] = fmaxf(tops[x], s[TC_UNIT - 4 + x]);
-                const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-                const bool grow = (top - mx) * a.scale2 > 8.f || (mx == -INFINITY && top > -INFINITY);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float next = fmaxf(mx, top), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
-                    mx = next;
-                    l *= f;
-                    if (i >= step) {  // (the first unit starts the accumulator)
+            const int step = joint ? 2 : 1, first = joint ? st : 0;
+            const uint32_t halves0 = halves;
+            for (int i = first; i < m; i += step) {
+                const int ui = g.unit + i, k_unit = (ui < g.u_sink ? ui : g.u_first + ui - g.u_sink) * TC_UNIT;
 #pragma unroll 1
-                        for (int c = 0; c < D / 16; c++) {
-                            float o[16];
-                            tc_ld16(to + 16 * c, o);
-                            uint32_t q[16];
+                for (int h = 0; h < 2; h++, halves++) {
+                    const int k0 = k_unit + h * TC_HALF;
+                    const uint32_t ts = tsc + h * TC_HALF;
+                    if (alive) alive = tc_wait(s_full + 8 * (2 * st + h), par[h], a.status);
+                    par[h] ^= 1u;
+                    __syncwarp();
+                    tc_fence_after();
+                    float s[TC_HALF];
 #pragma unroll
-                            for (int x = 0; x < 16; x++) q[x] = __float_as_uint(o[x] * f);
-                            tc_st16(to + 16 * c, q);
+                    for (int c = 0; c < 2; c++) tc_ld32(ts + 32 * c, s + 32 * c);
+#pragma unroll
+                    for (int c = 0; c < 2; c++) tc_ld_wait32(s + 32 * c);
+                    const int j0 = k0 + base_pos;
+                    const bool whole = j0 + TC_HALF - 1 <= min_row && k0 + TC_HALF <= g.key_end && (a.window == 0 || j0 > max_row - a.window || j0 + TC_HALF <= a.sinks);
+                    if (!whole) {
+                        // key kk of the half is visible from `from` to `end` and below `sink`
+                        const int end = min(pos - base_pos + 1, g.key_end) - k0, from = a.window > 0 ? pos - a.window + 1 - base_pos - k0 : INT_MIN,
+                                  sink = a.sinks - base_pos - k0;
+#pragma unroll
+                        for (int kk = 0; kk < TC_HALF; kk++)
+                            if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
+                    }
+                    float tops[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int kk = 4; kk < TC_HALF - 4; kk += 8)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) tops[x] = max3(tops[x], s[kk + x], s[kk + 4 + x]);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) tops[x] = fmaxf(tops[x], s[TC_HALF - 4 + x]);
+                    const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
+                    const bool grow = (top - mx) * a.scale2 > 8.f || (mx == -INFINITY && top > -INFINITY);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float next = fmaxf(mx, top), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
+                        mx = next;
+                        l *= f;
+                        if (halves != halves0) {  // (the first half starts the accumulator)
+                            if (alive) alive = tc_wait(o_full + 8 * st, (halves - 1) & 1, a.status);
+                            __syncwarp();
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D / 16; c++) {
+                                float o[16];
+                                tc_ld16(to + 16 * c, o);
+                                uint32_t q[16];
+#pragma unroll
+                                for (int x = 0; x < 16; x++) q[x] = __float_as_uint(o[x] * f);
+                                tc_st16(to + 16 * c, q);
+                            }
                         }
                     }
-                }
-                const float off = mx == -INFINITY ? 0.f : -mx * a.scale2;
-                const uint64_t off_2 = f2(off, off);
-                uint64_t sums[2] = {0ull, 0ull};
+                    const float off = mx == -INFINITY ? 0.f : -mx * a.scale2;
+                    const uint64_t off_2 = f2(off, off);
+                    uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    uint32_t q[16];
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t q[16];
 #pragma unroll
-                    for (int x = 0; x < 16; x++) {
-                        const uint64_t y = fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale_2, off_2);
-                        float e0, e1;
-                        f2_split(y, e0, e1);
-                        e0 = ex2(e0);
-                        e1 = ex2(e1);
-                        sums[x & 1] = add2(sums[x & 1], f2(e0, e1));
-                        q[x] = pack2<BF16>(e0, e1);
+                        for (int x = 0; x < 16; x++) {
+                            float e0, e1;
+                            f2_split(fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale_2, off_2), e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                            sums[x & 1] = add2(sums[x & 1], f2(e0, e1));
+                            q[x] = pack2<BF16>(e0, e1);
+                        }
+                        tc_st16(ts + 16 * c, q);
                     }
-                    tc_st16(ts + 16 * c, q);
-                }
-                {
+                    tc_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + 8 * (2 * st + h));
                     float x, y;
                     f2_split(add2(sums[0], sums[1]), x, y);
                     l += x + y;
                 }
-                tc_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * st);
             }
             // ---- results ----
-            if (!joint || m > st) {
-                if (alive) alive = tc_wait(o_full + 8 * st, o_par, a.status);
-                o_par ^= 1u;
-            }
+            // (the last two products in turn: a parity tells a phase only from its neighbours)
+            for (uint32_t x = 2; x > 0 && first < m; x--)
+                if (alive) alive = tc_wait(o_full + 8 * st, (halves - x) & 1, a.status);
             __syncwarp();
             tc_fence_after();
             const float m2 = mx == -INFINITY ? -INFINITY : mx * a.scale2;
@@ -655,18 +666,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             const int u0 = g.unit;
             const bool pair = g.pair;
             seg_done(k);
-            if (pair) {   // both streams take every unit
-                for (int i = 0; i < m; i++) {
-                    copy(u0 + i, false);
-                    copy(u0 + i, true);
-                }
-            } else {      // stream 0 the even ones, stream 1 the odd ones
-                copy(u0, false);
-                if (m > 1) copy(u0 + 1, false);
-                for (int i = 0; i < m; i++) {
-                    copy(u0 + i, true);
-                    if (i + 2 < m) copy(u0 + i + 2, false);
-                }
+            // a pair takes every unit: K V K V ...; else stream 0 the even ones, stream 1 the odd ones: K K V K V ... V V
+            int ki = 0, vi = 0;
+#pragma unroll 1
+            for (int x = 0; x < 2 * m; x++) {
+                const bool is_v = ki == m || (pair ? ki > vi : ki > vi + 1);
+                copy(u0 + (is_v ? vi : ki), is_v);
+                if (is_v) vi++;
+                else ki++;
             }
         }
         // the last copies have landed before the CTA may end: the product warp waits for every slot
@@ -675,8 +682,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         const int st = warp == TC_MMA_WARP ? 0 : 1;
         bool alive = true;
         int n = 0;                       // slots that earlier items took
-        uint32_t q_par = 0u, p_par = 0u;
-        constexpr uint32_t idesc_s = tc_idesc<BF16>(TC_UNIT, false), idesc_o = tc_idesc<BF16>(D, true);
+        uint32_t q_par = 0u, p_par[2] = {0u, 0u};
+        constexpr uint32_t idesc_s = tc_idesc<BF16>(TC_HALF, false), idesc_o = tc_idesc<BF16>(D, true);
         const uint32_t sc = tmem + C::S_COL + st * TC_UNIT, o = tmem + C::O_COL + st * D;
         const uint64_t qd = smem_desc_sw128(base + (uint32_t)st * C::SLOT_BYTES);
         auto slot_addr = [&](int i) { return base + C::RING_AT + (uint32_t)(i % C::SLOTS) * C::SLOT_BYTES; };
@@ -698,42 +705,49 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 q_par ^= 1u;
             }
             for (int i = first - step; i < m; i += step) {
-                // O += P V of unit i, then S = Q K^T of the next one
+                // half by half: O += P V of unit i, then S = Q K^T of the next one into the same buffer
                 const bool with_v = i >= first, with_k = i + step < m;
                 const int vs = with_v ? v_slot(i) : 0, ks = with_k ? k_slot(i + step) : 0;
                 if (with_v) wait_slot(vs);
                 if (with_k) wait_slot(ks);
-                if (with_v) {
-                    if (alive) alive = tc_wait(p_full + 8 * st, p_par, a.status);
-                    p_par ^= 1u;
-                }
-                __syncwarp();
-                tc_fence_after();
-                if (elect_one()) {
+#pragma unroll 1
+                for (int h = 0; h < 2; h++) {
                     if (with_v) {
-                        const uint64_t vd = tc_desc_v(slot_addr(vs), C::HALF_BYTES);
-#pragma unroll
-                        for (int kk = 0; kk < TC_UNIT / 16; kk++)
-                            tc_mma_ts(o, sc + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, i == first && kk == 0 ? 0u : 1u);
-                        if (!with_k) umma_commit(o_full + 8 * st);
-                        umma_commit(kv_empty + 8 * (vs % C::SLOTS));
-                        if (!pair) umma_commit(kv_empty + 8 * (vs % C::SLOTS));
+                        if (alive) alive = tc_wait(p_full + 8 * (2 * st + h), p_par[h], a.status);
+                        p_par[h] ^= 1u;
                     }
-                    if (with_k) {
-                        const uint64_t kd = smem_desc_sw128(slot_addr(ks));
+                    __syncwarp();
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (with_v) {
+                            const uint64_t vd = tc_desc_v(slot_addr(vs) + (uint32_t)(h * TC_HALF * 128), C::HALF_BYTES);
 #pragma unroll
-                        for (int h = 0; h < C::HALVES; h++)
+                            for (int kk = 0; kk < TC_HALF / 16; kk++)
+                                tc_mma_ts(o, sc + h * TC_HALF + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, i == first && h + kk == 0 ? 0u : 1u);
+                            umma_commit(o_full + 8 * st);
+                            if (h == 1) {
+                                umma_commit(kv_empty + 8 * (vs % C::SLOTS));
+                                if (!pair) umma_commit(kv_empty + 8 * (vs % C::SLOTS));
+                            }
+                        }
+                        if (with_k) {
+                            const uint64_t kd = smem_desc_sw128(slot_addr(ks) + (uint32_t)(h * TC_HALF * 128));
 #pragma unroll
-                            for (int kk = 0; kk < 4; kk++)
-                                tc_mma_ss(sc, qd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), kd + (uint64_t)(h * (C::HALF_BYTES >> 4) + 2 * kk), idesc_s,
-                                          h + kk > 0 ? 1u : 0u);
-                        umma_commit(s_full + 8 * st);
-                        if (i + 2 * step >= m) umma_commit(q_empty + 8 * st);
-                        umma_commit(kv_empty + 8 * (ks % C::SLOTS));
-                        if (!pair) umma_commit(kv_empty + 8 * (ks % C::SLOTS));
+                            for (int x = 0; x < C::HALVES; x++)
+#pragma unroll
+                                for (int kk = 0; kk < 4; kk++)
+                                    tc_mma_ss(sc + h * TC_HALF, qd + (uint64_t)(x * (C::HALF_BYTES >> 4) + 2 * kk), kd + (uint64_t)(x * (C::HALF_BYTES >> 4) + 2 * kk),
+                                              idesc_s, x + kk > 0 ? 1u : 0u);
+                            umma_commit(s_full + 8 * (2 * st + h));
+                            if (h == 1) {
+                                if (i + 2 * step >= m) umma_commit(q_empty + 8 * st);
+                                umma_commit(kv_empty + 8 * (ks % C::SLOTS));
+                                if (!pair) umma_commit(kv_empty + 8 * (ks % C::SLOTS));
+                            }
+                        }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             n += 2 * m;
         }
