@@ -5,7 +5,7 @@
 // 128 keys.  Its two halves are two streams that take turns: while the softmax of one runs on the CUDA cores, the tensor core multiplies for the other.
 //   S = Q K^T     128 rows x 64 keys (half a unit), Q and K in shared memory (K-major, 128-byte swizzle), S in one of the stream's two
 //                 score buffers in tensor memory
-//   softmax       one thread per row: 64 scores from tensor memory, running maximum and sum in registers, weights in the 16-bit type
+//   softmax       one thread per row: 64 scores from tensor memory, reference and sum in registers, weights in the 16-bit type
 //                 back into the columns that the scores had
 //   O += P V      P from tensor memory, V as it lies in its pages (keys as rows: the transposed operand form), O in tensor memory
 // The scores of half j + 1 are complete while the softmax works on half j.  With one buffer of 128 keys per stream the
@@ -19,7 +19,7 @@
 // record per item, so that they keep their registers for scores, and copies the queries (one copy per stream and 64 columns: the
 // G heads of a run of tokens are the rows of a tile as they lie).  Products of one stream execute in the order of issue, so the scores of half
 // j + 2 may follow the product that reads the weights of half j from the same columns.  The softmax warps rescale the output in
-// place, which they do only when the maximum has grown by 2^8 and once the last product that they asked for is complete.
+// place, which they do only when the weights outgrow their reference and once the last product that they asked for is complete.
 #include <climits>
 
 #include "ttq_devutil.cuh"
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             int pos = -1;
             if (valid) pos = a.prefix_pass ? paged_row_pos(a, g.q0 + tok) : g.pos0 + tok;
             const int min_row = __reduce_min_sync(0xffffffffu, valid ? pos : INT_MAX), max_row = __reduce_max_sync(0xffffffffu, valid ? pos : -1);
-            float mx = -INFINITY, l = 0.f;  // running maximum of the scores (unscaled) and sum
+            float mx = valid ? -INFINITY : 0.f, l = 0.f;  // reference for the scores (unscaled) and sum
             const int step = joint ? 2 : 1, first = joint ? st : 0;
             const uint32_t halves0 = halves;
             for (int i = first; i < m; i += step) {
@@ -421,58 +421,67 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                         for (int kk = 0; kk < TC_HALF; kk++)
                             if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
                     }
-                    float tops[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                    for (int kk = 4; kk < TC_HALF - 4; kk += 8)
-#pragma unroll
-                        for (int x = 0; x < 4; x++) tops[x] = max3(tops[x], s[kk + x], s[kk + 4 + x]);
-#pragma unroll
-                    for (int x = 0; x < 4; x++) tops[x] = fmaxf(tops[x], s[TC_HALF - 4 + x]);
-                    const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]);
-                    const bool grow = (top - mx) * a.scale2 > 8.f || (mx == -INFINITY && top > -INFINITY);
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float next = fmaxf(mx, top), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
-                        mx = next;
-                        l *= f;
-                        if (halves != halves0) {  // (the first half starts the accumulator)
-                            if (alive) alive = tc_wait(o_full + 8 * st, (halves - 1) & 1, a.status);
-                            __syncwarp();
-                            tc_fence_after();
+                    // The weights are taken relative to the row's reference `mx`, which follows the maximum only when they grow too
+                    // large (a sum of 2^15: every weight is finite in fp16): the maximum of 64 scores costs a fifth of their softmax.
+                    float sum;
+                    bool redo = mx == -INFINITY;
 #pragma unroll 1
-                            for (int c = 0; c < D / 16; c++) {
-                                float o[16];
-                                tc_ld16(to + 16 * c, o);
-                                uint32_t q[16];
+                    for (int turn = 0;; turn++) {
+                        if (__any_sync(0xffffffffu, redo)) {
+                            float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                                for (int x = 0; x < 16; x++) q[x] = __float_as_uint(o[x] * f);
-                                tc_st16(to + 16 * c, q);
+                            for (int kk = 4; kk < TC_HALF - 4; kk += 8)
+#pragma unroll
+                                for (int x = 0; x < 4; x++) tops[x] = max3(tops[x], s[kk + x], s[kk + 4 + x]);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) tops[x] = fmaxf(tops[x], s[TC_HALF - 4 + x]);
+                            const float next = fmaxf(mx, fmaxf(max3(tops[0], tops[1], tops[2]), tops[3])), f = mx == -INFINITY ? 0.f : ex2((mx - next) * a.scale2);
+                            mx = next;
+                            l *= f;
+                            tc_st_wait();
+                            if (halves != halves0) {  // (the first half starts the accumulator)
+                                if (alive) alive = tc_wait(o_full + 8 * st, (halves - 1) & 1, a.status);
+                                __syncwarp();
+                                tc_fence_after();
+#pragma unroll 1
+                                for (int c = 0; c < D / 16; c++) {
+                                    float o[16];
+                                    tc_ld16(to + 16 * c, o);
+                                    uint32_t q[16];
+#pragma unroll
+                                    for (int x = 0; x < 16; x++) q[x] = __float_as_uint(o[x] * f);
+                                    tc_st16(to + 16 * c, q);
+                                }
                             }
                         }
-                    }
-                    const float off = mx == -INFINITY ? 0.f : -mx * a.scale2;
-                    const uint64_t off_2 = f2(off, off);
-                    uint64_t sums[2] = {0ull, 0ull};
+                        const float off = mx == -INFINITY ? 0.f : -mx * a.scale2;
+                        const uint64_t off_2 = f2(off, off);
+                        uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        uint32_t q[16];
+                        for (int c = 0; c < 2; c++) {
+                            uint32_t q[16];
 #pragma unroll
-                        for (int x = 0; x < 16; x++) {
-                            float e0, e1;
-                            f2_split(fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale_2, off_2), e0, e1);
-                            e0 = ex2(e0);
-                            e1 = ex2(e1);
-                            sums[x & 1] = add2(sums[x & 1], f2(e0, e1));
-                            q[x] = pack2<BF16>(e0, e1);
+                            for (int x = 0; x < 16; x++) {
+                                float e0, e1;
+                                f2_split(fma2(f2(s[32 * c + 2 * x], s[32 * c + 2 * x + 1]), scale_2, off_2), e0, e1);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                                sums[x & 1] = add2(sums[x & 1], f2(e0, e1));
+                                q[x] = pack2<BF16>(e0, e1);
+                            }
+                            tc_st16(ts + 16 * c, q);
                         }
-                        tc_st16(ts + 16 * c, q);
+                        float x, y;
+                        f2_split(add2(sums[0], sums[1]), x, y);
+                        sum = x + y;
+                        redo = !(sum <= 32768.f);
+                        if (turn > 0 || !__any_sync(0xffffffffu, redo)) break;
                     }
+                    l += sum;
                     tc_st_wait();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(p_full + 8 * (2 * st + h));
-                    float x, y;
-                    f2_split(add2(sums[0], sums[1]), x, y);
-                    l += x + y;
                 }
             }
             // ---- results ----
@@ -590,90 +599,80 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         bool alive = true;
         uint32_t fix_par = 0;
         const int page_mask = (1 << a.page_shift) - 1;
-        // Unit i of the item into the next slot: boxes of box_rows slots of one page.  Boxes that no row sees are left out of K (their scores
-        // are masked) and are zeros in V; rows of a page that no row sees are zeroed in V, where a weight of zero would meet them.
-        int key_end = 0, lo = 0, sink = 0, u_sink = 0, u_first = 0, head = 0, seq = 0;
+        // K and V of a unit into the next two slots: boxes of box_rows slots of one page.  Boxes that no row sees are left out of K
+        // (their scores are masked) and are zeros in V; rows of a page that no row sees are zeroed in V, where a weight of zero would
+        // meet them.  One warp's instruction latency bounds this loop, so what can be shared between K and V is.
         int cache_first = -1, cache_b = -1, page_cache = 0;  // lane i: page number cache_first + i of the table of sequence cache_b
-        const int boxes = TC_UNIT / box_rows;
-        auto visible = [&](int from, int rows) { return from < key_end && (from + rows > lo || from < sink); };
-        auto copy = [&](int i, bool is_v) {
-            const int k0 = (i < u_sink ? i : u_first + i - u_sink) * TC_UNIT, idx = k0 >> a.page_shift;
-            if (cache_b != seq || idx < cache_first || idx + boxes > cache_first + 32) {
-                cache_b = seq;
-                cache_first = idx;
-                const int at = idx + lane;
-                page_cache = a.n_pages;  // beyond the last page: zeros
-                if (at <= (key_end - 1) >> a.page_shift) {
-                    page_cache = a.prefix_pass ? a.prefix_table[at] : a.block_table[(int64_t)seq * a.ld_table + at];
-                    if (page_cache < 0 || page_cache >= a.n_pages) {
-                        page_cache = a.n_pages;
-                        if (visible(at << a.page_shift, page_mask + 1)) atomicOr(a.status, PAGED_BAD_INDEX);
-                    }
-                }
-            }
-            int page[8];
-            uint32_t wanted = 0;
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                page[r] = __shfl_sync(0xffffffffu, page_cache, (idx - cache_first + r) & 31);
-                if (r < boxes) {
-                    if (visible(k0 + r * box_rows, box_rows)) wanted |= 1u << r;
-                    else page[r] = a.n_pages;
-                }
-            }
-            if (is_v) wanted = (1u << boxes) - 1u;
-            const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES, full = kv_full + 8 * (n % C::SLOTS);
-            const bool fix = is_v && (k0 + TC_UNIT > key_end || (k0 < lo && k0 + TC_UNIT > sink));
-            const uint32_t bar = fix ? fix_bar : full;
-            if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
-            __syncwarp();
+        const int boxes = TC_UNIT / box_rows, box_bytes = box_rows * 128;
+        auto issue = [&](const CUtensorMap &map, uint32_t wanted, uint32_t bar, const int (&page)[8], int slot0, int head) {
+            const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES;
             if (elect_one()) {
-                if (wanted) mbar_expect_tx(bar, (uint32_t)(__popc(wanted) * box_rows * 128 * C::HALVES));
+                if (wanted) mbar_expect_tx(bar, (uint32_t)(__popc(wanted) * box_bytes * C::HALVES));
                 else mbar_arrive(bar);
 #pragma unroll
                 for (int r = 0; r < 8; r++)
                     if (wanted >> r & 1u) {
 #pragma unroll
                         for (int h = 0; h < C::HALVES; h++)
-                            tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * box_rows * 128), is_v ? &vmap : &kmap, 64 * h, (k0 + r * box_rows) & page_mask,
-                                          head, page[r], bar);
+                            tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * box_bytes), &map, 64 * h, (slot0 + r * box_rows) & page_mask, head, page[r], bar);
                     }
             }
             __syncwarp();
-            if (fix) {
-                if (alive) alive = tc_wait(fix_bar, fix_par, a.status);
-                fix_par ^= 1u;
-                for (int r = lane / 8; r < TC_UNIT; r += 4) {
-                    const int key = k0 + r;
-                    if (key >= key_end || (key < lo && key >= sink)) {
-#pragma unroll
-                        for (int h = 0; h < C::HALVES; h++) sts128<0>(slot + (uint32_t)(h * C::HALF_BYTES + r * 128 + (lane & 7) * 16), 0u, 0u, 0u, 0u);
-                    }
-                }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full);
-            }
-            n++;
+        };
+        auto wait_empty = [&]() {
+            if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
+            __syncwarp();
         };
         for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
-            const int m = g.m;
+            const int m = g.m, u0 = g.unit, u_sink = g.u_sink, u_first = g.u_first, key_end = g.key_end, lo = g.lo, sink = g.sink, head = g.head, seq = g.b;
             if (m == 0) break;
-            key_end = g.key_end; lo = g.lo; sink = g.sink;
-            u_sink = g.u_sink; u_first = g.u_first;
-            head = g.head; seq = g.b;
-            const int u0 = g.unit;
-            const bool pair = g.pair;
             seg_done(k);
-            // a pair takes every unit: K V K V ...; else stream 0 the even ones, stream 1 the odd ones: K K V K V ... V V
-            int ki = 0, vi = 0;
+            auto visible = [&](int from, int rows) { return from < key_end && (from + rows > lo || from < sink); };
 #pragma unroll 1
-            for (int x = 0; x < 2 * m; x++) {
-                const bool is_v = ki == m || (pair ? ki > vi : ki > vi + 1);
-                copy(u0 + (is_v ? vi : ki), is_v);
-                if (is_v) vi++;
-                else ki++;
+            for (int i = u0; i < u0 + m; i++) {
+                const int k0 = (i < u_sink ? i : u_first + i - u_sink) * TC_UNIT, idx = k0 >> a.page_shift;
+                if (cache_b != seq || idx < cache_first || idx + boxes > cache_first + 32) {
+                    cache_b = seq;
+                    cache_first = idx;
+                    const int at = idx + lane;
+                    page_cache = a.n_pages;  // beyond the last page: zeros
+                    if (at <= (key_end - 1) >> a.page_shift) {
+                        page_cache = a.prefix_pass ? a.prefix_table[at] : a.block_table[(int64_t)seq * a.ld_table + at];
+                        if (page_cache < 0 || page_cache >= a.n_pages) {
+                            page_cache = a.n_pages;
+                            if (visible(at << a.page_shift, page_mask + 1)) atomicOr(a.status, PAGED_BAD_INDEX);
+                        }
+                    }
+                }
+                const int mine = __shfl_sync(0xffffffffu, page_cache, (idx - cache_first + lane) & 31);
+                const uint32_t seen = __ballot_sync(0xffffffffu, lane < boxes && visible(k0 + lane * box_rows, box_rows));
+                int page[8];
+#pragma unroll
+                for (int r = 0; r < 8; r++) page[r] = __shfl_sync(0xffffffffu, seen >> lane & 1u ? mine : a.n_pages, r);
+                wait_empty();
+                issue(kmap, seen, kv_full + 8 * (n % C::SLOTS), page, k0, head);
+                n++;
+                const bool fix = k0 + TC_UNIT > key_end || (k0 < lo && k0 + TC_UNIT > sink);
+                const uint32_t full = kv_full + 8 * (n % C::SLOTS);
+                wait_empty();
+                issue(vmap, (1u << boxes) - 1u, fix ? fix_bar : full, page, k0, head);
+                if (fix) {
+                    const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES;
+                    if (alive) alive = tc_wait(fix_bar, fix_par, a.status);
+                    fix_par ^= 1u;
+                    for (int r = lane / 8; r < TC_UNIT; r += 4) {
+                        const int key = k0 + r;
+                        if (key >= key_end || (key < lo && key >= sink)) {
+#pragma unroll
+                            for (int h = 0; h < C::HALVES; h++) sts128<0>(slot + (uint32_t)(h * C::HALF_BYTES + r * 128 + (lane & 7) * 16), 0u, 0u, 0u, 0u);
+                        }
+                    }
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full);
+                }
+                n++;
             }
         }
         // the last copies have landed before the CTA may end: the product warp waits for every slot
@@ -696,9 +695,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             if (m == 0) break;
             const bool pair = g.pair;
             seg_done(k);
-            // Slots in the order of the copies: K V K V ... for a pair, K K V K V K ... V V otherwise
-            auto v_slot = [&](int i) { return n + (pair ? 2 * i + 1 : min(m, 2) + i + min(i, max(0, m - 2))); };
-            auto k_slot = [&](int i) { return pair ? n + 2 * i : (i < 2 ? n + i : v_slot(i - 2) + 1); };
+            // slots in the order of the copies: K V K V ...
+            auto k_slot = [&](int i) { return n + 2 * i; };
+            auto v_slot = [&](int i) { return n + 2 * i + 1; };
             const int first = pair ? 0 : st, step = pair ? 1 : 2;
             if (first < m) {
                 if (alive) alive = tc_wait(q_full + 8 * st, q_par, a.status);
