@@ -292,6 +292,11 @@ struct TcWalk {
     }
 };
 
+// Named barriers of the two softmax warps that share a scheduler: TC_TURN_BAR + 2 (warp & 3) + stream.
+constexpr int TC_TURN_BAR = 2;
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void pair_arrive(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ CUtensorMap kmap,
                                                                  const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap qmap,
@@ -383,6 +388,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         const uint64_t scale_2 = f2(a.scale2, a.scale2);
         bool alive = true;
         uint32_t halves = 0, par[2] = {0u, 0u};  // halves done so far; parities of the buffers
+        if (st == 1) pair_arrive(TC_TURN_BAR + 2 * (warp & 3));  // stream 0 begins
         for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
             const int m = g.m;
@@ -423,6 +429,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     }
                     // The weights are taken relative to the row's reference `mx`, which follows the maximum only when they grow too
                     // large (a sum of 2^15: every weight is finite in fp16): the maximum of 64 scores costs a fifth of their softmax.
+                    // The streams' exponentials take turns.  Each alone keeps the special-function unit busy (590 clocks for 64 rows' weights of a
+                    // warp, 512 at the unit's rate); both at once take as long as one after the other, and then both wait for
+                    // their next scores at once, the unit idle.
+                    if (!joint) pair_sync(TC_TURN_BAR + 2 * (warp & 3) + st);
                     float sum;
                     bool redo = mx == -INFINITY;
 #pragma unroll 1
@@ -477,6 +487,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                         redo = !(sum <= 32768.f);
                         if (turn > 0 || !__any_sync(0xffffffffu, redo)) break;
                     }
+                    if (!joint) pair_arrive(TC_TURN_BAR + 2 * (warp & 3) + 1 - st);
                     l += sum;
                     tc_st_wait();
                     tc_fence_before();
@@ -591,6 +602,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             if (joint) named_barrier(1, TC_SOFTMAX_THREADS);  // the exchange and the other's accumulator are used again
             seg_done(k);
         }
+        if (st == 0) pair_sync(TC_TURN_BAR + 2 * (warp & 3));    // stream 1's last arrival
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_OTHER_REGS));
         if (warp == TC_TMA_WARP) {
