@@ -429,7 +429,7 @@ typedef struct ttq_sampling {
 /* ids[m] = the next token of logits row m [V] (f32, bf16 or f16), drawn with the random number u[m] in [0, 1).
  * With w_i = exp((x_i - max x) / temperature) the tokens in descending order of x (equal logits: lowest index first) are cut to
  * the first top_k (0 or less: all), of those to the shortest run that holds top_p of their weight (1 or more: all; at least
- * one token stays), of those to w_i >= min_p.  The result is the first token, in the order of the vocabulary, at which the
+ * one token stays), of those to w_i >= min_p (the largest logit always stays).  The result is the first token, in the order of the vocabulary, at which the
  * cumulative weight of what is left exceeds u[m] times its total.  temperature <= 0 or NaN: the token of the largest logit (lowest
  * index).  NaN logits count as -inf, a row of nothing but -inf gives -1; where a logit is +inf only such tokens have weight.
  * Weights are computed in 64 bits and summed as 2^-44 fixed point, so that the cuts fall where the definition has them and

@@ -1,255 +1,395 @@
 // Sampling: the next token of every row of logits from given random numbers, with temperature, top-k, top-p and min-p.
 //
-// All three cuts keep a head of the same order (logit descending, index ascending), so a row's result needs no sort: the logit t at
-// which the head ends, and how many tokens with exactly this logit still belong to it.  t is found by descending through the
-// 32 bits of an order-preserving key, 11, 11 and 10 bits at a time, with a histogram of counts and weights per step.
-// Weights are w = exp((x - max) / T), computed in 64 bits and summed as 2^-44 fixed point: integer sums are exact, do not depend on the
-// order of the atomics, and their rounding (2^-45 a token, where the largest weight is 1) is far below the weight of any token that
-// decides a cut.  In 32 bits a cut among 10^5 tokens of similar weight falls on a neighbour of the right one about once in 400 rows.
+// All three cuts keep a head of the same order (logit descending, index ascending), so a row's result needs no sort: the logit at which
+// the head ends, and how many tokens with exactly this logit still belong to it.  Weights are w = exp((x - max) / T), computed
+// in 64 bits and summed as 2^-44 fixed point: integer sums are exact, do not depend on the order of the atomics, and their rounding
+// (2^-45 a token, where the largest weight is 1) is far below the weight of any token that decides a cut.  In 32 bits a cut among 10^5
+// tokens of similar weight falls on a neighbour of the right one about once in 400 rows.
+//
+// A cluster of CTAs holds a row in shared memory, so the logits are read once.  The cut is found by histograms of counts or weights:
+// first over 2048 equal parts of the range that has weight (max - 32 T to max: evenly spread logits, few collisions), then over the
+// order-preserving keys of the part's logits, 2048 at a time, until a bin is one key.  What a bin needs of all CTAs is added into the
+// first one's shared memory.  Bound: one reading of the logits; in practice the 64-bit exponentials (11 instructions each, half the
+// rate of 32-bit ones) for large batches, the chain of cluster barriers for small ones.
+#include <cooperative_groups.h>
+
 #include "ttq_internal.cuh"
 
 namespace ttq {
 namespace {
 
-constexpr int SAMPLE_THREADS = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
-constexpr int BINS = 2048;
+constexpr int BINS = 2048, BINS_PER_THREAD = BINS / SAMPLE_THREADS;
+constexpr int MAX_CLUSTER = 8;
 constexpr double FIXED_ONE = 17592186044416.0;  // 2^44
+constexpr float FIXED_RANGE = 32.f;              // exp(-32 * 2047 / 2048) < 2^-46: no weight in the last part
+typedef unsigned long long u64;
 
 struct SampleArgs {
     const void *logits;
-    int dt, V;
+    int dt, V, slice;
     int64_t ld;
     ttq_sampling s;
     const float *u;
     int64_t *ids;
 };
 
-// Order-preserving: larger float, larger key; -0 and +0 alike; NaN below everything (as -inf).
+// Order-preserving: larger float, larger key.
 __device__ __forceinline__ uint32_t key_of(float x) {
-    if (x != x) x = -INFINITY;
-    const uint32_t b = __float_as_uint(x + 0.f);
+    const uint32_t b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct Shared {
-    uint32_t cnt[BINS], lo[BINS], hi[BINS];
-    unsigned long long warp_sum[SAMPLE_WARPS];
-    int warp_cnt[SAMPLE_WARPS];
-    unsigned long long above_mass, found_mass;
-    int above_cnt, found_bin, found_cnt;
-    int result;
+    uint32_t lo[BINS], hi[BINS];    // this CTA's histogram
+    uint32_t glo[BINS], ghi[BINS];  // the row's (first CTA)
+    double table[64];               // 2^(j / 64)
+    u64 warp_sum[SAMPLE_WARPS];
+    // exchanged between the CTAs of a row
+    u64 best, mass;
+    uint32_t kmin, range_lo, range_hi;
+    int ties;
+    // a level's result (first CTA)
+    u64 found_before, found_mass;
+    int found_bin, found_n;
 };
 
-// Sum of v over lower-numbered threads; `all`: over every thread.
 template <class T>
-__device__ __forceinline__ T block_exclusive(T v, T *warp_sums, T &all) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    T incl = v;
+__device__ __forceinline__ T warp_inclusive(T v) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const T x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
+        const T x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
     }
+    return v;
+}
+// Sum of v over lower-numbered threads; `all`: over every thread.
+__device__ __forceinline__ u64 block_exclusive(u64 v, u64 *warp_sums, u64 &all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const u64 incl = warp_inclusive(v);
     __syncthreads();
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
-    T before = 0;
-    all = 0;
-    for (int w = 0; w < SAMPLE_WARPS; w++) {
-        if (w < warp) before += warp_sums[w];
-        all += warp_sums[w];
-    }
-    return before + incl - v;
+    const u64 w = lane < SAMPLE_WARPS ? warp_sums[lane] : 0, wi = warp_inclusive(w);
+    all = __shfl_sync(0xffffffffu, wi, SAMPLE_WARPS - 1);
+    return __shfl_sync(0xffffffffu, wi - w, warp) + incl - v;
+}
+__device__ __forceinline__ void add_u64(uint32_t *lo, uint32_t *hi, u64 v) {
+    const uint32_t l = (uint32_t)v, old = atomicAdd(lo, l);
+    const uint32_t h = (uint32_t)(v >> 32) + (old + l < old ? 1u : 0u);
+    if (h) atomicAdd(hi, h);
 }
 
-__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs a) {
-    __shared__ Shared sh;
+// exp((x - max) / T) in 2^-44 fixed point.  2^y with y = 64ths + r: a table and the series of 2^r to r^5 (|r| <= 1/128: 1e-17).
+struct Weigher {
+    double dmax, scale;  // log2(e) / T
+    const double *table;
+    __device__ __forceinline__ u64 operator()(float x) const {
+        const double y = ((double)x - dmax) * scale;
+        if (!(y > -46.0)) return y == y ? 0 : (u64)FIXED_ONE;  // (NaN: infinity less itself)
+        constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low bits
+        const double kd = fma(y, 64.0, MAGIC);
+        const int k = __double2loint(kd);
+        const double r = fma(kd - MAGIC, -0.015625, y);
+        double p = fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3);  // ln(2)^n / n!
+        p = fma(p, r, 5.5504108664821580e-2);
+        p = fma(p, r, 2.4022650695910072e-1);
+        p = fma(p, r, 6.9314718055994531e-1);
+        p = fma(p, r, 1.0) * table[k & 63];
+        const double v = __hiloint2double(__double2hiint(p) + (((k >> 6) + 44) << 20), __double2loint(p)) + 4503599627370496.0;  // + 2^52
+        return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
+    }
+};
+
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    Shared &sh = *reinterpret_cast<Shared *>(smem_raw);
+    float *xs = reinterpret_cast<float *>(smem_raw + sizeof(Shared));
+    cg::cluster_group cluster = cg::this_cluster();
+    const int CS = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    Shared &first = *cluster.map_shared_rank(&sh, 0);
+    auto cluster_sync = [&]() {
+        if (CS == 1) __syncthreads();
+        else cluster.sync();
+    };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t row = blockIdx.x / CS;
+    const int V = a.V, i_first = rank * a.slice, n = max(0, min(a.slice, V - i_first));
+    if (tid < 64) sh.table[tid] = exp2((double)tid * 0.015625);
+    for (int i = tid; i < BINS; i += SAMPLE_THREADS) sh.lo[i] = sh.hi[i] = sh.glo[i] = sh.ghi[i] = 0;
+    if (tid == 0) {
+        sh.best = 0;
+        sh.kmin = 0xffffffffu;
+    }
     grid_launch_dependents();
     grid_dependency_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int64_t row = blockIdx.x;
-    const int V = a.V;
-    const int64_t base = row * a.ld;
     const float temperature = a.s.temperature_dev ? a.s.temperature_dev[row] : a.s.temperature;
     const float top_p = a.s.top_p_dev ? a.s.top_p_dev[row] : a.s.top_p;
     const float min_p = a.s.min_p_dev ? a.s.min_p_dev[row] : a.s.min_p;
     int top_k = a.s.top_k_dev ? a.s.top_k_dev[row] : a.s.top_k;
     if (top_k <= 0 || top_k > V) top_k = V;
 
-    // largest key and its lowest index
-    unsigned long long best = 0;
-    for (int i = tid; i < V; i += SAMPLE_THREADS) {
-        const unsigned long long k = ((unsigned long long)key_of(load_as_float(a.logits, a.dt, base + i)) << 32) | (0xffffffffu - (uint32_t)i);
-        best = k > best ? k : best;
+    // the row into shared memory (NaN as -inf, -0 as +0); its largest logit with the lowest index, and its smallest
+    u64 best = 0;
+    uint32_t kmin = 0xffffffffu;
+    {
+        const int64_t base = row * a.ld + i_first;
+#pragma unroll 8
+        for (int i = tid; i < n; i += SAMPLE_THREADS) {
+            float x = load_as_float(a.logits, a.dt, base + i) + 0.f;
+            if (x != x) x = -INFINITY;
+            xs[i] = x;
+            const uint32_t k = key_of(x);
+            const u64 c = ((u64)k << 32) | (0xffffffffu - (uint32_t)(i_first + i));
+            best = c > best ? c : best;
+            if (x != -INFINITY) kmin = min(kmin, k);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long x = __shfl_xor_sync(0xffffffffu, best, o);
+        const u64 x = __shfl_xor_sync(0xffffffffu, best, o);
         best = x > best ? x : best;
     }
-    if (lane == 0) sh.warp_sum[warp] = best;
+    kmin = __reduce_min_sync(0xffffffffu, kmin);
     __syncthreads();
-    for (int w = 0; w < SAMPLE_WARPS; w++) best = sh.warp_sum[w] > best ? sh.warp_sum[w] : best;
+    if (lane == 0) {
+        atomicMax(&sh.best, best);
+        atomicMin(&sh.kmin, kmin);
+    }
+    cluster_sync();
+    for (int c = 0; c < CS; c++) {
+        const Shared &o = *cluster.map_shared_rank(&sh, c);
+        best = o.best > best ? o.best : best;
+        kmin = min(kmin, o.kmin);
+    }
     const uint32_t kmax = (uint32_t)(best >> 32);
     const float xmax = of_key(kmax);
-    const int argmax = (int)(0xffffffffu - (uint32_t)best);
     if (xmax == -INFINITY || !(temperature > 0.f)) {
-        if (tid == 0) a.ids[row] = xmax == -INFINITY ? -1 : argmax;
+        if (rank == 0 && tid == 0) a.ids[row] = xmax == -INFINITY ? -1 : (int)(0xffffffffu - (uint32_t)best);
+        cluster_sync();  // (no CTA leaves while another may read its shared memory)
         return;
     }
-    const double dmax = xmax, dtemp = temperature;
-    auto weight = [&](uint32_t k) -> double {
-        return k == kmax ? 1.0 : exp(((double)of_key(k) - dmax) / dtemp);  // (an infinite maximum leaves weight to itself only)
-    };
-    auto fixed = [&](double w) { return (unsigned long long)__double2ull_rn(w * FIXED_ONE); };
+    const Weigher weight{(double)xmax, 1.4426950408889634 / (double)temperature, sh.table};
 
-    // One descent.  Elements: keys above `lim`, and `lim_n` of those equal to it.  Finds the key at which the running count
-    // (by_mass false) or weight (true), from the top, reaches the target: key, copies of it inside, count and weight before it.
-    auto descend = [&](bool by_mass, int target_cnt, double target_mass, uint32_t lim, int lim_n, uint32_t &key, int &copies,
-                       unsigned long long &mass_before) {
-        uint32_t prefix = 0;
-        int cnt_before = 0;
-        mass_before = 0;
-        for (int level = 0; level < 3; level++) {
-            const int shift = level == 0 ? 21 : (level == 1 ? 10 : 0), bits = level == 2 ? 10 : 11;
-            __syncthreads();
-            for (int i = tid; i < BINS; i += SAMPLE_THREADS) sh.cnt[i] = sh.lo[i] = sh.hi[i] = 0;
-            __syncthreads();
-            auto add = [&](uint32_t k, uint32_t n) {
-                if (level > 0 && (k >> (shift + bits)) != prefix) return;
-                const int bin = (k >> shift) & ((1 << bits) - 1);
-                atomicAdd(&sh.cnt[bin], n);
-                const unsigned long long f = fixed(weight(k)) * n;
-                const uint32_t lo = (uint32_t)f, old = atomicAdd(&sh.lo[bin], lo);
-                const uint32_t hi = (uint32_t)(f >> 32) + (old + lo < old ? 1u : 0u);
-                if (hi) atomicAdd(&sh.hi[bin], hi);
-            };
-            for (int i = tid; i < V; i += SAMPLE_THREADS) {
-                const uint32_t k = key_of(load_as_float(a.logits, a.dt, base + i));
-                if (k > lim) add(k, 1);
-            }
-            if (tid == 0) add(lim, (uint32_t)lim_n);
-            __syncthreads();
-            // two bins per thread, the highest first
-            const int b1 = BINS - 1 - 2 * tid, b0 = b1 - 1;
-            const int n1 = (int)sh.cnt[b1], n0 = (int)sh.cnt[b0];
-            const unsigned long long m1 = ((unsigned long long)sh.hi[b1] << 32) | sh.lo[b1], m0 = ((unsigned long long)sh.hi[b0] << 32) | sh.lo[b0];
-            int all_n;
-            unsigned long long all_m;
-            int cn = cnt_before + block_exclusive(n1 + n0, sh.warp_cnt, all_n);
-            unsigned long long cm = mass_before + block_exclusive(m1 + m0, sh.warp_sum, all_m);
-            auto reached = [&](int n, unsigned long long m) { return by_mass ? (double)m >= target_mass : n >= target_cnt; };
-            if (tid == 0) sh.found_bin = -1;
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int n = j == 0 ? n1 : n0, bin = j == 0 ? b1 : b0;
-                const unsigned long long m = j == 0 ? m1 : m0;
-                if (n > 0 && reached(cn + n, cm + m) && !reached(cn, cm)) {
-                    sh.found_bin = bin;
-                    sh.above_cnt = cn;
-                    sh.above_mass = cm;
-                    sh.found_cnt = n;
+    // Level 0: 2048 parts of the range from the largest logit down to the smallest, or to where weights vanish.  Monotone in x: a
+    // difference, a product and a conversion, each rounded.  The last part also holds everything below.
+    const float clip = FIXED_RANGE * temperature, range = fminf(clip, xmax - of_key(kmin)), per_part = (float)BINS / range;
+    auto part_of = [&](float x) { return x == xmax ? 0 : (int)fminf((xmax - x) * per_part, (float)(BINS - 1)); };
+
+    // One descent through the tokens with keys above `lim`, and `lim_n` of those equal to it: the key at which the running count
+    // (by_mass false) or weight (true), from the top, reaches the target; how many tokens of this key are inside and in all.
+    // False: the target is not reached before the weights vanish, nothing is cut.
+    auto descend = [&](bool by_mass, u64 target_n, double p, uint32_t lim, u64 lim_n, uint32_t &key, u64 &inside, u64 &in_all) -> bool {
+        u64 before = 0;
+        double target = 0.0;
+        int level = 0, part = 0, shift = 0;
+        uint32_t top = 0, bottom = 0;  // keys of the levels from 1 on
+        while (true) {
+            // this CTA's tokens into its histogram (level 0) or, few, into the first CTA's (later)
+            uint32_t *lo = level == 0 ? sh.lo : first.glo, *hi = level == 0 ? sh.hi : first.ghi;
+            auto add = [&](float x, uint32_t k, u64 copies) {
+                int bin;
+                if (level == 0) {
+                    bin = part_of(x);
+                } else {
+                    if (k > top || k < bottom) return;
+                    bin = (int)((top - k) >> shift);
                 }
-                cn += n;
-                cm += m;
+                if (by_mass) add_u64(lo + bin, hi + bin, weight(x) * copies);
+                else atomicAdd(lo + bin, (uint32_t)copies);
+            };
+            for (int i = tid; i < n; i += SAMPLE_THREADS) {
+                const float x = xs[i];
+                const uint32_t k = key_of(x);
+                if (k > lim) add(x, k, 1);
             }
-            __syncthreads();
-            const int bin = sh.found_bin;
-            if (bin < 0) {  // (target within rounding of the whole: everything stays)
-                key = lim;
-                copies = lim_n;
-                return;
+            if (lim_n > 0 && rank == 0 && tid == 0) add(of_key(lim), lim, lim_n);
+            if (level == 0) {
+                __syncthreads();
+                for (int i = tid; i < BINS; i += SAMPLE_THREADS) {
+                    const uint32_t l = sh.lo[i], h = sh.hi[i];
+                    if (l | h) {
+                        add_u64(first.glo + i, first.ghi + i, ((u64)h << 32) | l);
+                        sh.lo[i] = sh.hi[i] = 0;
+                    }
+                }
             }
-            cnt_before = sh.above_cnt;
-            mass_before = sh.above_mass;
-            prefix = (prefix << bits) | (uint32_t)bin;
-        }
-        key = prefix;
-        const int have = sh.found_cnt;
-        if (by_mass) {
-            const double each = (double)fixed(weight(key));
-            double r = each > 0.0 ? ceil((target_mass - (double)mass_before) / each) : 1.0;
-            copies = r < 1.0 ? 1 : (r > have ? have : (int)r);
-        } else {
-            copies = target_cnt - cnt_before;
+            cluster_sync();
+            if (rank == 0) {
+                u64 v[BINS_PER_THREAD], mine = 0, all;
+#pragma unroll
+                for (int j = 0; j < BINS_PER_THREAD; j++) {
+                    const int b = BINS_PER_THREAD * tid + j;
+                    v[j] = ((u64)sh.ghi[b] << 32) | sh.glo[b];
+                    sh.glo[b] = sh.ghi[b] = 0;
+                    mine += v[j];
+                }
+                if (tid == 0) sh.found_bin = -1;
+                u64 cum = before + block_exclusive(mine, sh.warp_sum, all);
+                if (level == 0 && by_mass) target = p * (double)all;
+                auto reached = [&](u64 c) { return by_mass ? (double)c >= target : c >= target_n; };
+#pragma unroll
+                for (int j = 0; j < BINS_PER_THREAD; j++) {
+                    if (v[j] > 0 && reached(cum + v[j]) && !reached(cum)) {
+                        sh.found_bin = BINS_PER_THREAD * tid + j;
+                        sh.found_before = cum;
+                        sh.found_mass = v[j];
+                    }
+                    cum += v[j];
+                }
+                if (tid == 0) {
+                    sh.range_lo = 0xffffffffu;
+                    sh.range_hi = 0;
+                }
+            }
+            cluster_sync();
+            const int bin = first.found_bin;
+            before = first.found_before;
+            if (bin < 0 || (level == 0 && bin == BINS - 1 && range == clip)) {
+                cluster_sync();  // (the result is written again)
+                return false;
+            }
+            if (level == 0) {
+                // the keys of the part's tokens
+                part = bin;
+                uint32_t klo = 0xffffffffu, khi = 0;
+                auto see = [&](float x, uint32_t k) {
+                    if (part_of(x) == part) {
+                        klo = min(klo, k);
+                        khi = max(khi, k);
+                    }
+                };
+                for (int i = tid; i < n; i += SAMPLE_THREADS) {
+                    const float x = xs[i];
+                    const uint32_t k = key_of(x);
+                    if (k > lim) see(x, k);
+                }
+                if (lim_n > 0 && rank == 0 && tid == 0) see(of_key(lim), lim);
+                klo = __reduce_min_sync(0xffffffffu, klo);
+                khi = __reduce_max_sync(0xffffffffu, khi);
+                if (lane == 0 && khi > 0) {
+                    atomicMin(&first.range_lo, klo);
+                    atomicMax(&first.range_hi, khi);
+                }
+                cluster_sync();
+                bottom = first.range_lo;
+                top = first.range_hi;
+            } else {
+                if (shift == 0) {
+                    key = top - (uint32_t)bin;
+                    const u64 mass = first.found_mass;
+                    if (by_mass) {
+                        const u64 each = weight(of_key(key));
+                        in_all = each > 0 ? mass / each : 1;
+                        // `target` is known to the first CTA only: it shares the number of tokens inside
+                        if (rank == 0 && tid == 0) {
+                            const double r = each > 0 ? ceil((target - (double)before) / (double)each) : 1.0;
+                            sh.found_n = r < 1.0 ? 1 : (r > (double)in_all ? (int)in_all : (int)r);
+                        }
+                        cluster_sync();
+                        inside = (u64)first.found_n;
+                    } else {
+                        in_all = mass;
+                        inside = target_n - before;
+                    }
+                    cluster_sync();  // (the result is written again)
+                    return true;
+                }
+                const uint32_t up = top - ((uint32_t)bin << shift);
+                const uint32_t down = up - ((1u << shift) - 1u);
+                bottom = down < bottom || down > up ? bottom : down;
+                top = up;
+            }
+            shift = 0;
+            while (((top - bottom) >> shift) >= (uint32_t)BINS) shift++;
+            level++;
+            // (the first CTA has cleared its histogram before the barrier that published the bin)
         }
     };
 
-    // cut: keys above cut_key and the first cut_n of those equal to it
+    // cut: keys above cut_key and the first cut_n of the cut_all equal to it
     uint32_t cut_key = 0;
-    int cut_n = V;
-    unsigned long long before;
-    if (top_k < V) descend(false, top_k, 0.0, 0, 0, cut_key, cut_n, before);
+    u64 cut_n = 0, cut_all = 0;
+    if (top_k < V && !descend(false, (u64)top_k, 0.0, 0, 0, cut_key, cut_n, cut_all)) cut_key = 0, cut_n = cut_all = 0;
     if (top_p < 1.f) {
-        unsigned long long total;
-        if (top_k < V) {
-            total = before + fixed(weight(cut_key)) * (unsigned long long)cut_n;
-        } else {
-            unsigned long long mine = 0;
-            for (int i = tid; i < V; i += SAMPLE_THREADS) mine += fixed(weight(key_of(load_as_float(a.logits, a.dt, base + i))));
-            block_exclusive(mine, sh.warp_sum, total);
-        }
-        const double target = fmax((double)top_p, 0.0) * (double)total;
-        const uint32_t lim = top_k < V ? cut_key : 0;
-        const int lim_n = top_k < V ? cut_n : 0;
-        if (target > 0.0) {
-            descend(true, 0, target, lim, lim_n, cut_key, cut_n, before);
-        } else {
+        uint32_t key;
+        u64 inside, in_all;
+        if (top_p > 0.f) {
+            if (descend(true, 0, (double)top_p, cut_key, cut_n, key, inside, in_all)) {
+                cut_all = key == cut_key ? cut_all : in_all;  // (at the count's cut only its own copies were weighed)
+                cut_key = key;
+                cut_n = inside;
+            }
+        } else {  // one token: the largest logit, lowest index
             cut_key = kmax;
             cut_n = 1;
+            cut_all = 2;  // ties are ranked below
         }
     }
 
-    // what is left, in the order of the vocabulary: every warp a contiguous run of it
-    const int run = (V + SAMPLE_WARPS - 1) / SAMPLE_WARPS, i0 = warp * run, i1 = min(V, i0 + run);
-    // first the tokens that tie with the cut
-    int ties = 0;
-    for (int i = i0 + lane; i < i1; i += 32) ties += key_of(load_as_float(a.logits, a.dt, base + i)) == cut_key;
-    ties = __reduce_add_sync(0xffffffffu, ties);
-    int all_ties;
-    int ties_before = block_exclusive(lane == 0 ? ties : 0, sh.warp_cnt, all_ties);
-    ties_before = __shfl_sync(0xffffffffu, ties_before, 0);
-    // weight that token i keeps; `tie_rank`: ties before it
-    auto kept = [&](uint32_t k, int tie_rank) -> unsigned long long {
-        if (k < cut_key || (k == cut_key && tie_rank >= cut_n)) return 0;
-        const double w = weight(k);
-        return w >= (double)min_p || k == kmax ? fixed(w) : 0;
-    };
-    auto walk = [&](auto &&visit) {  // visit(i, kept weight, whole chunk) over this warp's run; false ends it
-        int tie = ties_before;
+    // what is left, in the order of the vocabulary: every warp a contiguous run of the slice
+    const int run = (n + SAMPLE_WARPS - 1) / SAMPLE_WARPS, i0 = min(n, warp * run), i1 = min(n, i0 + run);
+    u64 ties_before = 0;
+    const bool rank_ties = cut_n < cut_all;
+    if (rank_ties) {
+        u64 ties = 0, all;
+        for (int i = i0 + lane; i < i1; i += 32) ties += key_of(xs[i]) == cut_key;
+        ties = (u64)__reduce_add_sync(0xffffffffu, (unsigned)ties);
+        ties_before = __shfl_sync(0xffffffffu, block_exclusive(lane == 0 ? ties : 0, sh.warp_sum, all), 0);
+        if (tid == 0) sh.ties = (int)all;
+        cluster_sync();
+        for (int c = 0; c < rank; c++) ties_before += (u64)cluster.map_shared_rank(&sh, c)->ties;
+    }
+    const double floor_w = (double)min_p * FIXED_ONE;
+    auto walk = [&](auto &&visit) {  // visit(i, kept weight) over this warp's run, 32 tokens at a time; false ends it
+        u64 tie = ties_before;
         for (int i = i0; i < i1; i += 32) {
             const bool in = i + lane < i1;
-            const uint32_t k = in ? key_of(load_as_float(a.logits, a.dt, base + i + lane)) : 0;
-            const unsigned eq = __ballot_sync(0xffffffffu, in && k == cut_key);
-            const unsigned long long w = in ? kept(k, tie + __popc(eq & ((1u << lane) - 1u))) : 0;
-            tie += __popc(eq);
+            const float x = in ? xs[i + lane] : -INFINITY;
+            const uint32_t k = key_of(x);
+            bool keep = in && k >= cut_key;
+            if (rank_ties) {
+                const unsigned eq = __ballot_sync(0xffffffffu, in && k == cut_key);
+                if (k == cut_key && tie + __popc(eq & ((1u << lane) - 1u)) >= cut_n) keep = false;
+                tie += __popc(eq);
+            }
+            u64 w = 0;
+            if (__any_sync(0xffffffffu, keep)) {
+                if (keep) w = weight(x);
+                if ((double)w < floor_w && k != kmax) w = 0;
+            }
             if (!visit(i + lane, w)) break;
         }
     };
-    unsigned long long mine = 0, total;
-    walk([&](int, unsigned long long w) { mine += w; return true; });
+    u64 mine = 0, here;
+    walk([&](int, u64 w) { mine += w; return true; });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    unsigned long long start = block_exclusive(lane == 0 ? mine : 0ull, sh.warp_sum, total);
-    start = __shfl_sync(0xffffffffu, start, 0);
-    // first token whose cumulative weight exceeds the target; the last one with weight if rounding leaves none
+    u64 start = __shfl_sync(0xffffffffu, block_exclusive(lane == 0 ? mine : 0, sh.warp_sum, here), 0);
+    if (tid == 0) sh.mass = here;
+    cluster_sync();
+    u64 total = 0;
+    for (int c = 0; c < CS; c++) {
+        const u64 m = cluster.map_shared_rank(&sh, c)->mass;
+        if (c < rank) start += m;
+        total += m;
+    }
+    cluster_sync();  // (no CTA leaves while another may read its shared memory)
+    // first token whose cumulative weight exceeds the target
     double target = (double)fminf(fmaxf(a.u[row], 0.f), 1.f) * (double)total;
     if (target >= (double)total) target = (double)(total - 1);
     if (mine > 0 && (double)start <= target && target < (double)(start + mine)) {
-        unsigned long long cum = start;
-        walk([&](int i, unsigned long long w) {
-            unsigned long long incl = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long x = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += x;
-            }
+        u64 cum = start;
+        walk([&](int i, u64 w) {
+            const u64 incl = warp_inclusive(w);
             const unsigned hit = __ballot_sync(0xffffffffu, (double)(cum + incl) > target);
             if (hit) {
-                if (lane == __ffs(hit) - 1) a.ids[row] = i;
+                if (lane == __ffs(hit) - 1) a.ids[row] = i_first + i;
                 return false;
             }
             cum += __shfl_sync(0xffffffffu, incl, 31);
@@ -262,9 +402,30 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
 
 cudaError_t launch_sample(const void *logits, int dt, int64_t M, int V, int64_t ld, const ttq_sampling &s, const float *u, int64_t *ids, int sms,
                           cudaStream_t st) {
-    (void)sms;
-    const SampleArgs a{logits, dt, V, ld, s, u, ids};
-    return launch_pdl(sample_kernel, dim3((unsigned)M), dim3(SAMPLE_THREADS), 0, st, a);
+    // CTAs per row: as many as it takes to fill the card with two CTAs per SM, at least so many that two fit there with their slices
+    // (a row of 2^18 logits: 128 KB a CTA, one per SM)
+    int cluster = 1;
+    while (cluster < MAX_CLUSTER && ((int64_t)M * cluster * 2 <= 2 * (int64_t)sms || (V + cluster - 1) / cluster > 18432) && V / cluster > SAMPLE_THREADS) cluster *= 2;
+    const int slice = (V + cluster - 1) / cluster;
+    const size_t smem = sizeof(Shared) + (size_t)slice * sizeof(float);
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(Shared) + ((1 << 18) / MAX_CLUSTER) * sizeof(float)));
+    if (e != cudaSuccess) return e;
+    static const bool pdl = env_flag("TTQ_PDL", true);
+    const SampleArgs a{logits, dt, V, slice, ld, s, u, ids};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(M * cluster));
+    cfg.blockDim = dim3(SAMPLE_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, sample_kernel, a);
 }
 
 }  // namespace ttq
