@@ -7,9 +7,10 @@
 // tokens of similar weight falls on a neighbour of the right one about once in 400 rows.
 //
 // A cluster of CTAs holds a row in shared memory, so the logits are read once.  The cut is found by histograms of counts or weights:
-// first over 2048 equal parts of the range that has weight (max - 32 T to max: evenly spread logits, few collisions), then over the
-// order-preserving keys of the part's logits, 2048 at a time, until a bin is one key.  What a bin needs of all CTAs is added into the
-// first one's shared memory.  Bound: one reading of the logits; in practice the 64-bit exponentials (11 instructions each, half the
+// first over 2048 equal parts of the range that has weight (max - 32 T to max: evenly spread logits, few collisions).  The tokens of the
+// part with the cut, a few hundred, go to the first CTA, which goes on alone: histograms over the order-preserving keys, 2048 at
+// a time, until a bin is one key.  (Only where a part holds more than LIST tokens do all CTAs go on, adding into the first
+// one's histogram.)  Bound: one reading of the logits; in practice the 64-bit exponentials (11 instructions each, half the
 // rate of 32-bit ones) for large batches, the chain of cluster barriers for small ones.
 #include <cooperative_groups.h>
 
@@ -23,6 +24,7 @@ namespace cg = cooperative_groups;
 constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int BINS = 2048, BINS_PER_THREAD = BINS / SAMPLE_THREADS;
+constexpr int LIST = 2048;     // tokens that the first CTA takes over
 constexpr int MAX_CLUSTER = 8;
 constexpr double FIXED_ONE = 17592186044416.0;  // 2^44
 constexpr float FIXED_RANGE = 32.f;              // exp(-32 * 2047 / 2048) < 2^-46: no weight in the last part
@@ -45,8 +47,8 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct Shared {
-    uint32_t lo[BINS], hi[BINS];    // this CTA's histogram
-    uint32_t glo[BINS], ghi[BINS];  // the row's (first CTA)
+    uint32_t lo[BINS], hi[BINS];    // this CTA's histogram; the first CTA's becomes the row's
+    uint32_t list[LIST];            // keys of the tokens that decide (first CTA)
     double table[64];               // 2^(j / 64)
     u64 warp_sum[SAMPLE_WARPS];
     // exchanged between the CTAs of a row
@@ -55,7 +57,11 @@ struct Shared {
     int ties;
     // a level's result (first CTA)
     u64 found_before, found_mass;
-    int found_bin, found_n;
+    int found_bin, list_n;
+    // a descent's (first CTA)
+    uint32_t cut_key;
+    u64 cut_inside, cut_all;
+    int cut_found;
 };
 
 template <class T>
@@ -121,10 +127,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     const int64_t row = blockIdx.x / CS;
     const int V = a.V, i_first = rank * a.slice, n = max(0, min(a.slice, V - i_first));
     if (tid < 64) sh.table[tid] = exp2((double)tid * 0.015625);
-    for (int i = tid; i < BINS; i += SAMPLE_THREADS) sh.lo[i] = sh.hi[i] = sh.glo[i] = sh.ghi[i] = 0;
+    for (int i = tid; i < BINS; i += SAMPLE_THREADS) sh.lo[i] = sh.hi[i] = 0;
     if (tid == 0) {
         sh.best = 0;
         sh.kmin = 0xffffffffu;
+        sh.list_n = 0;
     }
     grid_launch_dependents();
     grid_dependency_wait();
@@ -138,16 +145,41 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     u64 best = 0;
     uint32_t kmin = 0xffffffffu;
     {
-        const int64_t base = row * a.ld + i_first;
-#pragma unroll 8
-        for (int i = tid; i < n; i += SAMPLE_THREADS) {
-            float x = load_as_float(a.logits, a.dt, base + i) + 0.f;
-            if (x != x) x = -INFINITY;
+        auto take = [&](int i, float x) {
+            x = x != x ? -INFINITY : x + 0.f;
             xs[i] = x;
             const uint32_t k = key_of(x);
             const u64 c = ((u64)k << 32) | (0xffffffffu - (uint32_t)(i_first + i));
             best = c > best ? c : best;
             if (x != -INFINITY) kmin = min(kmin, k);
+        };
+        // 16 bytes per load from the first aligned address on, all in flight together
+        const int size = a.dt == TTQ_DT_F32 ? 4 : 2, per = 16 / size;
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(a.logits) + (row * a.ld + i_first) * size;
+        const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15) / size), groups = (n - head) / per;
+        if (tid < head) take(tid, load_as_float(src, a.dt, tid));
+        if (tid < n - head - groups * per) take(head + groups * per + tid, load_as_float(src, a.dt, head + groups * per + tid));
+        const uint4 *vec = reinterpret_cast<const uint4 *>(src + head * size);
+        for (int g0 = tid; g0 < groups; g0 += 8 * SAMPLE_THREADS) {
+            uint4 r[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (g0 + j * SAMPLE_THREADS < groups) r[j] = vec[g0 + j * SAMPLE_THREADS];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int g = g0 + j * SAMPLE_THREADS;
+                if (g >= groups) break;
+                if (size == 4) {
+                    const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
+#pragma unroll
+                    for (int q = 0; q < 4; q++) take(head + 4 * g + q, __uint_as_float(w[q]));
+                } else {
+                    float f[8];
+                    xh_unpack(r[j], a.dt, f);
+#pragma unroll
+                    for (int q = 0; q < 8; q++) take(head + 8 * g + q, f[q]);
+                }
+            }
         }
     }
 #pragma unroll
@@ -181,146 +213,189 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     const float clip = FIXED_RANGE * temperature, range = fminf(clip, xmax - of_key(kmin)), per_part = (float)BINS / range;
     auto part_of = [&](float x) { return x == xmax ? 0 : (int)fminf((xmax - x) * per_part, (float)(BINS - 1)); };
 
-    // One descent through the tokens with keys above `lim`, and `lim_n` of those equal to it: the key at which the running count
-    // (by_mass false) or weight (true), from the top, reaches the target; how many tokens of this key are inside and in all.
-    // False: the target is not reached before the weights vanish, nothing is cut.
-    auto descend = [&](bool by_mass, u64 target_n, double p, uint32_t lim, u64 lim_n, uint32_t &key, u64 &inside, u64 &in_all) -> bool {
-        u64 before = 0;
-        double target = 0.0;
-        int level = 0, part = 0, shift = 0;
-        uint32_t top = 0, bottom = 0;  // keys of the levels from 1 on
-        while (true) {
-            // this CTA's tokens into its histogram (level 0) or, few, into the first CTA's (later)
-            uint32_t *lo = level == 0 ? sh.lo : first.glo, *hi = level == 0 ? sh.hi : first.ghi;
-            auto add = [&](float x, uint32_t k, u64 copies) {
-                int bin;
-                if (level == 0) {
-                    bin = part_of(x);
-                } else {
-                    if (k > top || k < bottom) return;
-                    bin = (int)((top - k) >> shift);
-                }
-                if (by_mass) add_u64(lo + bin, hi + bin, weight(x) * copies);
-                else atomicAdd(lo + bin, (uint32_t)copies);
-            };
-            for (int i = tid; i < n; i += SAMPLE_THREADS) {
-                const float x = xs[i];
-                const uint32_t k = key_of(x);
-                if (k > lim) add(x, k, 1);
+    // every token of this CTA: f(logit, key), four at a time
+    auto each_token = [&](auto &&f) {
+        int i = tid;
+        for (; i + 3 * SAMPLE_THREADS < n; i += 4 * SAMPLE_THREADS) {
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = xs[i + j * SAMPLE_THREADS];
+#pragma unroll
+            for (int j = 0; j < 4; j++) f(x[j], key_of(x[j]));
+        }
+        for (; i < n; i += SAMPLE_THREADS) f(xs[i], key_of(xs[i]));
+    };
+    // The first CTA: the bin of the row's histogram at which the running count or weight, from `before` on, reaches the target (-1:
+    // none), and the histogram cleared.  `p` >= 0: the target is this part of the whole.
+    auto scan = [&](bool by_mass, u64 before, u64 target_n, double &target, double p) {
+        u64 v[BINS_PER_THREAD], mine = 0, all;
+#pragma unroll
+        for (int j = 0; j < BINS_PER_THREAD; j++) {
+            const int b = BINS_PER_THREAD * tid + j;
+            v[j] = ((u64)sh.hi[b] << 32) | sh.lo[b];
+            sh.lo[b] = sh.hi[b] = 0;
+            mine += v[j];
+        }
+        if (tid == 0) sh.found_bin = -1;
+        u64 cum = before + block_exclusive(mine, sh.warp_sum, all);
+        if (p >= 0.0) target = p * (double)all;
+        auto reached = [&](u64 c) { return by_mass ? (double)c >= target : c >= target_n; };
+#pragma unroll
+        for (int j = 0; j < BINS_PER_THREAD; j++) {
+            if (v[j] > 0 && reached(cum + v[j]) && !reached(cum)) {
+                sh.found_bin = BINS_PER_THREAD * tid + j;
+                sh.found_before = cum;
+                sh.found_mass = v[j];
             }
-            if (lim_n > 0 && rank == 0 && tid == 0) add(of_key(lim), lim, lim_n);
-            if (level == 0) {
-                __syncthreads();
+            cum += v[j];
+        }
+        __syncthreads();
+    };
+
+    // One descent through the tokens with keys above `lim`, and `lim_n` of those equal to it: the key at which the running count
+    // (by_mass false) or weight (true: p of the whole), from the top, reaches the target; how many tokens of this key are inside
+    // and in all.  `few`: no more than LIST tokens are above `lim`.  False: the target is not reached before the weights vanish,
+    // nothing is cut.
+    auto descend = [&](bool by_mass, u64 target_n, double p, uint32_t lim, u64 lim_n, bool few, uint32_t &key, u64 &inside, u64 &in_all) -> bool {
+        double target = 0.0;  // (the first CTA's)
+        u64 before = 0;
+        int part = -1;
+        if (!few) {
+            auto add = [&](float x, u64 copies) {
+                const int bin = part_of(x);
+                if (by_mass) add_u64(sh.lo + bin, sh.hi + bin, weight(x) * copies);
+                else atomicAdd(sh.lo + bin, (uint32_t)copies);
+            };
+            each_token([&](float x, uint32_t k) {
+                if (k > lim) add(x, 1);
+            });
+            if (lim_n > 0 && rank == 0 && tid == 0) add(of_key(lim), lim_n);
+            __syncthreads();
+            if (rank > 0)
                 for (int i = tid; i < BINS; i += SAMPLE_THREADS) {
                     const uint32_t l = sh.lo[i], h = sh.hi[i];
                     if (l | h) {
-                        add_u64(first.glo + i, first.ghi + i, ((u64)h << 32) | l);
+                        add_u64(first.lo + i, first.hi + i, ((u64)h << 32) | l);
                         sh.lo[i] = sh.hi[i] = 0;
                     }
                 }
-            }
             cluster_sync();
-            if (rank == 0) {
-                u64 v[BINS_PER_THREAD], mine = 0, all;
-#pragma unroll
-                for (int j = 0; j < BINS_PER_THREAD; j++) {
-                    const int b = BINS_PER_THREAD * tid + j;
-                    v[j] = ((u64)sh.ghi[b] << 32) | sh.glo[b];
-                    sh.glo[b] = sh.ghi[b] = 0;
-                    mine += v[j];
-                }
-                if (tid == 0) sh.found_bin = -1;
-                u64 cum = before + block_exclusive(mine, sh.warp_sum, all);
-                if (level == 0 && by_mass) target = p * (double)all;
-                auto reached = [&](u64 c) { return by_mass ? (double)c >= target : c >= target_n; };
-#pragma unroll
-                for (int j = 0; j < BINS_PER_THREAD; j++) {
-                    if (v[j] > 0 && reached(cum + v[j]) && !reached(cum)) {
-                        sh.found_bin = BINS_PER_THREAD * tid + j;
-                        sh.found_before = cum;
-                        sh.found_mass = v[j];
-                    }
-                    cum += v[j];
-                }
-                if (tid == 0) {
-                    sh.range_lo = 0xffffffffu;
-                    sh.range_hi = 0;
-                }
-            }
+            if (rank == 0) scan(by_mass, 0, target_n, target, by_mass ? p : -1.0);
             cluster_sync();
-            const int bin = first.found_bin;
+            part = first.found_bin;
             before = first.found_before;
-            if (bin < 0 || (level == 0 && bin == BINS - 1 && range == clip)) {
-                cluster_sync();  // (the result is written again)
-                return false;
+            if (part < 0 || (part == BINS - 1 && range == clip)) return false;
+        }
+        // the part's tokens to the first CTA
+        auto chosen = [&](float x, uint32_t k) { return k > lim && (part < 0 || part_of(x) == part); };
+        each_token([&](float x, uint32_t k) {
+            if (chosen(x, k)) {
+                const int at = atomicAdd(&first.list_n, 1);
+                if (at < LIST) first.list[at] = k;
             }
-            if (level == 0) {
-                // the keys of the part's tokens
-                part = bin;
-                uint32_t klo = 0xffffffffu, khi = 0;
-                auto see = [&](float x, uint32_t k) {
-                    if (part_of(x) == part) {
-                        klo = min(klo, k);
-                        khi = max(khi, k);
-                    }
-                };
-                for (int i = tid; i < n; i += SAMPLE_THREADS) {
-                    const float x = xs[i];
-                    const uint32_t k = key_of(x);
-                    if (k > lim) see(x, k);
-                }
-                if (lim_n > 0 && rank == 0 && tid == 0) see(of_key(lim), lim);
-                klo = __reduce_min_sync(0xffffffffu, klo);
-                khi = __reduce_max_sync(0xffffffffu, khi);
-                if (lane == 0 && khi > 0) {
-                    atomicMin(&first.range_lo, klo);
-                    atomicMax(&first.range_hi, khi);
-                }
-                cluster_sync();
-                bottom = first.range_lo;
-                top = first.range_hi;
-            } else {
-                if (shift == 0) {
-                    key = top - (uint32_t)bin;
-                    const u64 mass = first.found_mass;
-                    if (by_mass) {
-                        const u64 each = weight(of_key(key));
-                        in_all = each > 0 ? mass / each : 1;
-                        // `target` is known to the first CTA only: it shares the number of tokens inside
-                        if (rank == 0 && tid == 0) {
-                            const double r = each > 0 ? ceil((target - (double)before) / (double)each) : 1.0;
-                            sh.found_n = r < 1.0 ? 1 : (r > (double)in_all ? (int)in_all : (int)r);
+        });
+        cluster_sync();
+        const int listed = first.list_n;
+        const bool alone = listed <= LIST, with_lim = lim_n > 0 && (part < 0 || part_of(of_key(lim)) == part);
+        if (rank == 0 || !alone) {
+            auto sync = [&]() {
+                if (alone) __syncthreads();
+                else cluster_sync();
+            };
+            if (alone && few && by_mass) {  // the whole has not been weighed yet
+                u64 mine = 0, all;
+                for (int i = tid; i < listed; i += SAMPLE_THREADS) mine += weight(of_key(sh.list[i]));
+                if (tid == 0 && with_lim) mine += weight(of_key(lim)) * lim_n;
+                block_exclusive(mine, sh.warp_sum, all);
+                target = p * (double)all;
+            }
+            // keys in [bottom, top], 2048 bins of 2^shift keys at a time
+            uint32_t klo = 0xffffffffu, khi = 0;
+            auto tokens = [&](auto &&f) {
+                if (alone)
+                    for (int i = tid; i < listed; i += SAMPLE_THREADS) f(sh.list[i], (u64)1);
+                else
+                    each_token([&](float x, uint32_t k) {
+                        if (chosen(x, k)) f(k, (u64)1);
+                    });
+                if (with_lim && rank == 0 && tid == 0) f(lim, lim_n);
+            };
+            tokens([&](uint32_t k, u64) {
+                klo = min(klo, k);
+                khi = max(khi, k);
+            });
+            if (rank == 0 && tid == 0) {
+                sh.range_lo = 0xffffffffu;
+                sh.range_hi = 0;
+            }
+            klo = __reduce_min_sync(0xffffffffu, klo);
+            khi = __reduce_max_sync(0xffffffffu, khi);
+            sync();
+            if (lane == 0 && khi > 0) {
+                atomicMin(&first.range_lo, klo);
+                atomicMax(&first.range_hi, khi);
+            }
+            sync();
+            uint32_t bottom = first.range_lo, top = first.range_hi;
+            while (true) {
+                int shift = 0;
+                while (((top - bottom) >> shift) >= (uint32_t)BINS) shift++;
+                tokens([&](uint32_t k, u64 copies) {
+                    if (k > top || k < bottom) return;
+                    const int bin = (int)((top - k) >> shift);
+                    if (by_mass) add_u64(first.lo + bin, first.hi + bin, weight(of_key(k)) * copies);
+                    else atomicAdd(first.lo + bin, (uint32_t)copies);
+                });
+                sync();
+                if (rank == 0) scan(by_mass, before, target_n, target, -1.0);
+                sync();
+                const int bin = first.found_bin;
+                if (bin >= 0) before = first.found_before;
+                if (bin < 0 || shift == 0) {
+                    if (rank == 0 && tid == 0) {
+                        sh.cut_found = bin >= 0;
+                        if (bin >= 0) {
+                            const uint32_t k = top - (uint32_t)bin;
+                            sh.cut_key = k;
+                            if (by_mass) {
+                                const u64 each = weight(of_key(k));  // (a bin with weight was found)
+                                const u64 have = sh.found_mass / each;
+                                const double r = ceil((target - (double)before) / (double)each);
+                                sh.cut_all = have;
+                                sh.cut_inside = r < 1.0 ? 1 : (r > (double)have ? have : (u64)r);
+                            } else {
+                                sh.cut_all = sh.found_mass;
+                                sh.cut_inside = target_n - before;
+                            }
                         }
-                        cluster_sync();
-                        inside = (u64)first.found_n;
-                    } else {
-                        in_all = mass;
-                        inside = target_n - before;
                     }
-                    cluster_sync();  // (the result is written again)
-                    return true;
+                    break;
                 }
-                const uint32_t up = top - ((uint32_t)bin << shift);
-                const uint32_t down = up - ((1u << shift) - 1u);
+                const uint32_t up = top - ((uint32_t)bin << shift), down = up - ((1u << shift) - 1u);
                 bottom = down < bottom || down > up ? bottom : down;
                 top = up;
+                sync();  // (the result is written again)
             }
-            shift = 0;
-            while (((top - bottom) >> shift) >= (uint32_t)BINS) shift++;
-            level++;
-            // (the first CTA has cleared its histogram before the barrier that published the bin)
         }
+        cluster_sync();
+        const bool found = first.cut_found != 0;
+        key = first.cut_key;
+        inside = first.cut_inside;
+        in_all = first.cut_all;
+        if (rank == 0 && tid == 0) sh.list_n = 0;
+        cluster_sync();  // (the list and the result are written again)
+        return found;
     };
 
     // cut: keys above cut_key and the first cut_n of the cut_all equal to it
     uint32_t cut_key = 0;
     u64 cut_n = 0, cut_all = 0;
-    if (top_k < V && !descend(false, (u64)top_k, 0.0, 0, 0, cut_key, cut_n, cut_all)) cut_key = 0, cut_n = cut_all = 0;
+    if (top_k < V && !descend(false, (u64)top_k, 0.0, 0, 0, false, cut_key, cut_n, cut_all)) cut_key = 0, cut_n = cut_all = 0;
     if (top_p < 1.f) {
         uint32_t key;
         u64 inside, in_all;
         if (top_p > 0.f) {
-            if (descend(true, 0, (double)top_p, cut_key, cut_n, key, inside, in_all)) {
+            if (descend(true, 0, (double)top_p, cut_key, cut_n, cut_n > 0 && top_k <= LIST, key, inside, in_all)) {
                 cut_all = key == cut_key ? cut_all : in_all;  // (at the count's cut only its own copies were weighed)
                 cut_key = key;
                 cut_n = inside;
