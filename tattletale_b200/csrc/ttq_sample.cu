@@ -8,8 +8,8 @@
 //
 // A cluster of CTAs holds a row in shared memory, so the logits are read once.  The cut is found by histograms of counts or weights:
 // first over 2048 equal parts of the range that has weight (max - 32 T to max: evenly spread logits, few collisions).  The tokens of the
-// part with the cut, a few hundred, go to the first CTA, which goes on alone: histograms over the order-preserving keys, 2048 at
-// a time, until a bin is one key.  (Only where a part holds more than LIST tokens do all CTAs go on, adding into the first
+// part with the cut, a few hundred, go to the first CTA, which goes on alone: each against each, or, above 512, histograms over the
+// order-preserving keys, 2048 at a time, until a bin is one key.  (Only where a part holds more than LIST tokens do all CTAs go on, adding into the first
 // one's histogram.)  Bound: one reading of the logits; in practice the 64-bit exponentials (11 instructions each, half the
 // rate of 32-bit ones) for large batches, the chain of cluster barriers for small ones.
 #include <cooperative_groups.h>
@@ -25,6 +25,7 @@ constexpr int SAMPLE_THREADS = 512;
 constexpr int SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int BINS = 2048, BINS_PER_THREAD = BINS / SAMPLE_THREADS;
 constexpr int LIST = 2048;     // tokens that the first CTA takes over
+constexpr int PAIRS = 512;     // of which so many are compared pair by pair (a thread each)
 constexpr int MAX_CLUSTER = 8;
 constexpr double FIXED_ONE = 17592186044416.0;  // 2^44
 constexpr float FIXED_RANGE = 32.f;              // exp(-32 * 2047 / 2048) < 2^-46: no weight in the last part
@@ -48,7 +49,8 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 
 struct Shared {
     uint32_t lo[BINS], hi[BINS];    // this CTA's histogram; the first CTA's becomes the row's
-    uint32_t list[LIST];            // keys of the tokens that decide (first CTA)
+    u64 list_w[PAIRS + 1];          // and their counts or weights
+    uint32_t list[LIST + 1];        // keys of the tokens that decide (first CTA)
     double table[64];               // 2^(j / 64)
     u64 warp_sum[SAMPLE_WARPS];
     // exchanged between the CTAs of a row
@@ -96,8 +98,9 @@ struct Weigher {
     double dmax, scale;  // log2(e) / T
     const double *table;
     __device__ __forceinline__ u64 operator()(float x) const {
-        const double y = ((double)x - dmax) * scale;
-        if (!(y > -46.0)) return y == y ? 0 : (u64)FIXED_ONE;  // (NaN: infinity less itself)
+        const double d = ((double)x - dmax) * scale;
+        const bool live = d > -46.0;
+        const double y = live ? d : 0.0;
         constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low bits
         const double kd = fma(y, 64.0, MAGIC);
         const int k = __double2loint(kd);
@@ -108,7 +111,8 @@ struct Weigher {
         p = fma(p, r, 6.9314718055994531e-1);
         p = fma(p, r, 1.0) * table[k & 63];
         const double v = __hiloint2double(__double2hiint(p) + (((k >> 6) + 44) << 20), __double2loint(p)) + 4503599627370496.0;  // + 2^52
-        return (u64)__double_as_longlong(v) & 0xfffffffffffffull;
+        const u64 w = (u64)__double_as_longlong(v) & 0xfffffffffffffull;
+        return live ? w : (d == d ? 0 : (u64)FIXED_ONE);  // (NaN: infinity less itself)
     }
 };
 
@@ -194,10 +198,16 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         atomicMin(&sh.kmin, kmin);
     }
     cluster_sync();
-    for (int c = 0; c < CS; c++) {
-        const Shared &o = *cluster.map_shared_rank(&sh, c);
-        best = o.best > best ? o.best : best;
-        kmin = min(kmin, o.kmin);
+    {
+        const Shared &o = *cluster.map_shared_rank(&sh, lane < CS ? lane : 0);
+        best = o.best;
+        kmin = __reduce_min_sync(0xffffffffu, o.kmin);
+#pragma unroll
+        for (int m = MAX_CLUSTER / 2; m > 0; m >>= 1) {
+            const u64 x = __shfl_xor_sync(0xffffffffu, best, m);
+            best = x > best ? x : best;
+        }
+        best = __shfl_sync(0xffffffffu, best, 0);
     }
     const uint32_t kmax = (uint32_t)(best >> 32);
     const float xmax = of_key(kmax);
@@ -309,6 +319,42 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 block_exclusive(mine, sh.warp_sum, all);
                 target = p * (double)all;
             }
+            if (alone && listed <= PAIRS) {
+                const int entries = listed + (with_lim ? 1 : 0);
+                for (int i = tid; i < entries; i += SAMPLE_THREADS) {
+                    const uint32_t k = i < listed ? sh.list[i] : lim;
+                    const u64 copies = i < listed ? 1 : lim_n;
+                    if (i == listed) sh.list[i] = lim;
+                    sh.list_w[i] = by_mass ? weight(of_key(k)) * copies : copies;
+                }
+                if (tid == 0) sh.cut_found = 0;
+                __syncthreads();
+                for (int i = tid; i < entries; i += SAMPLE_THREADS) {
+                    const uint32_t k = sh.list[i];
+                    u64 above = before, same = 0;
+                    int ties = 0;
+#pragma unroll 4
+                    for (int j = 0; j < entries; j++) {
+                        const uint32_t kj = sh.list[j];
+                        const u64 w = sh.list_w[j];
+                        if (kj > k) above += w;
+                        if (kj == k) same += w, ties++;
+                    }
+                    auto reached = [&](u64 c) { return by_mass ? (double)c >= target : c >= target_n; };
+                    if (same > 0 && reached(above + same) && !reached(above)) {  // (one key; its ties write the same)
+                        const u64 have = i < listed ? (u64)ties : lim_n;
+                        sh.cut_key = k;
+                        sh.cut_all = have;
+                        if (by_mass) {
+                            const double r = ceil((target - (double)above) / (double)(same / have));
+                            sh.cut_inside = r < 1.0 ? 1 : (r > (double)have ? have : (u64)r);
+                        } else {
+                            sh.cut_inside = target_n - above;
+                        }
+                        sh.cut_found = 1;
+                    }
+                }
+            } else {
             // keys in [bottom, top], 2048 bins of 2^shift keys at a time
             uint32_t klo = 0xffffffffu, khi = 0;
             auto tokens = [&](auto &&f) {
@@ -376,6 +422,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
                 top = up;
                 sync();  // (the result is written again)
             }
+            }
         }
         cluster_sync();
         const bool found = first.cut_found != 0;
@@ -421,6 +468,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         for (int c = 0; c < rank; c++) ties_before += (u64)cluster.map_shared_rank(&sh, c)->ties;
     }
     const double floor_w = (double)min_p * FIXED_ONE;
+    const float cut_x = cut_key > 0 ? of_key(cut_key) : -INFINITY;
     auto walk = [&](auto &&visit) {  // visit(i, kept weight) over this warp's run, 32 tokens at a time; false ends it
         u64 tie = ties_before;
         for (int i = i0; i < i1; i += 32) {
@@ -442,17 +490,39 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         }
     };
     u64 mine = 0, here;
-    walk([&](int, u64 w) { mine += w; return true; });
+    if (rank_ties) {
+        walk([&](int, u64 w) { mine += w; return true; });
+    } else {
+        // four tokens of a lane at a time: the weights' chain of 64-bit instructions is long
+        auto sum = [&](auto &&x4, int m) {
+            u64 w[4];
+#pragma unroll
+            for (int j = 0; j < m; j++) {
+                const uint32_t k = key_of(x4[j]);
+                w[j] = weight(x4[j]);
+                mine += k < cut_key || ((double)w[j] < floor_w && k != kmax) ? 0 : w[j];
+            }
+        };
+        int i = i0 + lane;
+        for (; i + 96 < i1; i += 128) {
+            const float x4[4] = {xs[i], xs[i + 32], xs[i + 64], xs[i + 96]};
+            if (x4[0] >= cut_x || x4[1] >= cut_x || x4[2] >= cut_x || x4[3] >= cut_x) sum(x4, 4);
+        }
+        for (; i < i1; i += 32) {
+            const float x4[4] = {xs[i]};
+            sum(x4, 1);
+        }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     u64 start = __shfl_sync(0xffffffffu, block_exclusive(lane == 0 ? mine : 0, sh.warp_sum, here), 0);
     if (tid == 0) sh.mass = here;
     cluster_sync();
-    u64 total = 0;
-    for (int c = 0; c < CS; c++) {
-        const u64 m = cluster.map_shared_rank(&sh, c)->mass;
-        if (c < rank) start += m;
-        total += m;
+    u64 total;
+    {
+        const u64 m = lane < CS ? cluster.map_shared_rank(&sh, lane)->mass : 0, incl = warp_inclusive(m);
+        start += __shfl_sync(0xffffffffu, incl - m, rank);
+        total = __shfl_sync(0xffffffffu, incl, 31);
     }
     cluster_sync();  // (no CTA leaves while another may read its shared memory)
     // first token whose cumulative weight exceeds the target

@@ -69,6 +69,23 @@ def test_ties_and_signed_zeros(ctx):
     assert int(got) == 0
 
 
+def test_many_equal_logits(ctx):
+    """Ten thousands of tokens that tie at the cut, and a bulk far narrower than the row's range."""
+    v = 60000
+    g = torch.Generator().manual_seed(7)
+    flat = torch.zeros(v)
+    flat[100] = 3.0
+    narrow = 5.0 + 1e-6 * torch.randn(v, generator=g)
+    narrow[::1000] = -20.0
+    coarse = torch.round(torch.randn(v, generator=g)).to(torch.float32)
+    rows, us, settings = [], [], []
+    for x in (flat, narrow, coarse):
+        for s in ((1.0, 5000, 1.0, 0.0), (1.0, 0, 0.7, 0.0), (0.3, 30000, 0.9, 0.0), (1.0, 2500, 0.5, 0.1), (20.0, 0, 0.5, 0.0)):
+            for u in (0.1, 0.77):
+                rows.append(x), us.append(u), settings.append(s)
+    check(ctx, torch.stack(rows).cuda(), torch.tensor(us).cuda(), settings)
+
+
 def test_infinities_nan_and_rows_of_nothing(ctx):
     v = 777
     g = torch.Generator().manual_seed(2)
