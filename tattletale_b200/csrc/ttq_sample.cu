@@ -51,7 +51,7 @@ struct Shared {
     uint32_t lo[BINS], hi[BINS];    // this CTA's histogram; the first CTA's becomes the row's
     u64 list_w[PAIRS + 1];          // and their counts or weights
     uint32_t list[LIST + 1];        // keys of the tokens that decide (first CTA)
-    double table[64];               // 2^(j / 64)
+    double table[512];              // 2^(j / 512)
     u64 warp_sum[SAMPLE_WARPS];
     // exchanged between the CTAs of a row
     u64 best, mass;
@@ -93,26 +93,28 @@ __device__ __forceinline__ void add_u64(uint32_t *lo, uint32_t *hi, u64 v) {
     if (h) atomicAdd(hi, h);
 }
 
-// exp((x - max) / T) in 2^-44 fixed point.  2^y with y = 64ths + r: a table and the series of 2^r to r^5 (|r| <= 1/128: 1e-17).
+// exp((x - max) / T) in 2^-44 fixed point.  2^y with y = 512ths + r: a table and the series of 2^r to r^3 (|r| <= 2^-10: 9e-15 of the
+// weight).  64-bit instructions are what the sampler spends its time on (a quarter of the 32-bit rate and less), so the
+// logit is widened by integer instructions and the range is checked in 32 bits: beyond -46 the weight is zero either way.
+constexpr int TABLE = 512;
 struct Weigher {
+    float xmax, scale32;
     double dmax, scale;  // log2(e) / T
     const double *table;
     __device__ __forceinline__ u64 operator()(float x) const {
-        const double d = ((double)x - dmax) * scale;
-        const bool live = d > -46.0;
-        const double y = live ? d : 0.0;
+        const uint32_t b = __float_as_uint(x);
+        const double xd = __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));  // (below 2^-126: below 2^-126)
+        const double y = (xd - dmax) * scale;
         constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low bits
-        const double kd = fma(y, 64.0, MAGIC);
+        const double kd = fma(y, (double)TABLE, MAGIC);
         const int k = __double2loint(kd);
-        const double r = fma(kd - MAGIC, -0.015625, y);
-        double p = fma(r, 1.3333558146428443e-3, 9.6181291076284772e-3);  // ln(2)^n / n!
-        p = fma(p, r, 5.5504108664821580e-2);
-        p = fma(p, r, 2.4022650695910072e-1);
+        const double r = fma(kd - MAGIC, -1.0 / TABLE, y);
+        double p = fma(r, 5.5504108664821580e-2, 2.4022650695910072e-1);  // ln(2)^n / n!
         p = fma(p, r, 6.9314718055994531e-1);
-        p = fma(p, r, 1.0) * table[k & 63];
-        const double v = __hiloint2double(__double2hiint(p) + (((k >> 6) + 44) << 20), __double2loint(p)) + 4503599627370496.0;  // + 2^52
+        p = fma(p, r, 1.0) * table[k & (TABLE - 1)];
+        const double v = __hiloint2double(__double2hiint(p) + (((k >> 9) + 44) << 20), __double2loint(p)) + 4503599627370496.0;  // + 2^52
         const u64 w = (u64)__double_as_longlong(v) & 0xfffffffffffffull;
-        return live ? w : (d == d ? 0 : (u64)FIXED_ONE);  // (NaN: infinity less itself)
+        return x == xmax ? (u64)FIXED_ONE : ((x - xmax) * scale32 > -46.f ? w : 0);
     }
 };
 
@@ -130,7 +132,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t row = blockIdx.x / CS;
     const int V = a.V, i_first = rank * a.slice, n = max(0, min(a.slice, V - i_first));
-    if (tid < 64) sh.table[tid] = exp2((double)tid * 0.015625);
+    static_assert(TABLE == SAMPLE_THREADS, "one entry per thread");
+    sh.table[tid] = exp2((double)tid / TABLE);
     for (int i = tid; i < BINS; i += SAMPLE_THREADS) sh.lo[i] = sh.hi[i] = 0;
     if (tid == 0) {
         sh.best = 0;
@@ -216,12 +219,14 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         cluster_sync();  // (no CTA leaves while another may read its shared memory)
         return;
     }
-    const Weigher weight{(double)xmax, 1.4426950408889634 / (double)temperature, sh.table};
+    const double scale = 1.4426950408889634 / (double)temperature;
+    const Weigher weight{xmax, (float)scale, (double)xmax, scale, sh.table};
 
     // Level 0: 2048 parts of the range from the largest logit down to the smallest, or to where weights vanish.  Monotone in x: a
     // difference, a product and a conversion, each rounded.  The last part also holds everything below.
-    const float clip = FIXED_RANGE * temperature, range = fminf(clip, xmax - of_key(kmin)), per_part = (float)BINS / range;
-    auto part_of = [&](float x) { return x == xmax ? 0 : (int)fminf((xmax - x) * per_part, (float)(BINS - 1)); };
+    const float clip = FIXED_RANGE * temperature, range = fminf(clip, xmax - of_key(kmin)), per_part = fminf((float)BINS / range, 3e38f);
+    auto place_of = [&](float x) { return x == xmax ? 0.f : (xmax - x) * per_part; };
+    auto part_of = [&](float x) { return (int)fminf(place_of(x), (float)(BINS - 1)); };
 
     // every token of this CTA: f(logit, key), four at a time
     auto each_token = [&](auto &&f) {
@@ -297,7 +302,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             if (part < 0 || (part == BINS - 1 && range == clip)) return false;
         }
         // the part's tokens to the first CTA
-        auto chosen = [&](float x, uint32_t k) { return k > lim && (part < 0 || part_of(x) == part); };
+        const float from = part < 0 ? -1.f : (float)part, to = part < 0 || part == BINS - 1 ? INFINITY : (float)(part + 1);
+        auto chosen = [&](float x, uint32_t k) {
+            const float at = place_of(x);
+            return k > lim && at >= from && !(at >= to && to < INFINITY);
+        };
         each_token([&](float x, uint32_t k) {
             if (chosen(x, k)) {
                 const int at = atomicAdd(&first.list_n, 1);
@@ -467,7 +476,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         cluster_sync();
         for (int c = 0; c < rank; c++) ties_before += (u64)cluster.map_shared_rank(&sh, c)->ties;
     }
-    const double floor_w = (double)min_p * FIXED_ONE;
+    const u64 floor_w = min_p > 0.f ? (u64)ceil(fmin((double)min_p, 2.0) * FIXED_ONE) : 0;
     const float cut_x = cut_key > 0 ? of_key(cut_key) : -INFINITY;
     auto walk = [&](auto &&visit) {  // visit(i, kept weight) over this warp's run, 32 tokens at a time; false ends it
         u64 tie = ties_before;
@@ -484,7 +493,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             u64 w = 0;
             if (__any_sync(0xffffffffu, keep)) {
                 if (keep) w = weight(x);
-                if ((double)w < floor_w && k != kmax) w = 0;
+                if (w < floor_w && k != kmax) w = 0;
             }
             if (!visit(i + lane, w)) break;
         }
@@ -500,7 +509,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
             for (int j = 0; j < m; j++) {
                 const uint32_t k = key_of(x4[j]);
                 w[j] = weight(x4[j]);
-                mine += k < cut_key || ((double)w[j] < floor_w && k != kmax) ? 0 : w[j];
+                mine += k < cut_key || (w[j] < floor_w && k != kmax) ? 0 : w[j];
             }
         };
         int i = i0 + lane;

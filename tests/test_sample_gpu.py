@@ -130,6 +130,15 @@ def test_one_setting_for_all_and_out(ctx):
     assert torch.equal(out.cpu(), expect(logits, u, [(0.8, 40, 0.9, 0.01)] * 9))
 
 
+@pytest.mark.parametrize("v", [3000, 20000])
+def test_a_row_per_multiprocessor(ctx, v):
+    """Batches large enough for one CTA per row, held in shared memory and not."""
+    g = torch.Generator().manual_seed(v)
+    m = 2 * torch.cuda.get_device_properties(0).multi_processor_count + 3
+    logits = (2.0 * torch.randn(m, v, generator=g)).cuda()
+    check(ctx, logits, torch.rand(m, generator=g).cuda(), [SETTINGS[r % len(SETTINGS)] for r in range(m)])
+
+
 def test_distribution(ctx):
     """Evenly spaced random numbers: every token comes up in proportion to its weight, to one draw."""
     n = 20000
