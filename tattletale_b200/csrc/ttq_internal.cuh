@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdlib>
 #include <stdint.h>
 
@@ -211,6 +212,22 @@ inline int device_sms() {
     }
     return cache[dev];
 }
+
+// A call per device of the process (kernel attributes belong to a device), half a microsecond of every launch otherwise.
+struct OncePerDevice {
+    std::atomic<bool> done[64] = {};
+    template <class F>
+    cudaError_t operator()(F &&f) {
+        int dev = 0;
+        const cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 0 || dev >= 64) return f();
+        if (done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+        const cudaError_t r = f();
+        if (r == cudaSuccess) done[dev].store(true, std::memory_order_release);
+        return r;
+    }
+};
 
 inline bool env_flag(const char *name, bool dflt) {
     const char *v = getenv(name);

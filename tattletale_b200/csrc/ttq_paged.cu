@@ -150,20 +150,22 @@ __global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __gr
 
 // ---- attention, tiles of 16 rows -------------------------------------------------------------------
 // Memory bound: 4 d flops per key, row and 2 bytes x 2 d of cache; 16 rows are 32 flops a byte, a hundred TFLOP/s at the
-// card's bandwidth, which m16n8k16 products reach with few warps.  A CTA of four warps takes units of 64 keys, each warp 16 of
-// them as a pipeline of its own: its lanes issue the tiled copies of 16 slots of one page into the warp's ring (128-byte
-// swizzle, read by ldmatrix without conflicts), wait for their own stage only and keep maximum, sum and output of the tile in
-// registers; the warps meet once per item.  Three 8 KB stages (d = 128) per warp, two CTAs per SM: 192 KB in flight per SM,
-// several times what the memory's latency asks for, which covers the table look-ups and item ends in between.
+// card's bandwidth, which m16n8k16 products reach with few warps.  A CTA of four warps takes units of 64 keys (d = 64: 128), each
+// warp 16 (32) of them as a pipeline of its own: its lanes issue the tiled copies of 16 slots of one page into the warp's ring
+// (128-byte swizzle, read by ldmatrix without conflicts), wait for their own stage only and keep maximum, sum and output of the
+// tile in registers; the warps meet once per item.  Three 8 KB stages per warp, two CTAs per SM: 192 KB in flight per SM,
+// several times what the memory's latency asks for, which covers the table look-ups and item ends in between.  A stage's
+// bookkeeping takes about as long as 4 KB do (23 windows of 4096 keys, d = 64: 55 us with stages of 16 keys).
 constexpr int ROWS_WARPS = 4;
 constexpr int ROWS_THREADS = ROWS_WARPS * 32;
-constexpr int ROWS_UNIT = 16 * ROWS_WARPS;
 constexpr int ROWS_TILE = 16;
 
 template <int D>
 struct RowsCfg {
-    static constexpr int STAGES = D == 128 ? 3 : 6;
-    static constexpr int TILE_BYTES = 16 * D * 2;          // 16 keys of K (or V)
+    static constexpr int STAGES = 3;
+    static constexpr int KT = 128 / D;                     // blocks of 16 keys in a warp's tile
+    static constexpr int KEYS = 16 * KT, UNIT = KEYS * ROWS_WARPS;
+    static constexpr int TILE_BYTES = KEYS * D * 2;        // a tile of K (or V)
     static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
     static constexpr int RING = ROWS_WARPS * STAGES * STAGE_BYTES;
     static constexpr int OPITCH = D + 4;                   // floats
@@ -206,22 +208,24 @@ struct RowsWalk {
     int b, item, items, unit;
 };
 __device__ __forceinline__ int rows_items(const PagedArgs &a, int n) { return a.hkv * ((n * a.G + ROWS_TILE - 1) / ROWS_TILE); }
+template <int U>
 __device__ __forceinline__ void rows_enter(const PagedArgs &a, RowsWalk &w, int min_pos) {
     const int nb = a.prefix_pass ? 1 : a.B;
     for (; w.b < nb; w.b++) {
         w.s = paged_seq(a, w.b, min_pos);
         if (w.s.n > 0) break;
     }
-    w.u = paged_units<ROWS_UNIT>(w.s);
+    w.u = paged_units<U>(w.s);
     w.items = rows_items(a, w.s.n);
     w.item = w.unit = 0;
 }
+template <int U>
 __device__ __forceinline__ void rows_next(const PagedArgs &a, RowsWalk &w, int min_pos, bool more) {
     if (++w.unit == w.u.count) {
         w.unit = 0;
         if (++w.item == w.items && more) {
             w.b++;
-            rows_enter(a, w, min_pos);
+            rows_enter<U>(a, w, min_pos);
         }
     }
 }
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                                                                                     const __grid_constant__ CUtensorMap kmap,
                                                                                     const __grid_constant__ CUtensorMap vmap) {
     using C = RowsCfg<D>;
-    constexpr int HALVES = D / 64;
+    constexpr int HALVES = D / 64, KT = C::KT, KEYS = C::KEYS, UNIT = C::UNIT;
     extern __shared__ uint8_t smem_raw[];
     __shared__ alignas(8) uint64_t full_s[ROWS_WARPS * C::STAGES];
     __shared__ int64_t red[ROWS_WARPS + 4];
@@ -253,13 +257,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     const PagedShare sh = paged_share<ROWS_THREADS, 1>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
         if (!ok) return 0;
         const PagedSeq s = paged_seq(a, b, min_pos);
-        return s.n > 0 ? (int64_t)rows_items(a, s.n) * paged_units<ROWS_UNIT>(s).count : 0;
+        return s.n > 0 ? (int64_t)rows_items(a, s.n) * paged_units<UNIT>(s).count : 0;
     });
     if (sh.u0 >= sh.u1) return;
 
     RowsWalk cw;  // the unit being computed
     cw.b = sh.b;
-    rows_enter(a, cw, sh.min_pos);
+    rows_enter<UNIT>(a, cw, sh.min_pos);
     {
         const int64_t off = sh.u0 - sh.seq_u;
         cw.item = (int)(off / cw.u.count);
@@ -268,45 +272,51 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     RowsWalk lw = cw;  // the unit whose copy is issued next
     int64_t lpos = sh.u0;
     int issued = 0, taken = 0;
-    int page_cache = 0, cache_first = -1, cache_b = -1;  // lane i: page of this warp's keys in unit cache_first + i of sequence cache_b
+    int page_cache[KT], cache_first = -1, cache_b = -1;  // lane i: pages of this warp's keys in unit cache_first + i of sequence cache_b
 
     const int base_pos = a.prefix_pass ? 0 : a.prefix_len;  // absolute position of key 0
-    auto wanted = [&](const RowsWalk &w, int k0) {
-        return k0 < w.s.key_end && (a.window == 0 || k0 + 15 >= w.s.lo || k0 < w.s.sink);
+    auto wanted = [&](const RowsWalk &w, int k0, int keys) {
+        return k0 < w.s.key_end && (a.window == 0 || k0 + keys > w.s.lo || k0 < w.s.sink);
     };
     auto fill = [&]() {
         while (lpos < sh.u1 && issued - taken < C::STAGES) {
-            const int k0 = paged_unit_index(lw.u, lw.unit) * ROWS_UNIT + 16 * warp;
-            if (wanted(lw, k0)) {
+            const int k0 = paged_unit_index(lw.u, lw.unit) * UNIT + KEYS * warp;
+            if (wanted(lw, k0, KEYS)) {
                 if (cache_b != lw.b || lw.unit < cache_first || lw.unit >= cache_first + 32) {
                     cache_b = lw.b;
                     cache_first = lw.unit;
-                    const int ku = lw.unit + lane < lw.u.count ? paged_unit_index(lw.u, lw.unit + lane) * ROWS_UNIT + 16 * warp : -1;
-                    page_cache = -1;
-                    if (ku >= 0 && wanted(lw, ku))
-                        page_cache = a.prefix_pass ? a.prefix_table[ku >> a.page_shift] : a.block_table[(int64_t)lw.b * a.ld_table + (ku >> a.page_shift)];
+                    const int ku = lw.unit + lane < lw.u.count ? paged_unit_index(lw.u, lw.unit + lane) * UNIT + KEYS * warp : -1;
+#pragma unroll
+                    for (int t = 0; t < KT; t++) {
+                        page_cache[t] = a.n_pages;  // zeros are read from beyond the last page
+                        if (ku >= 0 && wanted(lw, ku + 16 * t, 16)) {
+                            const int page = a.prefix_pass ? a.prefix_table[(ku + 16 * t) >> a.page_shift] : a.block_table[(int64_t)lw.b * a.ld_table + ((ku + 16 * t) >> a.page_shift)];
+                            if (page >= 0 && page < a.n_pages) page_cache[t] = page;
+                            else atomicOr(a.status, PAGED_BAD_INDEX);
+                        }
+                    }
                 }
-                int page = __shfl_sync(0xffffffffu, page_cache, lw.unit - cache_first);
-                if (page < 0 || page >= a.n_pages) {  // zeros are read from beyond the last page
-                    page = a.n_pages;
-                    if (lane == 0) atomicOr(a.status, PAGED_BAD_INDEX);
-                }
+                int page[KT];
+#pragma unroll
+                for (int t = 0; t < KT; t++) page[t] = __shfl_sync(0xffffffffu, page_cache[t], lw.unit - cache_first);
                 const int st = issued % C::STAGES;
                 const uint32_t dst = ring + (uint32_t)st * C::STAGE_BYTES, bar = bars + 8 * st;
                 if (elect_one()) {
                     mbar_expect_tx(bar, C::STAGE_BYTES);
-                    const int slot = k0 & ((1 << a.page_shift) - 1), head = lw.item % a.hkv;
+                    const int head = lw.item % a.hkv, mask = (1 << a.page_shift) - 1;
 #pragma unroll
-                    for (int h = 0; h < HALVES; h++) {
-                        tma_load_page(dst + h * 2048, &kmap, 64 * h, slot, head, page, bar);
-                        tma_load_page(dst + C::TILE_BYTES + h * 2048, &vmap, 64 * h, slot, head, page, bar);
-                    }
+                    for (int t = 0; t < KT; t++)
+#pragma unroll
+                        for (int h = 0; h < HALVES; h++) {
+                            tma_load_page(dst + t * 2048 + h * 2048, &kmap, 64 * h, (k0 + 16 * t) & mask, head, page[t], bar);
+                            tma_load_page(dst + C::TILE_BYTES + t * 2048 + h * 2048, &vmap, 64 * h, (k0 + 16 * t) & mask, head, page[t], bar);
+                        }
                 }
                 __syncwarp();
                 issued++;
             }
             lpos++;
-            rows_next(a, lw, sh.min_pos, lpos < sh.u1);
+            rows_next<UNIT>(a, lw, sh.min_pos, lpos < sh.u1);
         }
     };
     fill();
@@ -349,35 +359,38 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     int64_t seg_start = sh.u0;
 
     for (int64_t pos = sh.u0; pos < sh.u1; pos++) {
-        const int k0 = paged_unit_index(cw.u, cw.unit) * ROWS_UNIT + 16 * warp;
-        if (wanted(cw, k0)) {
+        const int k0 = paged_unit_index(cw.u, cw.unit) * UNIT + KEYS * warp;
+        if (wanted(cw, k0, KEYS)) {
             const int st = taken % C::STAGES;
             const uint32_t kt = ring + (uint32_t)st * C::STAGE_BYTES, vt = kt + C::TILE_BYTES;
             mbar_wait_bounded(bars + 8 * st, (taken / C::STAGES) & 1, a.status);
-            float s[2][4] = {};
-            {
+            float s[2 * KT][4] = {};
+#pragma unroll
+            for (int t = 0; t < KT; t++) {
                 const int r = (lane & 7) + ((lane >> 4) << 3), cc = (lane >> 3) & 1;
-                const uint32_t row = kt + r * 128;
+                const uint32_t row = kt + t * 2048 + r * 128;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ks++) {
                     uint32_t b[4];
                     const int c = 2 * ks + cc;
                     ldsm4(row + (c >> 3) * 2048 + (((c & 7) ^ (r & 7)) << 4), b);
-                    mma16816<BF16>(s[0], qf[ks], b[0], b[1]);
-                    mma16816<BF16>(s[1], qf[ks], b[2], b[3]);
+                    mma16816<BF16>(s[2 * t], qf[ks], b[0], b[1]);
+                    mma16816<BF16>(s[2 * t + 1], qf[ks], b[2], b[3]);
                 }
             }
             // visibility: whole tiles need no test
             const int j0 = k0 + base_pos;
-            const bool whole = j0 + 15 <= min_row && k0 + 15 < cw.s.key_end && (a.window == 0 || j0 > max_row - a.window || j0 + 15 < a.sinks);
-            uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
+            const bool whole = j0 + KEYS - 1 <= min_row && k0 + KEYS <= cw.s.key_end && (a.window == 0 || j0 > max_row - a.window || j0 + KEYS <= a.sinks);
+            uint32_t vm[2 * KT];
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+            for (int n = 0; n < 2 * KT; n++) {
+                vm[n] = 0xffffffffu;
 #pragma unroll
                 for (int i = 0; i < 4; i++) s[n][i] *= a.scale2;
+            }
             if (!whole) {
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
+                for (int n = 0; n < 2 * KT; n++) {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int k = k0 + 8 * n + 2 * t4 + e, j = k + base_pos;
@@ -388,11 +401,16 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                         if (!v1) s[n][2 + e] = -INFINITY;
                         // values that no row sees may be anything: zero them
                         const bool any = in && j <= max_row && (a.window == 0 || j > min_row - a.window || j < a.sinks);
-                        if (!any) (n == 0 ? vm0 : vm1) &= e == 0 ? 0xffff0000u : 0x0000ffffu;
+                        if (!any) vm[n] &= e == 0 ? 0xffff0000u : 0x0000ffffu;
                     }
                 }
             }
-            float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+            float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 2 * KT; n++) {
+                x0 = fmaxf(x0, fmaxf(s[n][0], s[n][1]));
+                x1 = fmaxf(x1, fmaxf(s[n][2], s[n][3]));
+            }
 #pragma unroll
             for (int d = 1; d < 4; d <<= 1) {
                 x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
@@ -414,23 +432,25 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             }
             const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
+            for (int n = 0; n < 2 * KT; n++) {
                 s[n][0] = ex2(s[n][0] - z0); s[n][1] = ex2(s[n][1] - z0);
                 s[n][2] = ex2(s[n][2] - z1); s[n][3] = ex2(s[n][3] - z1);
                 l0 += s[n][0] + s[n][1];
                 l1 += s[n][2] + s[n][3];
             }
-            const uint32_t p[4] = {pack2<BF16>(s[0][0], s[0][1]), pack2<BF16>(s[0][2], s[0][3]), pack2<BF16>(s[1][0], s[1][1]), pack2<BF16>(s[1][2], s[1][3])};
-            {
+#pragma unroll
+            for (int t = 0; t < KT; t++) {
+                const uint32_t p[4] = {pack2<BF16>(s[2 * t][0], s[2 * t][1]), pack2<BF16>(s[2 * t][2], s[2 * t][3]), pack2<BF16>(s[2 * t + 1][0], s[2 * t + 1][1]),
+                                       pack2<BF16>(s[2 * t + 1][2], s[2 * t + 1][3])};
                 const int r = (lane & 7) + (((lane >> 3) & 1) << 3), cc = lane >> 4;
-                const uint32_t row = vt + r * 128;
+                const uint32_t row = vt + t * 2048 + r * 128;
 #pragma unroll
                 for (int np = 0; np < D / 16; np++) {
                     uint32_t b[4];
                     const int c = 2 * np + cc;
                     ldsm4t(row + (c >> 3) * 2048 + (((c & 7) ^ (r & 7)) << 4), b);
-                    mma16816<BF16>(o[2 * np], p, b[0] & vm0, b[1] & vm1);
-                    mma16816<BF16>(o[2 * np + 1], p, b[2] & vm0, b[3] & vm1);
+                    mma16816<BF16>(o[2 * np], p, b[0] & vm[2 * t], b[1] & vm[2 * t + 1]);
+                    mma16816<BF16>(o[2 * np + 1], p, b[2] & vm[2 * t], b[3] & vm[2 * t + 1]);
                 }
             }
             taken++;
@@ -469,7 +489,17 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             joint(g, M0, x);
             joint(g + 8, M1, x);
             const float c0 = m0 == -INFINITY ? 0.f : ex2(m0 - M0), c1 = m1 == -INFINITY ? 0.f : ex2(m1 - M1);
-            // one after the other into one buffer: a second one would cost the second CTA of the SM
+            // At the share's end the warps' rings are free and take a result each; before, one after the other adds into one buffer (a
+            // second one would cost the second CTA of the SM).
+            if (pos + 1 == sh.u1) {
+                float *mine = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)));
+#pragma unroll
+                for (int n = 0; n < D / 8; n++) {
+                    *reinterpret_cast<float2 *>(mine + g * C::OPITCH + 8 * n + 2 * t4) = make_float2(o[n][0] * c0, o[n][1] * c0);
+                    *reinterpret_cast<float2 *>(mine + (g + 8) * C::OPITCH + 8 * n + 2 * t4) = make_float2(o[n][2] * c1, o[n][3] * c1);
+                }
+                __syncthreads();
+            } else {
 #pragma unroll
             for (int turn = 0; turn < ROWS_WARPS; turn++) {
                 if (warp == turn) {
@@ -488,6 +518,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                 }
                 __syncthreads();
             }
+            }
         }
         const int rows = min(ROWS_TILE, cw.s.n * a.G - cw.item / a.hkv * ROWS_TILE);
         const int own_slot = 2 * blockIdx.x + (seg_start == item_start ? 1 : 0);
@@ -496,10 +527,18 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             const int r = i / (D / 8), col = i % (D / 8) * 8;
             float m, l, v[8];
             joint(r, m, l);
-            const float4 *src = reinterpret_cast<const float4 *>(obuf + r * C::OPITCH + col);
-            const float4 y0 = src[0], y1 = src[1];
-            v[0] = y0.x; v[1] = y0.y; v[2] = y0.z; v[3] = y0.w;
-            v[4] = y1.x; v[5] = y1.y; v[6] = y1.z; v[7] = y1.w;
+            const bool apart = pos + 1 == sh.u1;
+#pragma unroll
+            for (int x = 0; x < 8; x++) v[x] = 0.f;
+#pragma unroll
+            for (int w = 0; w < ROWS_WARPS; w++)
+                if (w == 0 || apart) {
+                    const float *from = apart ? reinterpret_cast<const float *>(smem_raw + (ring_base - smem_u32(smem_raw)) + w * C::STAGES * C::STAGE_BYTES) : obuf;
+                    const float4 *src = reinterpret_cast<const float4 *>(from + r * C::OPITCH + col);
+                    const float4 y0 = src[0], y1 = src[1];
+                    v[0] += y0.x; v[1] += y0.y; v[2] += y0.z; v[3] += y0.w;
+                    v[4] += y1.x; v[5] += y1.y; v[6] += y1.z; v[7] += y1.w;
+                }
             if (complete) {
                 int token, head;
                 row_of(cw.item, cw.s, r, token, head);
@@ -535,7 +574,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
         }
         if (pos + 1 < sh.u1) {
             __syncthreads();  // obuf, ml_s and last_s are written again
-            rows_next(a, cw, sh.min_pos, true);
+            rows_next<UNIT>(a, cw, sh.min_pos, true);
             seg_start = pos + 1;
             begin();
         }
@@ -546,7 +585,8 @@ template <int D, bool BF16>
 cudaError_t launch_rows_t(const PagedArgs &a, const PagedMaps &maps, cudaStream_t st) {
     using C = RowsCfg<D>;
     auto kernel = paged_rows_kernel<D, BF16>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static OncePerDevice once;
+    const cudaError_t e = once([&]() { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM); });
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3((unsigned)(PAGED_ROWS16_CTAS * a.sms)), dim3(ROWS_THREADS), C::SMEM, st, a, maps.k, maps.v);
 }

@@ -490,15 +490,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     if (!joint) pair_arrive(TC_TURN_BAR + 2 * (warp & 3) + 1 - st);
                     l += sum;
                     tc_st_wait();
+                    // A parity tells a phase only from its neighbours, so the last product is waited for from the one before it, which is
+                    // waited for here, where the last one cannot be under way yet.
+                    if (h == 1 && i + step >= m && alive) alive = tc_wait(o_full + 8 * st, (halves - 1) & 1, a.status);
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(p_full + 8 * (2 * st + h));
                 }
             }
             // ---- results ----
-            // (the last two products in turn: a parity tells a phase only from its neighbours)
-            for (uint32_t x = 2; x > 0 && first < m; x--)
-                if (alive) alive = tc_wait(o_full + 8 * st, (halves - x) & 1, a.status);
+            if (first < m && alive) alive = tc_wait(o_full + 8 * st, (halves - 1) & 1, a.status);
             __syncwarp();
             tc_fence_after();
             const float m2 = mx == -INFINITY ? -INFINITY : mx * a.scale2;
@@ -856,7 +857,8 @@ cudaError_t launch_tc_t(const PagedArgs &a, const PagedMaps &maps, int box_rows,
     using C = TcCfg<D>;
     static_assert(C::SMEM <= 227 * 1024, "shared memory of a CTA");
     auto kernel = paged_tc_kernel<D, BF16>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static OncePerDevice once;
+    const cudaError_t e = once([&]() { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM); });
     if (e != cudaSuccess) return e;
     const cudaError_t r = launch_pdl(kernel, dim3((unsigned)a.sms), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, maps.q, box_rows);
     if (r != cudaSuccess) return r;

@@ -562,7 +562,10 @@ cudaError_t launch_sample(const void *logits, int dt, int64_t M, int V, int64_t 
     while (cluster < MAX_CLUSTER && ((int64_t)M * cluster * 2 <= 2 * (int64_t)sms || (V + cluster - 1) / cluster > 18432) && V / cluster > SAMPLE_THREADS) cluster *= 2;
     const int slice = (V + cluster - 1) / cluster;
     const size_t smem = sizeof(Shared) + (size_t)slice * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(Shared) + ((1 << 18) / MAX_CLUSTER) * sizeof(float)));
+    static OncePerDevice once;
+    const cudaError_t e = once([&]() {
+        return cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(Shared) + ((1 << 18) / MAX_CLUSTER) * sizeof(float)));
+    });
     if (e != cudaSuccess) return e;
     static const bool pdl = env_flag("TTQ_PDL", true);
     const SampleArgs a{logits, dt, V, slice, ld, s, u, ids};

@@ -14,9 +14,15 @@ from ._lib import KvPages, PagedBatchArgs, Sampling, TtqError, check
 from .layers import Context, _dt, _stream_ptr
 
 
+# The checks below are on the path of every call of a decode step: plain comparisons, no views and no temporary tensors.
+
+def _elsewhere(name: str) -> TtqError:
+    return TtqError(1, f"{name} must live on the context's CUDA device")
+
+
 def _on(ctx: Context, t: torch.Tensor, name: str) -> torch.Tensor:
-    if not t.is_cuda or t.device.index != (ctx.device.index or 0):
-        raise TtqError(1, f"{name} must live on the context's CUDA device")
+    if t.get_device() != (ctx.device.index or 0):
+        raise _elsewhere(name)
     return t
 
 
@@ -63,45 +69,54 @@ class PagedAttention:
     def __init__(self, ctx: Context, n_q_heads: int, n_kv_heads: int, head_dim: int, page_size: int, max_seqs: int, max_tokens: int,
                  dtype: torch.dtype = torch.bfloat16, max_prefix_tokens: Optional[int] = None):
         self.ctx, self.hq, self.hkv, self.d, self.page_size, self.dtype = ctx, n_q_heads, n_kv_heads, head_dim, page_size, dtype
+        self.device, self.scale = ctx.device.index or 0, 1.0 / math.sqrt(head_dim)
         h = ctypes.c_void_p()
         check(ctx.handle, ctx._lib.ttq_paged_create(ctx.handle, _dt(dtype), n_q_heads, n_kv_heads, head_dim, page_size, max_seqs, max_tokens,
                                                     max_tokens if max_prefix_tokens is None else max_prefix_tokens, ctypes.byref(h)))
         self.handle = h
 
     def _pages(self, k_pages: torch.Tensor, v_pages: torch.Tensor) -> KvPages:
-        want = (self.hkv, self.page_size, self.d)
-        if tuple(k_pages.shape[1:]) != want or v_pages.shape != k_pages.shape:
-            raise TtqError(2, f"pages must be [n_pages, {want[0]}, {want[1]}, {want[2]}], k and v alike")
+        shape, st = k_pages.shape, k_pages.stride()
+        if len(shape) != 4 or shape[1] != self.hkv or shape[2] != self.page_size or shape[3] != self.d or v_pages.shape != shape:
+            raise TtqError(2, f"pages must be [n_pages, {self.hkv}, {self.page_size}, {self.d}], k and v alike")
         if k_pages.dtype != self.dtype or v_pages.dtype != self.dtype:
             raise TtqError(1, f"pages must be {self.dtype}")
-        _on(self.ctx, k_pages, "k_pages"), _on(self.ctx, v_pages, "v_pages")
-        st = k_pages.stride()
+        if k_pages.get_device() != self.device or v_pages.get_device() != self.device:
+            raise _elsewhere("k_pages and v_pages")
         if st != v_pages.stride() or st[3] != 1:
             raise TtqError(2, "k and v pages must have the same strides and a contiguous head dimension")
-        return KvPages(k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], st[0], st[1], st[2])
+        return KvPages(k_pages.data_ptr(), v_pages.data_ptr(), shape[0], st[0], st[1], st[2])
 
-    def _rows(self, t: torch.Tensor, width: int, name: str) -> torch.Tensor:
-        t = t if t.dim() == 2 else t.flatten(1)
-        if t.shape[1] != width:
-            raise TtqError(2, f"{name} has {t.shape[1]} values a row, expected {width}")
+    def _rows(self, t: torch.Tensor, heads: int, name: str):
+        """``t`` as rows of ``heads`` x head_dim values: a tensor that owns them, their number and pitch."""
+        shape, width = t.shape, heads * self.d
+        if len(shape) == 3:
+            if shape[1] != heads or shape[2] != self.d:
+                raise TtqError(2, f"{name} is {tuple(shape)}, expected [rows, {heads}, {self.d}]")
+        elif len(shape) != 2 or shape[1] != width:
+            raise TtqError(2, f"{name} is {tuple(shape)}, expected [rows, {width}]")
         if t.dtype != self.dtype:
             raise TtqError(1, f"{name} must be {self.dtype}")
-        _on(self.ctx, t, name)
-        return t if t.stride(1) == 1 else t.contiguous()
+        if t.get_device() != self.device:
+            raise _elsewhere(name)
+        st = t.stride()
+        if st[-1] != 1 or (len(shape) == 3 and st[1] != self.d and heads > 1):
+            t = t.contiguous()
+            st = t.stride()
+        return t, shape[0], st[0] if shape[0] > 1 else width
 
-    def _out(self, out: Optional[torch.Tensor], like: torch.Tensor, name: str):
+    def _out(self, out: Optional[torch.Tensor], n: int, like: torch.Tensor, name: str):
         """The result tensor and its row pitch."""
-        n = like.shape[0]
+        width = self.hq * self.d
         if out is None:
-            out = torch.empty((n, self.hq, self.d), dtype=self.dtype, device=like.device)
-            return out, self.hq * self.d
+            return torch.empty((n, self.hq, self.d), dtype=self.dtype, device=like.device), width
         _on(self.ctx, out, name)
-        if out.dtype != self.dtype or out.numel() != n * self.hq * self.d or out.shape[0] != n:
+        if out.dtype != self.dtype or out.numel() != n * width or out.shape[0] != n:
             raise TtqError(2, f"{name} must be [{n}, {self.hq}, {self.d}] {self.dtype}")
         inner = out.stride()[1:]
         if inner != ((self.d, 1) if out.dim() == 3 else (1,)):
             raise TtqError(2, f"the rows of {name} must be contiguous")
-        return out, out.stride(0) if n > 1 else self.hq * self.d
+        return out, out.stride(0) if n > 1 else width
 
     def append(self, qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, batch: PagedBatch, cos: torch.Tensor, sin: torch.Tensor,
                q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -109,8 +124,7 @@ class PagedAttention:
         """Normalises (where weights ``[head_dim]`` are given) and rotates the q and k heads of fused qkv rows, writes k and v into the
         sequences' pages, returns q ``[n_tokens, n_q_heads, head_dim]``.  ``cos`` / ``sin``: ``[positions, head_dim]``, f32 or the
         plan's dtype."""
-        rows = self._rows(qkv, (self.hq + 2 * self.hkv) * self.d, "qkv")
-        n = rows.shape[0]
+        rows, n, ld = self._rows(qkv, self.hq + 2 * self.hkv, "qkv")
         if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != self.d or cos.dtype != sin.dtype:
             raise TtqError(2, f"cos and sin must be [positions, {self.d}], alike")
         cos, sin = _on(self.ctx, cos, "cos").contiguous(), _on(self.ctx, sin, "sin").contiguous()
@@ -119,10 +133,10 @@ class PagedAttention:
             if w is not None and (w.dtype != self.dtype or w.numel() != self.d or not w.is_contiguous()):
                 raise TtqError(2, f"{name} must be {self.d} contiguous values of {self.dtype}")
             norms.append(None if w is None else _on(self.ctx, w, name).data_ptr())
-        q_out, ld_q = self._out(q_out, rows, "q_out")
+        q_out, ld_q = self._out(q_out, n, rows, "q_out")
         ctx = self.ctx
-        st = ctx._lib.ttq_paged_append(ctx.handle, self.handle, self._pages(k_pages, v_pages), batch._for(n, self.page_size), rows.data_ptr(),
-                                       rows.stride(0) if n > 1 else rows.shape[1], norms[0], norms[1], eps, cos.data_ptr(), sin.data_ptr(),
+        st = ctx._lib.ttq_paged_append(ctx.handle, self.handle, self._pages(k_pages, v_pages), batch._for(n, self.page_size), rows.data_ptr(), ld,
+                                       norms[0], norms[1], eps, cos.data_ptr(), sin.data_ptr(),
                                        _dt(cos.dtype), cos.shape[0], q_out.data_ptr(), ld_q, _stream_ptr(rows.device))
         if st != 0:
             check(ctx.handle, st)
@@ -132,13 +146,11 @@ class PagedAttention:
                 scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of the batch's rows ``q`` ``[n_tokens, n_q_heads, head_dim]`` over their sequences' pages.  With ``window``
         a token sees the ``window`` latest positions (its own among them) and the first ``sinks`` of the sequence."""
-        rows = self._rows(q, self.hq * self.d, "q")
-        n = rows.shape[0]
-        out, ld_out = self._out(out, rows, "out")
+        rows, n, ld = self._rows(q, self.hq, "q")
+        out, ld_out = self._out(out, n, rows, "out")
         ctx = self.ctx
         st = ctx._lib.ttq_paged_attention(ctx.handle, self.handle, self._pages(k_pages, v_pages), batch._for(n, self.page_size), rows.data_ptr(),
-                                          rows.stride(0) if n > 1 else rows.shape[1], 1.0 / math.sqrt(self.d) if scale is None else scale, window, sinks,
-                                          out.data_ptr(), ld_out, _stream_ptr(rows.device))
+                                          ld, self.scale if scale is None else scale, window, sinks, out.data_ptr(), ld_out, _stream_ptr(rows.device))
         if st != 0:
             check(ctx.handle, st)
         return out

@@ -207,6 +207,7 @@ def test_captured_call_follows_the_lengths(ctx, new):
         for out in outs:
             check_attention(out, shorter)
     assert torch.equal(outs[0], outs[1])
+    ctx.check_device_status()
     del graphs
 
 
