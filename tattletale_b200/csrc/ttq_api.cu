@@ -1661,6 +1661,9 @@ ttq_status paged_args(ttq_ctx *ctx, const ttq_paged *p, const ttq_kv_pages *kv, 
     a->hq = p->hq;
     a->hkv = p->hkv;
     a->G = p->hq / p->hkv;
+    a->tokens = a->G <= 128 ? 128 / a->G : 1;
+    a->inv_tokens2 = 1.f / (float)(2 * a->tokens);
+    a->inv_G = 1.f / (float)a->G;
     a->page_shift = p->page_shift;
     a->n_pages = (int)kv->n_pages;
     a->status = ctx->dev_status;

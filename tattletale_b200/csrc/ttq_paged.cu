@@ -201,13 +201,13 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     }
 }
 
-// Walk through the units of consecutive sequences.
+// Walk through the units of consecutive sequences: row tiles, kv heads, units.
 struct RowsWalk {
     PagedSeq s;
     PagedUnits u;
-    int b, item, items, unit;
+    int b, rt, head, unit;
 };
-__device__ __forceinline__ int rows_items(const PagedArgs &a, int n) { return a.hkv * ((n * a.G + ROWS_TILE - 1) / ROWS_TILE); }
+__device__ __forceinline__ int rows_tiles(const PagedArgs &a, int n) { return (n * a.G + ROWS_TILE - 1) / ROWS_TILE; }
 template <int U>
 __device__ __forceinline__ void rows_enter(const PagedArgs &a, RowsWalk &w, int min_pos) {
     const int nb = a.prefix_pass ? 1 : a.B;
@@ -216,16 +216,18 @@ __device__ __forceinline__ void rows_enter(const PagedArgs &a, RowsWalk &w, int 
         if (w.s.n > 0) break;
     }
     w.u = paged_units<U>(w.s);
-    w.items = rows_items(a, w.s.n);
-    w.item = w.unit = 0;
+    w.rt = w.head = w.unit = 0;
 }
 template <int U>
 __device__ __forceinline__ void rows_next(const PagedArgs &a, RowsWalk &w, int min_pos, bool more) {
     if (++w.unit == w.u.count) {
         w.unit = 0;
-        if (++w.item == w.items && more) {
-            w.b++;
-            rows_enter<U>(a, w, min_pos);
+        if (++w.head == a.hkv) {
+            w.head = 0;
+            if (++w.rt == rows_tiles(a, w.s.n) && more) {
+                w.b++;
+                rows_enter<U>(a, w, min_pos);
+            }
         }
     }
 }
@@ -246,6 +248,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     float *obuf = reinterpret_cast<float *>(smem_raw + (ring_base - smem_u32(smem_raw)) + C::RING);
     const uint32_t ring = ring_base + (uint32_t)warp * C::STAGES * C::STAGE_BYTES;
     const uint32_t bars = smem_u32(full_s) + (uint32_t)warp * C::STAGES * 8;
+    if (tid == 0) {
+        tma_prefetch(&kmap);
+        tma_prefetch(&vmap);
+    }
     if (lane == 0) {
         for (int i = 0; i < C::STAGES; i++) mbar_init(bars + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -257,7 +263,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     const PagedShare sh = paged_share<ROWS_THREADS, 1>(a, red, [&](int b, bool ok, int min_pos) -> int64_t {
         if (!ok) return 0;
         const PagedSeq s = paged_seq(a, b, min_pos);
-        return s.n > 0 ? (int64_t)rows_items(a, s.n) * paged_units<UNIT>(s).count : 0;
+        return s.n > 0 ? (int64_t)a.hkv * rows_tiles(a, s.n) * paged_units<UNIT>(s).count : 0;
     });
     if (sh.u0 >= sh.u1) return;
 
@@ -266,8 +272,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     rows_enter<UNIT>(a, cw, sh.min_pos);
     {
         const int64_t off = sh.u0 - sh.seq_u;
-        cw.item = (int)(off / cw.u.count);
-        cw.unit = (int)(off % cw.u.count);
+        const int item = (int)paged_div(off, cw.u.count);
+        cw.unit = (int)(off - (int64_t)item * cw.u.count);
+        cw.rt = item / a.hkv;
+        cw.head = item - cw.rt * a.hkv;
     }
     RowsWalk lw = cw;  // the unit whose copy is issued next
     int64_t lpos = sh.u0;
@@ -303,7 +311,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                 const uint32_t dst = ring + (uint32_t)st * C::STAGE_BYTES, bar = bars + 8 * st;
                 if (elect_one()) {
                     mbar_expect_tx(bar, C::STAGE_BYTES);
-                    const int head = lw.item % a.hkv, mask = (1 << a.page_shift) - 1;
+                    const int head = lw.head, mask = (1 << a.page_shift) - 1;
 #pragma unroll
                     for (int t = 0; t < KT; t++)
 #pragma unroll
@@ -325,17 +333,17 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     uint32_t qf[D / 16][4];
     float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     int pos0 = 0, pos1 = 0, min_row = 0, max_row = 0;
-    auto row_of = [&](int item, const PagedSeq &s, int r, int &token, int &head) {
-        const int x = item / a.hkv * ROWS_TILE + r, i = x / a.G;
-        token = s.q0 + i;
-        head = item % a.hkv * a.G + (x - i * a.G);
-        return i < s.n;
+    auto row_of = [&](int r, int &token, int &head) {
+        const int x = cw.rt * ROWS_TILE + r, i = paged_div(x, a.G, a.inv_G);
+        token = cw.s.q0 + i;
+        head = cw.head * a.G + (x - i * a.G);
+        return i < cw.s.n;
     };
     auto begin = [&]() {
 #pragma unroll
         for (int r = 0; r < 2; r++) {
             int token, head;
-            const bool ok = row_of(cw.item, cw.s, g + 8 * r, token, head);
+            const bool ok = row_of(g + 8 * r, token, head);
             int pos = -1;
             if (ok) pos = a.prefix_pass ? paged_row_pos(a, token) : cw.s.pos0 + token - cw.s.q0;
             const uint32_t *src = reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint16_t *>(a.q) + (ok ? (int64_t)token * a.ld_q + (int64_t)head * D : 0)) + t4;
@@ -520,7 +528,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             }
             }
         }
-        const int rows = min(ROWS_TILE, cw.s.n * a.G - cw.item / a.hkv * ROWS_TILE);
+        const int rows = min(ROWS_TILE, cw.s.n * a.G - cw.rt * ROWS_TILE);
         const int own_slot = 2 * blockIdx.x + (seg_start == item_start ? 1 : 0);
         float *part = a.part + (int64_t)own_slot * ROWS_TILE * (D + 2);
         for (int i = tid; i < rows * (D / 8); i += ROWS_THREADS) {
@@ -541,7 +549,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                 }
             if (complete) {
                 int token, head;
-                row_of(cw.item, cw.s, r, token, head);
+                row_of(r, token, head);
                 paged_finish8<BF16>(a, D, token, head, col, m, l, v);
             } else {
                 float4 *d = reinterpret_cast<float4 *>(part + r * D + col);
@@ -567,7 +575,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                     float m, l, v[8];
                     paged_gather8<ROWS_TILE>(a, D, c0, c1, r, col, m, l, v);
                     int token, head;
-                    row_of(cw.item, cw.s, r, token, head);
+                    row_of(r, token, head);
                     paged_finish8<BF16>(a, D, token, head, col, m, l, v);
                 }
             }

@@ -32,6 +32,8 @@ struct PagedArgs {
     const int *prefix_table;
     int prefix_pass;            // 1: all rows of the batch against the shared prefix's keys, results to pre_o / pre_lse
     int hq, hkv, G, page_shift, n_pages;
+    int tokens;                 // tensor-memory kernel: tokens of a stream, 128 / G
+    float inv_tokens2, inv_G;   // 1 / (2 tokens), 1 / G
     int window, sinks;          // window 0: none
     float scale2;               // scale * log2(e): scores and maxima are kept in units of log2
     float *pre_o, *pre_lse;     // [n_tokens][hq][d] normalised, [n_tokens][hq]; read by the other pass (nullptr: no prefix)
@@ -118,8 +120,21 @@ __device__ __forceinline__ int paged_row_pos(const PagedArgs &a, int token) {
     return a.kv_len[lo] - (a.q_start[lo + 1] - token);
 }
 
-// Owner among N shares [total * c / N, total * (c + 1) / N) of number u.
-__device__ __forceinline__ int paged_owner(int64_t u, int64_t total, int N) { return (int)(((u + 1) * N - 1) / total); }
+// Quotients.  The compiler's 64-bit division is several hundred clocks of a warp's time, its 32-bit one a hundred and more, and a CTA
+// stands behind a dozen of them before its first copy.
+__device__ __forceinline__ int64_t paged_div(int64_t x, int64_t d) {
+    return ((uint64_t)x | (uint64_t)d) >> 32 ? x / d : (int64_t)((uint32_t)x / (uint32_t)d);
+}
+__device__ __forceinline__ int paged_div(int x, int d, float inv) {  // x >= 0
+    if (x >= 1 << 22) return x / d;
+    const int q = (int)((float)x * inv), r = x - q * d;  // (the product is off by less than one)
+    return q + (r >= d ? 1 : 0) - (r < 0 ? 1 : 0);
+}
+// Shares of `total` numbers for N owners: the first `total % N` have one more than the others.  Owner of number u:
+__device__ __forceinline__ int paged_owner(int64_t u, int64_t total, int N) {
+    const int64_t size = paged_div(total, N), longer = total - size * N, edge = longer * (size + 1);
+    return (int)(u < edge ? paged_div(u, size + 1) : longer + paged_div(u - edge, size));
+}
 
 // What one CTA finds out before it starts.
 struct PagedShare {
@@ -131,7 +146,7 @@ struct PagedShare {
     int min_pos;     // prefix pass: smallest position of any token
 };
 
-// Shares of at least MIN_SHARE numbers each, at most one per CTA.
+// Number of shares: of at least MIN_SHARE numbers each, at most one per CTA.
 template <int MIN_SHARE>
 __device__ __forceinline__ int paged_shares(int64_t total) {
     const int64_t most = total / MIN_SHARE;
@@ -159,7 +174,16 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
         sh.min_pos = mp;
     }
     // total, then the sequence that holds the share's first unit (one pass over the lengths when they fit one chunk)
-    int64_t total = 0, u0 = 0;
+    int64_t total = 0, u0 = 0, u1 = 0;
+    auto bounds = [&]() {
+        sh.N = paged_shares<MIN_SHARE>(total);
+        u0 = u1 = total;
+        if ((int)blockIdx.x < sh.N) {
+            const int64_t size = paged_div(total, sh.N), longer = total - size * sh.N, c = blockIdx.x;
+            u0 = c * size + (c < longer ? c : longer);
+            u1 = u0 + size + (c < longer ? 1 : 0);
+        }
+    };
     for (int pass = 0; pass < 2; pass++) {
         int64_t running = 0;
         for (int base = 0; base < nb; base += THREADS) {
@@ -180,8 +204,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
             }
             if (nb <= THREADS) {
                 total = chunk;
-                sh.N = paged_shares<MIN_SHARE>(total);
-                u0 = (int)blockIdx.x < sh.N ? total * blockIdx.x / sh.N : total;
+                bounds();
                 pass = 1;
             }
             const int64_t at = before + incl - c;
@@ -194,13 +217,12 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
         }
         if (pass == 0) {
             total = running;
-            sh.N = paged_shares<MIN_SHARE>(total);
-            u0 = (int)blockIdx.x < sh.N ? total * blockIdx.x / sh.N : total;
+            bounds();
         }
     }
     sh.total = total;
     sh.u0 = u0;
-    sh.u1 = (int)blockIdx.x < sh.N ? total * (blockIdx.x + 1) / sh.N : u0;
+    sh.u1 = u1;
     sh.b = sh.u1 > sh.u0 ? (int)red[W] : 0;
     sh.seq_u = sh.u1 > sh.u0 ? red[W + 1] : 0;
     __syncthreads();
@@ -277,6 +299,7 @@ __device__ __forceinline__ void paged_gather8(const PagedArgs &a, int D, int c0,
 }
 
 // Four-dimensional tiled copies of the pages: (element of the head, slot, kv head, page).
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *map, int x, int slot, int head, int page, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),

@@ -53,7 +53,7 @@ constexpr int TC_SEGS = 4, TC_SEG_READERS = 11;  // (8 softmax warps, copies, tw
 struct TcSplit {
     int c1, rows, tok0, n, q0, head;
 };
-__device__ __forceinline__ int tc_tokens(const PagedArgs &a) { return TC_ROWS / a.G; }  // of a stream
+__device__ __forceinline__ int tc_tokens(const PagedArgs &a) { return a.tokens; }  // of a stream
 
 template <int D>
 struct TcCfg {
@@ -191,11 +191,11 @@ struct TcItem {
     PagedSeq k;      // key_end, lo, sink of this item (the rest as the sequence's)
     PagedUnits u;
     int tok0, tokens;
-    int weight, size;   // numbers of a unit and of the whole item
-    // units whose number is below p; unit i stands at TC_ITEM_WEIGHT + i * weight
-    __device__ __forceinline__ int units_before(int p) const { return max(0, min(u.count, (p - TC_ITEM_WEIGHT + weight - 1) / weight)); }
+    int shift, size;    // a unit has 1 << shift numbers; numbers of the whole item
+    // units whose number is below p; unit i stands at TC_ITEM_WEIGHT + (i << shift)
+    __device__ __forceinline__ int units_before(int p) const { return max(0, min(u.count, (p - TC_ITEM_WEIGHT + (1 << shift) - 1) >> shift)); }
 };
-__device__ __forceinline__ int tc_tiles(const PagedArgs &a, int n) { return (n + 2 * tc_tokens(a) - 1) / (2 * tc_tokens(a)); }
+__device__ __forceinline__ int tc_tiles(const PagedArgs &a, int n) { return paged_div(n + 2 * tc_tokens(a) - 1, 2 * tc_tokens(a), a.inv_tokens2); }
 __device__ __forceinline__ TcItem tc_item(const PagedArgs &a, const PagedSeq &s, int rt) {
     TcItem it;
     it.k = s;
@@ -210,8 +210,8 @@ __device__ __forceinline__ TcItem tc_item(const PagedArgs &a, const PagedSeq &s,
         }
     }
     it.u = paged_units<TC_UNIT>(it.k);
-    it.weight = it.tokens > tc_tokens(a) ? TC_PAIR_WEIGHT : 1;
-    it.size = TC_ITEM_WEIGHT + it.u.count * it.weight;
+    it.shift = it.tokens > tc_tokens(a) ? 1 : 0;
+    it.size = TC_ITEM_WEIGHT + (it.u.count << it.shift);
     return it;
 }
 // Numbers of one kv head's items of a sequence, by the whole warp (`s`: the same in all lanes).
@@ -248,7 +248,7 @@ struct TcWalk {
         enter(a, sh.min_pos);
         int64_t off = sh.u0 - sh.seq_u;
         const int64_t per_head = tc_seq_units(a, s, lane);
-        head = (int)(off / per_head);
+        head = (int)paged_div(off, per_head);
         off -= head * per_head;
         for (int base = 0;; base += 32) {
             const int c = base + lane < nt ? tc_item(a, s, base + lane).size : 0;
@@ -314,6 +314,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
     volatile uint32_t *slot_word = reinterpret_cast<volatile uint32_t *>(smem + C::MISC_AT + 16 * 8);
     TcSplit *splits = reinterpret_cast<TcSplit *>(a.counters);
     if (tid == 0) {
+        tma_prefetch(&kmap);
+        tma_prefetch(&vmap);
+        tma_prefetch(&qmap);
         for (int i = 0; i < C::SLOTS; i++) {
             mbar_init(kv_full + 8 * i, 1);
             mbar_init(kv_empty + 8 * i, 2);  // one arrival per stream, two of the only one that takes the slot
@@ -810,7 +813,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     g.slot = 2 * (int)blockIdx.x + (first == 0 ? 1 : 0);
                     // an item that begins here and goes on elsewhere is the share's last
                     if (first == 0 && !g.complete)
-                        splits[blockIdx.x] = {paged_owner(w.pos - w.at + TC_ITEM_WEIGHT + (int64_t)(w.it.u.count - 1) * w.it.weight, sh.total, sh.N),
+                        splits[blockIdx.x] = {paged_owner(w.pos - w.at + TC_ITEM_WEIGHT + ((int64_t)(w.it.u.count - 1) << w.it.shift), sh.total, sh.N),
                                               g.pair ? TC_ITEM_ROWS : TC_ROWS, g.tok0, g.n, g.q0, g.head};
                 }
                 segs[k % TC_SEGS] = g;
@@ -845,7 +848,7 @@ __global__ void __launch_bounds__(TC_JOIN_THREADS) paged_tc_join_kernel(const __
     const TcSplit sp = reinterpret_cast<const TcSplit *>(a.counters)[c0];
     const int i = blockIdx.y * TC_JOIN_THREADS + threadIdx.x, r = i / (D / 8), col = i % (D / 8) * 8;
     if (r >= sp.rows) return;
-    const int rr = r % TC_ROWS, t = rr / a.G, tok = sp.tok0 + r / TC_ROWS * tc_tokens(a) + t;
+    const int rr = r % TC_ROWS, t = paged_div(rr, a.G, a.inv_G), tok = sp.tok0 + r / TC_ROWS * tc_tokens(a) + t;
     if (t >= tc_tokens(a) || tok >= sp.n) return;
     float m, l, v[8];
     paged_gather8<TC_ITEM_ROWS>(a, D, c0, sp.c1, r, col, m, l, v);
