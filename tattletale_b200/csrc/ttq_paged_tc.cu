@@ -247,9 +247,16 @@ struct TcWalk {
         b = sh.b;
         enter(a, sh.min_pos);
         int64_t off = sh.u0 - sh.seq_u;
+        pos = sh.u0;
+        if (nt == 1) {
+            head = (int)paged_div(off, it.size);
+            at = (int)(off - (int64_t)head * it.size);
+            return;
+        }
         const int64_t per_head = tc_seq_units(a, s, lane);
         head = (int)paged_div(off, per_head);
         off -= head * per_head;
+#pragma unroll 1
         for (int base = 0;; base += 32) {
             const int c = base + lane < nt ? tc_item(a, s, base + lane).size : 0;
             int incl = c;
@@ -269,7 +276,6 @@ struct TcWalk {
             off -= __shfl_sync(0xffffffffu, incl, 31);
         }
         it = tc_item(a, s, rt);
-        pos = sh.u0;
     }
     // numbers of this item in the share
     __device__ __forceinline__ int here(const PagedShare &sh) const {
@@ -620,25 +626,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         // meet them.  One warp's instruction latency bounds this loop, so what can be shared between K and V is.
         int cache_first = -1, cache_b = -1, page_cache = 0;  // lane i: page number cache_first + i of the table of sequence cache_b
         const int boxes = TC_UNIT / box_rows, box_bytes = box_rows * 128;
-        auto issue = [&](const CUtensorMap &map, uint32_t wanted, uint32_t bar, const int (&page)[8], int slot0, int head) {
-            const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES;
-            if (elect_one()) {
-                if (wanted) mbar_expect_tx(bar, (uint32_t)(__popc(wanted) * box_bytes * C::HALVES));
-                else mbar_arrive(bar);
-#pragma unroll
-                for (int r = 0; r < 8; r++)
-                    if (wanted >> r & 1u) {
-#pragma unroll
-                        for (int h = 0; h < C::HALVES; h++)
-                            tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + r * box_bytes), &map, 64 * h, (slot0 + r * box_rows) & page_mask, head, page[r], bar);
-                    }
-            }
-            __syncwarp();
-        };
-        auto wait_empty = [&]() {
-            if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
-            __syncwarp();
-        };
         for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
             const int m = g.m, u0 = g.unit, u_sink = g.u_sink, u_first = g.u_first, key_end = g.key_end, lo = g.lo, sink = g.sink, head = g.head, seq = g.b;
@@ -663,32 +650,56 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
                 const int mine = __shfl_sync(0xffffffffu, page_cache, (idx - cache_first + lane) & 31);
                 const uint32_t seen = __ballot_sync(0xffffffffu, lane < boxes && visible(k0 + lane * box_rows, box_rows));
-                int page[8];
-#pragma unroll
-                for (int r = 0; r < 8; r++) page[r] = __shfl_sync(0xffffffffu, seen >> lane & 1u ? mine : a.n_pages, r);
-                wait_empty();
-                issue(kmap, seen, kv_full + 8 * (n % C::SLOTS), page, k0, head);
-                n++;
-                const bool fix = k0 + TC_UNIT > key_end || (k0 < lo && k0 + TC_UNIT > sink);
-                const uint32_t full = kv_full + 8 * (n % C::SLOTS);
-                wait_empty();
-                issue(vmap, (1u << boxes) - 1u, fix ? fix_bar : full, page, k0, head);
-                if (fix) {
-                    const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES;
-                    if (alive) alive = tc_wait(fix_bar, fix_par, a.status);
-                    fix_par ^= 1u;
-                    for (int r = lane / 8; r < TC_UNIT; r += 4) {
-                        const int key = k0 + r;
-                        if (key >= key_end || (key < lo && key >= sink)) {
-#pragma unroll
-                            for (int h = 0; h < C::HALVES; h++) sts128<0>(slot + (uint32_t)(h * C::HALF_BYTES + r * 128 + (lane & 7) * 16), 0u, 0u, 0u, 0u);
-                        }
-                    }
-                    fence_async_shared();
+                const int page = seen >> lane & 1u ? mine : a.n_pages;
+                const bool edge = k0 + TC_UNIT > key_end || (k0 < lo && k0 + TC_UNIT > sink);
+                // (four boxes at a time: a launch begins with cold instruction caches, and all sixteen copies unrolled took 10000 clocks for the
+                // first unit; one by one, pages of 16 slots keep the products waiting)
+#pragma unroll 1
+                for (int kv = 0; kv < 2; kv++, n++) {
+                    const uint32_t slot = base + C::RING_AT + (uint32_t)(n % C::SLOTS) * C::SLOT_BYTES, full = kv_full + 8 * (n % C::SLOTS);
+                    const uint32_t wanted = kv == 0 ? seen : (1u << boxes) - 1u;
+                    const bool fix = kv == 1 && edge;
+                    const uint32_t bar = fix ? fix_bar : full;
+                    const CUtensorMap *map = kv == 0 ? &kmap : &vmap;
+                    if (n >= C::SLOTS && alive) alive = tc_wait(kv_empty + 8 * (n % C::SLOTS), (uint32_t)((n / C::SLOTS - 1) & 1), a.status);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(full);
+                    if (elect_one()) {
+                        if (wanted) mbar_expect_tx(bar, (uint32_t)(__popc(wanted) * box_bytes * C::HALVES));
+                        else mbar_arrive(bar);
+                    }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int r0 = 0; r0 < boxes; r0 += 4) {
+                        int pg[4];
+#pragma unroll
+                        for (int r = 0; r < 4; r++) pg[r] = __shfl_sync(0xffffffffu, page, r0 + r);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                if (wanted >> (r0 + r) & 1u) {
+#pragma unroll
+                                    for (int h = 0; h < C::HALVES; h++)
+                                        tma_load_page(slot + (uint32_t)(h * C::HALF_BYTES + (r0 + r) * box_bytes), map, 64 * h, (k0 + (r0 + r) * box_rows) & page_mask, head,
+                                                      pg[r], bar);
+                                }
+                        }
+                        __syncwarp();
+                    }
+                    if (fix) {
+                        if (alive) alive = tc_wait(fix_bar, fix_par, a.status);
+                        fix_par ^= 1u;
+                        for (int r = lane / 8; r < TC_UNIT; r += 4) {
+                            const int key = k0 + r;
+                            if (key >= key_end || (key < lo && key >= sink)) {
+#pragma unroll
+                                for (int h = 0; h < C::HALVES; h++) sts128<0>(slot + (uint32_t)(h * C::HALF_BYTES + r * 128 + (lane & 7) * 16), 0u, 0u, 0u, 0u);
+                            }
+                        }
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(full);
+                    }
                 }
-                n++;
             }
         }
         // the last copies have landed before the CTA may end: the product warp waits for every slot
@@ -774,7 +785,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         bool alive = true;
         int used[2] = {0, 0};
         const uint32_t bytes = (uint32_t)(tc_tokens(a) * a.G * 128 * C::HALVES);
-        // Queries of item k, once the scores of the last item are complete.  A stream without a unit gets none.
+        // Queries of item k, once the scores of the last item are complete (the record of the one after it comes in time for the copies of
+        // its pages: with the scores of this one still to be made).  A stream without a unit gets none.
         auto queries = [&](int k) {
             const TcSeg &g = segs[k % TC_SEGS];
             for (int st = 0; st < (g.m == 0 ? 0 : (g.pair || g.m > 1 ? 2 : 1)); st++) {
@@ -811,19 +823,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     g.b = w.b; g.head = w.head; g.q0 = w.s.q0; g.pos0 = w.s.pos0;
                     g.complete = units == w.it.u.count;
                     g.slot = 2 * (int)blockIdx.x + (first == 0 ? 1 : 0);
-                    // an item that begins here and goes on elsewhere is the share's last
-                    if (first == 0 && !g.complete)
-                        splits[blockIdx.x] = {paged_owner(w.pos - w.at + TC_ITEM_WEIGHT + ((int64_t)(w.it.u.count - 1) << w.it.shift), sh.total, sh.N),
-                                              g.pair ? TC_ITEM_ROWS : TC_ROWS, g.tok0, g.n, g.q0, g.head};
                 }
                 segs[k % TC_SEGS] = g;
                 mbar_arrive(seg_full + 8 * (k % TC_SEGS));
             }
             __syncwarp();
-            // the queries of the item before, one record behind (the ring keeps a record until the last reader is done with it, and the
-            // products of an item wait for its queries)
-            if (k > 0) queries(k - 1);
             if (end) break;
+            queries(k);
+            // an item that begins here and goes on elsewhere is the share's last
+            if (lane == 0 && first == 0 && units < w.it.u.count)
+                splits[blockIdx.x] = {paged_owner(w.pos - w.at + TC_ITEM_WEIGHT + ((int64_t)(w.it.u.count - 1) << w.it.shift), sh.total, sh.N),
+                                      w.it.tokens > tc_tokens(a) ? TC_ITEM_ROWS : TC_ROWS, w.it.tok0, w.s.n, w.s.q0, w.head};
             w.next(a, sh);
             k++;
         }
