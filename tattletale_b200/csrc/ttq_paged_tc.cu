@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                         float x, y;
                         f2_split(add2(sums[0], sums[1]), x, y);
                         sum = x + y;
-                        redo = !(sum <= 32768.f);
+                        redo = valid && !(sum <= 32768.f);  // (rows of no token hold anything)
                         if (turn > 0 || !__any_sync(0xffffffffu, redo)) break;
                     }
                     if (!joint) pair_arrive(TC_TURN_BAR + 2 * (warp & 3) + 1 - st);
@@ -849,19 +849,61 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
 // Joins the parts of the items that share borders have cut: CTA (c, y) takes 256 groups of eight results of the item that begins in
 // share c, one thread each.  A launch of its own, since a single CTA reads the parts of a widely cut item (two hundred rows against a
 // long prefix: 2 MB) at a hundred GB/s: 95 us of 187 us when the last CTA to arrive did it (48 decode rows, prefix of 12345).
-constexpr int TC_JOIN_THREADS = 256;
+constexpr int TC_JOIN_THREADS = 256, TC_JOIN_PARTS = 160;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(TC_JOIN_THREADS) paged_tc_join_kernel(const __grid_constant__ PagedArgs a) {
     grid_launch_dependents();
     grid_dependency_wait();
+    constexpr int PER_ROW = D / 8, ROWS = TC_JOIN_THREADS / PER_ROW;
+    __shared__ float2 w_s[TC_JOIN_PARTS][ROWS];  // a part's weight for a row, and its weighted sum
     const int c0 = blockIdx.x;
     const TcSplit sp = reinterpret_cast<const TcSplit *>(a.counters)[c0];
-    const int i = blockIdx.y * TC_JOIN_THREADS + threadIdx.x, r = i / (D / 8), col = i % (D / 8) * 8;
-    if (r >= sp.rows) return;
+    const int first_row = blockIdx.y * ROWS, lr = threadIdx.x / PER_ROW, r = first_row + lr, lane = threadIdx.x % PER_ROW, col = lane * 8;
+    if (first_row >= sp.rows) return;
+    const int parts = sp.c1 - c0 + 1;
+    const int64_t pitch = (int64_t)TC_ITEM_ROWS * (D + 2);
+    auto part_of = [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * pitch; };
     const int rr = r % TC_ROWS, t = paged_div(rr, a.G, a.inv_G), tok = sp.tok0 + r / TC_ROWS * tc_tokens(a) + t;
-    if (t >= tc_tokens(a) || tok >= sp.n) return;
+    const bool valid = t < tc_tokens(a) && tok < sp.n;
     float m, l, v[8];
-    paged_gather8<TC_ITEM_ROWS>(a, D, c0, sp.c1, r, col, m, l, v);
+    if (parts <= TC_JOIN_PARTS) {
+        // the threads of a row share the parts' maxima and sums, then every thread adds its columns with all loads in flight
+        const float *ml = a.part + (int64_t)TC_ITEM_ROWS * D + 2 * r;
+        const unsigned group = __activemask();  // (whole warps)
+        m = -INFINITY;
+        if (valid)
+            for (int i = lane; i < parts; i += PER_ROW) {
+                const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + part_of(i)));
+                w_s[i][lr] = x;
+                m = fmaxf(m, x.x);
+            }
+#pragma unroll
+        for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(group, m, o));
+        l = 0.f;
+        if (valid)
+            for (int i = lane; i < parts; i += PER_ROW) {
+                const float2 x = w_s[i][lr];
+                const float w = x.x == -INFINITY ? 0.f : ex2(x.x - m);
+                w_s[i][lr].x = w;
+                w_s[i][lr].y = x.y * w;
+            }
+        __syncwarp();
+#pragma unroll
+        for (int x = 0; x < 8; x++) v[x] = 0.f;
+        if (!valid) return;
+        const float *o = a.part + (int64_t)r * D + col;
+#pragma unroll 8
+        for (int i = 0; i < parts; i++) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(o + part_of(i))), y = __ldcg(reinterpret_cast<const float4 *>(o + part_of(i) + 4));
+            const float w = w_s[i][lr].x;
+            l += w_s[i][lr].y;
+            v[0] = fmaf(w, x.x, v[0]); v[1] = fmaf(w, x.y, v[1]); v[2] = fmaf(w, x.z, v[2]); v[3] = fmaf(w, x.w, v[3]);
+            v[4] = fmaf(w, y.x, v[4]); v[5] = fmaf(w, y.y, v[5]); v[6] = fmaf(w, y.z, v[6]); v[7] = fmaf(w, y.w, v[7]);
+        }
+    } else {
+        if (!valid) return;
+        paged_gather8<TC_ITEM_ROWS>(a, D, c0, sp.c1, r, col, m, l, v);
+    }
     paged_finish8<BF16>(a, D, sp.q0 + tok, sp.head * a.G + (rr - t * a.G), col, m, l, v);
 }
 
