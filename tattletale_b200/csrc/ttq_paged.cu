@@ -15,10 +15,10 @@ namespace {
 // ---- append ----------------------------------------------------------------------------------------
 // Reads and writes 2 bytes per element of the fused rows and the cos / sin rows of each position: memory bound from a few hundred
 // tokens on, a launch below.  A thread holds elements 8 c .. 8 c + 7 of both halves of a head, so that a rotated pair is in one
-// thread; the D / 16 threads of a head sum its squares by shuffles.  The heads of a CTA's tokens are dealt out evenly, APPEND_DEPTH of a
-// thread's are loaded ahead, and four CTAs share an SM (cos, sin and the norm's weights come again and again from its cache): with
-// one head at a time and cos and sin held in registers 8101 tokens of 48 heads took 79 us, 2.6 TB/s.
-constexpr int APPEND_THREADS = 256, APPEND_DEPTH = 3;
+// thread; the D / 16 threads of a head sum its squares by shuffles.  The heads of a CTA's tokens are dealt out evenly and four CTAs share
+// an SM: cos, sin and the norm's weights come again and again from its cache, which leaves registers for as many.  8101 tokens of 48
+// heads: 57 us (3.6 TB/s), 79 with cos and sin held in registers (two CTAs), 61 to 82 with two to four heads of a thread in flight.
+constexpr int APPEND_THREADS = 256;
 
 struct AppendArgs {
     PagedArgs a;
@@ -91,65 +91,53 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) paged_append_kernel(const _
     const float inv_heads = 1.f / (float)heads;
     // the C threads of a head are consecutive lanes and take the same branches
     const unsigned group = C == 32 ? 0xffffffffu : ((1u << C) - 1u) << ((tid & 31) / C * C);
-    for (int p0 = slot; p0 < pairs; p0 += APPEND_DEPTH * SLOTS) {
-        uint4 raw[APPEND_DEPTH][2];
+    for (int x = slot; x < pairs; x += SLOTS) {
+        const int t = paged_div(x, heads, inv_heads), h = x - t * heads;
+        if (pos_s[t] < 0) continue;
+        const uint16_t *src = reinterpret_cast<const uint16_t *>(p.qkv) + (int64_t)(t0 + t) * p.ld_qkv + (int64_t)h * D;
+        uint4 r0 = __ldcs(reinterpret_cast<const uint4 *>(src + 8 * c)), r1 = __ldcs(reinterpret_cast<const uint4 *>(src + D / 2 + 8 * c));
+        uint16_t *out;
+        if (h < a.hq) out = reinterpret_cast<uint16_t *>(p.q_out) + (int64_t)(t0 + t) * p.ld_q + (int64_t)h * D;
+        else if (h < a.hq + a.hkv) out = reinterpret_cast<uint16_t *>(p.k) + dst_s[t] + (int64_t)(h - a.hq) * p.head_stride;
+        else out = reinterpret_cast<uint16_t *>(p.v) + dst_s[t] + (int64_t)(h - a.hq - a.hkv) * p.head_stride;
+        if (h < a.hq + a.hkv) {
+            float x0[8], x1[8], w[8];
+            unpack8(r0, BF16, x0);
+            unpack8(r1, BF16, x1);
+            const void *norm = h < a.hq ? p.q_norm : p.k_norm;
+            if (norm != nullptr) {
+                float ss = 0.f;
 #pragma unroll
-        for (int d = 0; d < APPEND_DEPTH; d++) {
-            const int x = p0 + d * SLOTS, t = paged_div(x, heads, inv_heads);
-            if (x < pairs && pos_s[t] >= 0) {
-                const uint16_t *src = reinterpret_cast<const uint16_t *>(p.qkv) + (int64_t)(t0 + t) * p.ld_qkv + (int64_t)(x - t * heads) * D;
-                raw[d][0] = *reinterpret_cast<const uint4 *>(src + 8 * c);
-                raw[d][1] = *reinterpret_cast<const uint4 *>(src + D / 2 + 8 * c);
+                for (int i = 0; i < 8; i++) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
+#pragma unroll
+                for (int o = C / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+                const float inv = rsqrtf(ss / (float)D + p.eps);
+                load8(norm, p.dt, 8 * c, w);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x0[i] = x0[i] * inv * w[i];
+                load8(norm, p.dt, D / 2 + 8 * c, w);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x1[i] = x1[i] * inv * w[i];
             }
+            const int64_t row = (int64_t)pos_s[t] * D;
+            float y[8];
+            load8(p.cosv, p.rope_dt, row + 8 * c, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = x0[i] * w[i];
+            load8(p.sinv, p.rope_dt, row + 8 * c, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] -= x1[i] * w[i];
+            r0 = pack8<BF16>(y);
+            load8(p.cosv, p.rope_dt, row + D / 2 + 8 * c, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = x1[i] * w[i];
+            load8(p.sinv, p.rope_dt, row + D / 2 + 8 * c, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] += x0[i] * w[i];
+            r1 = pack8<BF16>(y);
         }
-#pragma unroll
-        for (int d = 0; d < APPEND_DEPTH; d++) {
-            const int x = p0 + d * SLOTS, t = paged_div(x, heads, inv_heads), h = x - t * heads;
-            if (x >= pairs || pos_s[t] < 0) continue;
-            uint4 r0 = raw[d][0], r1 = raw[d][1];
-            uint16_t *out;
-            if (h < a.hq) out = reinterpret_cast<uint16_t *>(p.q_out) + (int64_t)(t0 + t) * p.ld_q + (int64_t)h * D;
-            else if (h < a.hq + a.hkv) out = reinterpret_cast<uint16_t *>(p.k) + dst_s[t] + (int64_t)(h - a.hq) * p.head_stride;
-            else out = reinterpret_cast<uint16_t *>(p.v) + dst_s[t] + (int64_t)(h - a.hq - a.hkv) * p.head_stride;
-            if (h < a.hq + a.hkv) {
-                float x0[8], x1[8], w[8];
-                unpack8(r0, BF16, x0);
-                unpack8(r1, BF16, x1);
-                const void *norm = h < a.hq ? p.q_norm : p.k_norm;
-                if (norm != nullptr) {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
-#pragma unroll
-                    for (int o = C / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-                    const float inv = rsqrtf(ss / (float)D + p.eps);
-                    load8(norm, p.dt, 8 * c, w);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x0[i] = x0[i] * inv * w[i];
-                    load8(norm, p.dt, D / 2 + 8 * c, w);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x1[i] = x1[i] * inv * w[i];
-                }
-                const int64_t row = (int64_t)pos_s[t] * D;
-                float y[8];
-                load8(p.cosv, p.rope_dt, row + 8 * c, w);
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = x0[i] * w[i];
-                load8(p.sinv, p.rope_dt, row + 8 * c, w);
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] -= x1[i] * w[i];
-                r0 = pack8<BF16>(y);
-                load8(p.cosv, p.rope_dt, row + D / 2 + 8 * c, w);
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] = x1[i] * w[i];
-                load8(p.sinv, p.rope_dt, row + D / 2 + 8 * c, w);
-#pragma unroll
-                for (int i = 0; i < 8; i++) y[i] += x0[i] * w[i];
-                r1 = pack8<BF16>(y);
-            }
-            *reinterpret_cast<uint4 *>(out + 8 * c) = r0;
-            *reinterpret_cast<uint4 *>(out + D / 2 + 8 * c) = r1;
-        }
+        *reinterpret_cast<uint4 *>(out + 8 * c) = r0;
+        *reinterpret_cast<uint4 *>(out + D / 2 + 8 * c) = r1;
     }
 }
 
