@@ -19,6 +19,7 @@ import torch
 from . import quantize as Q
 from ._lib import FMT_Q4_K, FMT_Q6_K
 from .layers import Context, QuantLinear, add_rmsnorm, decode_attention, rope_kv_append, silu_and_mul
+from .paged import sample
 
 
 @dataclass
@@ -130,10 +131,13 @@ class DecoderStack:
                 delta = self._row_parallel(L["down"], silu_and_mul(ctx, gu))
         return add_rmsnorm(ctx, h, delta, self.final_norm, cfg.rms_eps)
 
-    def step(self, token_ids: torch.Tensor) -> torch.Tensor:
-        """One decode step for `batch` sequences at position context-1; returns next token ids."""
+    def step(self, token_ids: torch.Tensor, u: torch.Tensor | None = None, **settings) -> torch.Tensor:
+        """One decode step for `batch` sequences at position context-1; returns next token ids: greedy, or drawn with the random numbers
+        ``u`` (one GPU) under the settings of ``sample``."""
+        if u is not None and self.world > 1:
+            raise ValueError("sampling needs the whole vocabulary's logits on one GPU")
         if self.fused_glue:
-            return self._pick(self.lm_head.forward(self._step_fused(token_ids), out_dtype=torch.float32))
+            return self._pick(self.lm_head.forward(self._step_fused(token_ids), out_dtype=torch.float32), u, settings)
         cfg, B, d = self.cfg, token_ids.shape[0], self.cfg.head_dim
         h = self.emb_rows[token_ids]
         for L in self.layers:
@@ -152,10 +156,12 @@ class DecoderStack:
             gu = L["gate_up"].forward(x)
             act = silu_and_mul(self.ctx, gu)
             h = h + self._row_parallel(L["down"], act)
-        return self._pick(self.lm_head.forward(self._rms(h, self.final_norm), out_dtype=torch.float32))
+        return self._pick(self.lm_head.forward(self._rms(h, self.final_norm), out_dtype=torch.float32), u, settings)
 
-    def _pick(self, logits: torch.Tensor) -> torch.Tensor:
-        """Greedy token over the (vocabulary-parallel) logits."""
+    def _pick(self, logits: torch.Tensor, u: torch.Tensor | None = None, settings=None) -> torch.Tensor:
+        """The sampled token, or the greedy one over the (vocabulary-parallel) logits."""
+        if u is not None:
+            return sample(self.ctx, logits, u, **(settings or {}))
         if self.world > 1:
             import torch.distributed as dist
 
