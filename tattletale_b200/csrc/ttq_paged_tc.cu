@@ -624,19 +624,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         // K and V of a unit into the next two slots: boxes of box_rows slots of one page.  Boxes that no row sees are left out of K
         // (their scores are masked) and are zeros in V; rows of a page that no row sees are zeroed in V, where a weight of zero would
         // meet them.  One warp's instruction latency bounds this loop, so what can be shared between K and V is.
-        int cache_first = -1, cache_b = -1, page_cache = 0;  // lane i: page number cache_first + i of the table of sequence cache_b
+        int cache_first = 0, page_cache = 0;  // lane i: page number cache_first + i of the item's table
         const int boxes = TC_UNIT / box_rows, box_bytes = box_rows * 128;
         for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
             const int m = g.m, u0 = g.unit, u_sink = g.u_sink, u_first = g.u_first, key_end = g.key_end, lo = g.lo, sink = g.sink, head = g.head, seq = g.b;
             if (m == 0) break;
             seg_done(k);
+            bool cached = false;  // (the entries are those of this item's keys: the next one of the sequence sees further)
             auto visible = [&](int from, int rows) { return from < key_end && (from + rows > lo || from < sink); };
 #pragma unroll 1
             for (int i = u0; i < u0 + m; i++) {
                 const int k0 = (i < u_sink ? i : u_first + i - u_sink) * TC_UNIT, idx = k0 >> a.page_shift;
-                if (cache_b != seq || idx < cache_first || idx + boxes > cache_first + 32) {
-                    cache_b = seq;
+                if (!cached || idx < cache_first || idx + boxes > cache_first + 32) {
+                    cached = true;
                     cache_first = idx;
                     const int at = idx + lane;
                     page_cache = a.n_pages;  // beyond the last page: zeros

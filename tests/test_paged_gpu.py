@@ -53,6 +53,16 @@ def test_prompts(ctx, lens, hq, hkv, d, page, dtype):
     check_attention(run(ctx, bt), bt)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("lens,hq,hkv,d,page,window", [([(1500, 0), (777, 300)], 32, 8, 128, 64, 0), ([(1111, 40)], 40, 8, 64, 16, 300),
+                                                       ([(900, 2000), (1, 5), (400, 0)], 28, 4, 128, 32, 0), ([(40, 3)] * 60, 16, 8, 64, 128, 0)])
+def test_many_items_per_cta(ctx, lens, hq, hkv, d, page, window, dtype):
+    """More row tiles and heads than the card has multiprocessors: every CTA serves items of several lengths, of one sequence and of
+    several, whole ones and ends of ones begun elsewhere."""
+    bt = Batch(lens, hq, hkv, d, page, dtype, seed=hq)
+    check_attention(run(ctx, bt, window=window, sinks=5), bt, window, 5)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (16, 0), (50, 4), (64, 64), (200, 130), (100000, 5)])
 @pytest.mark.parametrize("lens,hq,hkv,d,page", [STEPS[3], PROMPTS[1], PROMPTS[2], PROMPTS[4]])
 def test_windows(ctx, lens, hq, hkv, d, page, window, sinks):
