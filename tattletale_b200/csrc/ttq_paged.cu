@@ -485,56 +485,53 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             for (int w = 0; w < ROWS_WARPS; w++)
                 if (ml_s[w][r].x != -INFINITY) l = fmaf(ml_s[w][r].y, ex2(ml_s[w][r].x - m), l);
         };
+        const int rows = min(ROWS_TILE, cw.s.n * a.G - cw.rt * ROWS_TILE);
+        const bool apart = pos + 1 == sh.u1;
+        const int together = apart || rows <= 4 ? 4 : (rows <= 8 ? 2 : 1);
         {
             float M0, M1, x;
             joint(g, M0, x);
             joint(g + 8, M1, x);
             const float c0 = m0 == -INFINITY ? 0.f : ex2(m0 - M0), c1 = m1 == -INFINITY ? 0.f : ex2(m1 - M1);
-            // At the share's end the warps' rings are free and take a result each; before, one after the other adds into one buffer (a
-            // second one would cost the second CTA of the SM).
-            if (pos + 1 == sh.u1) {
-                float *mine = reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw)));
+            // At the share's end the warps' rings are free and take a result each.  Before, `together` warps at a time put theirs into the one
+            // buffer there is (a second one would cost the second CTA of the SM), all four where the tile has four rows.
+            float *mine = apart ? reinterpret_cast<float *>(smem_raw + (ring - smem_u32(smem_raw))) : obuf + (warp % together) * (ROWS_TILE / together) * C::OPITCH;
+            for (int turn = 0; turn < ROWS_WARPS / together; turn++) {
+                if (warp / together == turn) {
 #pragma unroll
-                for (int n = 0; n < D / 8; n++) {
-                    *reinterpret_cast<float2 *>(mine + g * C::OPITCH + 8 * n + 2 * t4) = make_float2(o[n][0] * c0, o[n][1] * c0);
-                    *reinterpret_cast<float2 *>(mine + (g + 8) * C::OPITCH + 8 * n + 2 * t4) = make_float2(o[n][2] * c1, o[n][3] * c1);
-                }
-                __syncthreads();
-            } else {
+                    for (int r = 0; r < 2; r++) {
+                        const float c = r == 0 ? c0 : c1;
+                        float *to = mine + (g + 8 * r) * C::OPITCH + 2 * t4;
+                        if (g + 8 * r < rows) {
 #pragma unroll
-            for (int turn = 0; turn < ROWS_WARPS; turn++) {
-                if (warp == turn) {
-#pragma unroll
-                    for (int n = 0; n < D / 8; n++) {
-                        float2 *d0 = reinterpret_cast<float2 *>(obuf + g * C::OPITCH + 8 * n + 2 * t4);
-                        float2 *d1 = reinterpret_cast<float2 *>(obuf + (g + 8) * C::OPITCH + 8 * n + 2 * t4);
-                        float2 v0 = make_float2(o[n][0] * c0, o[n][1] * c0), v1 = make_float2(o[n][2] * c1, o[n][3] * c1);
-                        if (turn > 0) {
-                            v0.x += d0->x; v0.y += d0->y;
-                            v1.x += d1->x; v1.y += d1->y;
+                            for (int n = 0; n < D / 8; n++) {
+                                float2 v = make_float2(o[n][2 * r] * c, o[n][2 * r + 1] * c);
+                                if (turn > 0) {
+                                    const float2 x = *reinterpret_cast<const float2 *>(to + 8 * n);
+                                    v.x += x.x;
+                                    v.y += x.y;
+                                }
+                                *reinterpret_cast<float2 *>(to + 8 * n) = v;
+                            }
                         }
-                        *d0 = v0;
-                        *d1 = v1;
                     }
                 }
                 __syncthreads();
             }
-            }
         }
-        const int rows = min(ROWS_TILE, cw.s.n * a.G - cw.rt * ROWS_TILE);
         const int own_slot = 2 * blockIdx.x + (seg_start == item_start ? 1 : 0);
         float *part = a.part + (int64_t)own_slot * ROWS_TILE * (D + 2);
         for (int i = tid; i < rows * (D / 8); i += ROWS_THREADS) {
             const int r = i / (D / 8), col = i % (D / 8) * 8;
             float m, l, v[8];
             joint(r, m, l);
-            const bool apart = pos + 1 == sh.u1;
 #pragma unroll
             for (int x = 0; x < 8; x++) v[x] = 0.f;
 #pragma unroll
             for (int w = 0; w < ROWS_WARPS; w++)
-                if (w == 0 || apart) {
-                    const float *from = apart ? reinterpret_cast<const float *>(smem_raw + (ring_base - smem_u32(smem_raw)) + w * C::STAGES * C::STAGE_BYTES) : obuf;
+                if (w < together) {
+                    const float *from = apart ? reinterpret_cast<const float *>(smem_raw + (ring_base - smem_u32(smem_raw)) + w * C::STAGES * C::STAGE_BYTES)
+                                              : obuf + w * (ROWS_TILE / together) * C::OPITCH;
                     const float4 *src = reinterpret_cast<const float4 *>(from + r * C::OPITCH + col);
                     const float4 y0 = src[0], y1 = src[1];
                     v[0] += y0.x; v[1] += y0.y; v[2] += y0.z; v[3] += y0.w;

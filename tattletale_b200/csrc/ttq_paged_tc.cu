@@ -185,7 +185,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // How the work is numbered: a unit of keys counts once for an item of one stream, twice for one of two; an item's start and end
 // count like TC_ITEM_WEIGHT of them.
-constexpr int TC_PAIR_WEIGHT = 2, TC_ITEM_WEIGHT = 4;
+constexpr int TC_PAIR_WEIGHT = 2, TC_ITEM_WEIGHT = 6;
 // Row tile rt of a sequence: its rows, and the keys that any of them sees.
 struct TcItem {
     PagedSeq k;      // key_end, lo, sink of this item (the rest as the sequence's)

@@ -48,13 +48,16 @@ class PagedBatch:
         if q_start.numel() != n + 1 or block_table.shape[0] != n:
             raise TtqError(2, f"q_start and block_table do not fit {n} sequences")
         self.q_start, self.kv_len, self.block_table, self.prefix_table = q_start, kv_len, block_table, prefix_table
-        self.n_seqs, self.max_q, self.prefix_len = n, max_q, prefix_len
+        self.n_seqs, self.max_q, self.prefix_len, self.device = n, max_q, prefix_len, q_start.get_device()
         self._args = PagedBatchArgs(n, 0, max_q, q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), block_table.shape[1],
                                     block_table.stride(0) if n > 1 else block_table.shape[1], prefix_len,
                                     None if prefix_table is None else prefix_table.data_ptr())
         self._page_entries = 0 if prefix_table is None else prefix_table.numel()
 
-    def _for(self, n_tokens: int, page_size: int) -> PagedBatchArgs:
+    def _for(self, plan: "PagedAttention", n_tokens: int) -> PagedBatchArgs:
+        if self.device != plan.device:
+            raise _elsewhere("the batch's tensors")
+        page_size = plan.page_size
         if self.prefix_len > self._page_entries * page_size:
             raise TtqError(2, f"prefix_table has {self._page_entries} pages of {page_size}, prefix_len is {self.prefix_len}")
         self._args.n_tokens = n_tokens
@@ -135,7 +138,7 @@ class PagedAttention:
             norms.append(None if w is None else _on(self.ctx, w, name).data_ptr())
         q_out, ld_q = self._out(q_out, n, rows, "q_out")
         ctx = self.ctx
-        st = ctx._lib.ttq_paged_append(ctx.handle, self.handle, self._pages(k_pages, v_pages), batch._for(n, self.page_size), rows.data_ptr(), ld,
+        st = ctx._lib.ttq_paged_append(ctx.handle, self.handle, self._pages(k_pages, v_pages), batch._for(self, n), rows.data_ptr(), ld,
                                        norms[0], norms[1], eps, cos.data_ptr(), sin.data_ptr(),
                                        _dt(cos.dtype), cos.shape[0], q_out.data_ptr(), ld_q, _stream_ptr(rows.device))
         if st != 0:
@@ -149,7 +152,7 @@ class PagedAttention:
         rows, n, ld = self._rows(q, self.hq, "q")
         out, ld_out = self._out(out, n, rows, "out")
         ctx = self.ctx
-        st = ctx._lib.ttq_paged_attention(ctx.handle, self.handle, self._pages(k_pages, v_pages), batch._for(n, self.page_size), rows.data_ptr(),
+        st = ctx._lib.ttq_paged_attention(ctx.handle, self.handle, self._pages(k_pages, v_pages), batch._for(self, n), rows.data_ptr(),
                                           ld, self.scale if scale is None else scale, window, sinks, out.data_ptr(), ld_out, _stream_ptr(rows.device))
         if st != 0:
             check(ctx.handle, st)
@@ -196,8 +199,8 @@ def sample(ctx: Context, logits: torch.Tensor, u: torch.Tensor, temperature: Uni
     _on(ctx, u, "u")
     if out is None:
         out = torch.empty((m,), dtype=torch.int64, device=logits.device)
-    elif out.dtype != torch.int64 or out.numel() != m or not out.is_contiguous() or not out.is_cuda:
-        raise TtqError(2, f"out must be {m} contiguous int64 values on the device")
+    elif _on(ctx, out, "out").dtype != torch.int64 or out.numel() != m or not out.is_contiguous():
+        raise TtqError(2, f"out must be {m} contiguous int64 values")
     st = ctx._lib.ttq_sample(ctx.handle, logits.data_ptr(), _dt(logits.dtype), m, v, logits.stride(0) if m > 1 else v, ctypes.byref(s), u.data_ptr(),
                              out.data_ptr(), _stream_ptr(logits.device))
     if st != 0:
