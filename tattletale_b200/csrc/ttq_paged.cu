@@ -17,7 +17,7 @@ namespace {
 // tokens on, a launch below.  A thread holds elements 8 c .. 8 c + 7 of both halves of a head, so that a rotated pair is in one
 // thread; the D / 16 threads of a head sum its squares by shuffles.  The heads of a CTA's tokens are dealt out evenly and four CTAs share
 // an SM: cos, sin and the norm's weights come again and again from its cache, which leaves registers for as many.  8101 tokens of 48
-// heads: 57 us (3.6 TB/s), 79 with cos and sin held in registers (two CTAs), 61 to 82 with two to four heads of a thread in flight.
+// heads: 55 us (3.7 TB/s), 79 with cos and sin held in registers (two CTAs), 61 to 82 with two to four heads of a thread in flight.
 constexpr int APPEND_THREADS = 256;
 
 struct AppendArgs {

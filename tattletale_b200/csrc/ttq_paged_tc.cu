@@ -5,11 +5,11 @@
 // 128 keys.  Its two halves are two streams that take turns: while the softmax of one runs on the CUDA cores, the tensor core multiplies for the other.
 //   S = Q K^T     128 rows x 64 keys (half a unit), Q and K in shared memory (K-major, 128-byte swizzle), S in one of the stream's two
 //                 score buffers in tensor memory
-//   softmax       one thread per row: 64 scores from tensor memory, reference and sum in registers, weights in the 16-bit type
+//   softmax       a thread per row: 64 scores from tensor memory, reference and sum in registers, weights in the 16-bit type
 //                 back into the columns that the scores had
 //   O += P V      P from tensor memory, V as it lies in its pages (keys as rows: the transposed operand form), O in tensor memory
-// The scores of half j + 1 are complete while the softmax works on half j.  With one buffer of 128 keys per stream the
-// softmax waited for product and product for softmax in turn: 4260 clocks per unit and stream pair instead of
+// The scores of half j + 1 are complete while the softmax works on half j.  With one buffer of 128 keys per stream the softmax
+// waited for the product and the product for the softmax: 4260 clocks per unit of both streams instead of 3500.
 // An item of one half gives both streams the same rows and every other unit of keys; the two results meet in tensor
 // memory, whose lanes the warps of both streams reach.  Tensor memory is full: 2 x 2 x 64 columns of scores, 2 x d of output.
 //
@@ -20,6 +20,10 @@
 // G heads of a run of tokens are the rows of a tile as they lie).  Products of one stream execute in the order of issue, so the scores of half
 // j + 2 may follow the product that reads the weights of half j from the same columns.  The softmax warps rescale the output in
 // place, which they do only when the weights outgrow their reference and once the last product that they asked for is complete.
+//
+// Bound: 4 d flops and one exponential per key and row; at d = 128 the special-function unit (16 a clock and SM) takes as long for a
+// unit's exponentials as the tensor core for its products, 2048 clocks for both streams.  Measured: 780 TFLOP/s on prompts of
+// 1111 to 4300 tokens (284 us, 47 % of the measured bf16 rate), 850 on 24000 shared keys.
 #include <climits>
 
 #include "ttq_devutil.cuh"
