@@ -86,6 +86,83 @@ def test_window_over_a_shared_prefix(ctx, lens, window, sinks):
     check_attention(run(ctx, bt, window=window, sinks=sinks), bt, window, sinks)
 
 
+@pytest.mark.parametrize("lens,hq,hkv,d,page,prefix", [
+    ([(1, 30), (1, 700)], 160, 1, 64, 16, 0),        # more query heads on a kv head than a stream of the tensor-memory kernel has rows
+    ([(3, 10), (40, 0)], 160, 1, 64, 32, 90),
+    ([(3, 10), (70, 200)], 128, 1, 128, 256, 40),    # as many; pages longer than a unit
+    ([(3, 10), (70, 200)], 65, 1, 64, 512, 0),       # half a stream idle
+    ([(300, 1000)], 96, 2, 128, 1024, 0),
+])
+def test_many_query_heads_and_long_pages(ctx, lens, hq, hkv, d, page, prefix):
+    bt = Batch(lens, hq, hkv, d, page, BF16, prefix=prefix, seed=hq)
+    check_attention(run(ctx, bt), bt)
+    check_attention(run(ctx, bt, window=64, sinks=7), bt, 64, 7)
+
+
+@pytest.mark.parametrize("lens", [[(1, i % 97) for i in range(1000)], [(i % 5, 3 * i % 211) for i in range(800)], [(150, 0)] + [(1, 40)] * 500 + [(33, 70)]])
+@pytest.mark.parametrize("prefix", [0, 33])
+def test_many_sequences(ctx, lens, prefix):
+    """More sequences than a CTA has threads."""
+    bt = Batch(lens, 4, 2, 64, 16, BF16, prefix=prefix, seed=5)
+    check_attention(run(ctx, bt), bt)
+    plan = bt.plan(ctx)
+    qkv = torch.randn(bt.rows, 8 * 64, device="cuda").to(BF16)
+    n_rope = int(bt.kv_len.max())
+    q = plan.append(qkv, bt.k, bt.v, bt.batch(), torch.ones(n_rope, 64, device="cuda"), torch.zeros(n_rope, 64, device="cuda"))
+    ctx.check_device_status()
+    assert torch.equal(q, qkv.view(-1, 8, 64)[:, :4])
+    row = 0
+    for b, (n, p) in enumerate(lens):
+        if n and b % 50 == 0:
+            at = p + n - 1
+            assert torch.equal(bt.k[int(bt.table_host[b, at // 16]), :, at % 16], qkv[row + n - 1].view(8, 64)[4:6])
+        row += n
+
+
+@pytest.mark.parametrize("prefix", [0, 33])
+@pytest.mark.parametrize("max_q", [1, 500])
+def test_a_batch_without_new_tokens(ctx, prefix, max_q):
+    """Every sequence sits this call out: nothing is written."""
+    bt = Batch([(1, 20), (2, 300)], 8, 2, 128, 16, BF16, prefix=prefix)
+    bt.q_start.zero_()
+    out = torch.full((3, 8, 128), 3.0, dtype=BF16, device="cuda")
+    plan = bt.plan(ctx)
+    plan.forward(bt.q, bt.k, bt.v, bt.batch(max_q), out=out)
+    assert (out == 3).all()
+    k0 = bt.k.clone()
+    plan.append(torch.ones(3, 12 * 128, dtype=BF16, device="cuda"), bt.k, bt.v, bt.batch(max_q), torch.ones(400, 128, device="cuda"),
+                torch.ones(400, 128, device="cuda"), q_out=out)
+    ctx.check_device_status()
+    assert (out == 3).all() and torch.equal(k0.view(torch.int16), bt.k.view(torch.int16))
+
+
+@pytest.mark.parametrize("new", [1, 200])
+def test_infinite_values_that_nobody_sees(ctx, new):
+    """Infinities and the type's extremes behind a sequence's end, in pages of nobody and before its window."""
+    window = 70
+    bt = Batch([(new, 400), (new, 77)], 8, 2, 128, 16, F16, seed=6)
+    want = run(ctx, bt, window=window)
+    for x, v in ((bt.k, float("inf")), (bt.v, -65504.0)):
+        x[torch.isnan(x)] = v
+    first = 400 - window + 1  # of sequence 0: no token sees the pages before this position
+    for page in bt.table_host[0, :first // 16].tolist():
+        bt.k[page], bt.v[page] = float("nan"), float("inf")
+    got = run(ctx, bt, window=window)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_scores_of_great_range(ctx, new):
+    """Scores that grow by hundreds along the keys, and rows whose first keys dwarf the rest: the running reference has to follow."""
+    for sign in (1, -1):
+        bt = Batch([(new, 900)], 4, 2, 64, 16, BF16, seed=7)
+        pos = torch.arange(900 + new, device="cuda")
+        pages, slots = bt.table_host[0][pos.cpu() // 16].long().cuda(), pos % 16
+        bt.k[pages, :, slots, 0] = (sign * pos.float() * 0.5).to(BF16)[:, None]
+        bt.q[..., 0] = 4.0
+        check_attention(run(ctx, bt), bt)
+
+
 @pytest.mark.parametrize("layout", ["nhd", "joint"])
 def test_page_layouts(ctx, layout):
     bt = Batch([(1, 200), (9, 31), (140, 0)], 8, 4, 128, 16, BF16, layout=layout, seed=3)
