@@ -1780,9 +1780,11 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
         a.prefix_pass = pass == 0;
         a.pre_o = bt->prefix_len > 0 ? p->pre_o : nullptr;
         a.pre_lse = p->pre_lse;
-        // few rows per kv head: the memory-bound kernel; from 17 on the tensor-memory kernel
+        // Few rows per kv head: the memory-bound kernel, a second tile of 16 reading K and V once more; from 33 rows on the tensor-memory
+        // kernel.  Measured (32 sequences of 4000 positions, 8 kv heads, d = 128): 16 rows 102 us (tensor memory: 208), 32 rows 181 (208),
+        // 64 rows 315 (210); 64 sequences of 2000, d = 64: 24 rows 95 (124); one of 500: 20 rows 13 (16), 64 rows 15 (17).
         const int64_t most = a.prefix_pass || bt->max_q == 0 ? bt->n_tokens : bt->max_q;
-        const bool few = most * a.G <= 16 || a.G > 128;
+        const bool few = most * a.G <= 32 || a.G > 128;
         a.counters = few ? p->counters : p->splits;
         const int slots = few ? 16 : (p->page_size < 128 ? p->page_size : 128);
         PagedMaps maps;

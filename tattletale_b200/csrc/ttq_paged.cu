@@ -2,8 +2,8 @@
 //
 //   paged_append_kernel   one CTA per few tokens: finds the tokens' sequences, normalises and rotates q and k heads, writes q
 //                         out and k, v into the pages
-//   paged_rows_kernel     attention of tiles of 16 rows (tokens x query heads of one kv head); memory bound: every key and value
-//                         is read once and feeds two 16-row tensor-core products from registers
+//   paged_rows_kernel     attention of tiles of 16 rows (tokens x query heads of one kv head), one or two of them per sequence; memory
+//                         bound: every key and value is read once per tile and feeds two products from registers
 #include <climits>
 
 #include "ttq_devutil.cuh"
