@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
         tma_prefetch(&qmap);
         for (int i = 0; i < C::SLOTS; i++) {
             mbar_init(kv_full + 8 * i, 1);
-            mbar_init(kv_empty + 8 * i, 2);  // one arrival per stream, two of the only one that takes the slot
+            mbar_init(kv_empty + 8 * i, 2);  // one arrival per stream
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(q_full + 8 * i, 1);
@@ -708,26 +708,35 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 }
             }
         }
-        // the last copies have landed before the CTA may end: the product warp waits for every slot
+        // the last copies have landed before the CTA may end: the product warps wait for every fill
     } else if (warp == TC_MMA_WARP || warp == TC_MMA1_WARP) {
         // ------------------------------------------------------------------------------------------ products of a stream
         const int st = warp == TC_MMA_WARP ? 0 : 1;
         bool alive = true;
-        int n = 0;                       // slots that earlier items took
+        int n = 0, seen = 0;             // fills of the ring: of earlier items; that this warp has seen
         uint32_t q_par = 0u, p_par[2] = {0u, 0u};
         constexpr uint32_t idesc_s = tc_idesc<BF16>(TC_HALF, false), idesc_o = tc_idesc<BF16>(D, true);
         const uint32_t sc = tmem + C::S_COL + st * TC_UNIT, o = tmem + C::O_COL + st * D;
         const uint64_t qd = smem_desc_sw128(base + (uint32_t)st * C::SLOT_BYTES);
         auto slot_addr = [&](int i) { return base + C::RING_AT + (uint32_t)(i % C::SLOTS) * C::SLOT_BYTES; };
-        auto wait_slot = [&](int i) {
-            if (alive) alive = tc_wait(kv_full + 8 * (i % C::SLOTS), (uint32_t)((i / C::SLOTS) & 1), a.status);
-        };
         for (int k = 0; seg_wait(k); k++) {
             const TcSeg &g = segs[k % TC_SEGS];
             const int m = g.m;
             if (m == 0) break;
             const bool pair = g.pair;
             seg_done(k);
+            // A parity tells a phase only from its neighbours: each of the two warps sees every fill of the ring in turn, and lets go of the
+            // other stream's at once (a warp that skipped them would take the copy before its own for it, where that one is still under
+            // way and the streams' slots have changed places).  They have been asked for before the warp's own next one: no time lost.
+            auto see = [&](int last) {
+                for (; seen <= last; seen++) {
+                    if (alive) alive = tc_wait(kv_full + 8 * (seen % C::SLOTS), (uint32_t)((seen / C::SLOTS) & 1), a.status);
+                    if (!pair && (((seen - n) >> 1) & 1) != st) {
+                        __syncwarp();  // (no lane still asks for this phase)
+                        if (lane == 0) mbar_arrive(kv_empty + 8 * (seen % C::SLOTS));
+                    }
+                }
+            };
             // slots in the order of the copies: K V K V ...
             auto k_slot = [&](int i) { return n + 2 * i; };
             auto v_slot = [&](int i) { return n + 2 * i + 1; };
@@ -740,8 +749,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                 // half by half: O += P V of unit i, then S = Q K^T of the next one into the same buffer
                 const bool with_v = i >= first, with_k = i + step < m;
                 const int vs = with_v ? v_slot(i) : 0, ks = with_k ? k_slot(i + step) : 0;
-                if (with_v) wait_slot(vs);
-                if (with_k) wait_slot(ks);
+                if (with_v) see(vs);
+                if (with_k) see(ks);
 #pragma unroll 1
                 for (int h = 0; h < 2; h++) {
                     if (with_v) {
@@ -757,10 +766,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                             for (int kk = 0; kk < TC_HALF / 16; kk++)
                                 tc_mma_ts(o, sc + h * TC_HALF + 8 * kk, vd + (uint64_t)((kk * 2048) >> 4), idesc_o, i == first && h + kk == 0 ? 0u : 1u);
                             umma_commit(o_full + 8 * st);
-                            if (h == 1) {
-                                umma_commit(kv_empty + 8 * (vs % C::SLOTS));
-                                if (!pair) umma_commit(kv_empty + 8 * (vs % C::SLOTS));
-                            }
+                            if (h == 1) umma_commit(kv_empty + 8 * (vs % C::SLOTS));
                         }
                         if (with_k) {
                             const uint64_t kd = smem_desc_sw128(slot_addr(ks) + (uint32_t)(h * TC_HALF * 128));
@@ -774,13 +780,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                             if (h == 1) {
                                 if (i + 2 * step >= m) umma_commit(q_empty + 8 * st);
                                 umma_commit(kv_empty + 8 * (ks % C::SLOTS));
-                                if (!pair) umma_commit(kv_empty + 8 * (ks % C::SLOTS));
                             }
                         }
                     }
                     __syncwarp();
                 }
             }
+            see(n + 2 * m - 1);
             n += 2 * m;
         }
     } else if (warp == TC_WALK_WARP) {
