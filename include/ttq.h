@@ -432,6 +432,7 @@ typedef struct ttq_sampling {
  * one token stays), of those to w_i >= min_p (the largest logit always stays).  The result is the first token, in the order of the vocabulary, at which the
  * cumulative weight of what is left exceeds u[m] times its total.  temperature <= 0 or NaN: the token of the largest logit (lowest
  * index).  NaN logits count as -inf, a row of nothing but -inf gives -1; where a logit is +inf only such tokens have weight.
+ * Random numbers outside [0, 1) count as the nearest one in it, NaN as 0.
  * Weights are computed in 64 bits and summed as 2^-44 fixed point, so that the cuts fall where the definition has them and
  * results do not depend on the order of summation.  Any M >= 0, V from 1 to 2^18. */
 TTQ_API ttq_status ttq_sample(ttq_ctx *ctx, const void *logits_dev, ttq_dtype dt, int64_t M, int64_t V, int64_t ld,

@@ -535,8 +535,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     }
     cluster_sync();  // (no CTA leaves while another may read its shared memory)
     // first token whose cumulative weight exceeds the target
-    double target = (double)fminf(fmaxf(a.u[row], 0.f), 1.f) * (double)total;
-    if (target >= (double)total) target = (double)(total - 1);
+    // (at most the largest u below 1: above 2^53 a double does not tell total - 1 from total)
+    const double target = (double)fminf(fmaxf(a.u[row], 0.f), 0x1.fffffep-1f) * (double)total;
     if (mine > 0 && (double)start <= target && target < (double)(start + mine)) {
         u64 cum = start;
         walk([&](int i, u64 w) {

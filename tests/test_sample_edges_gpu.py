@@ -1,0 +1,26 @@
+"""The sampler at its edges: random numbers outside their range."""
+import numpy as np
+import pytest
+import torch
+
+import tattletale_b200 as ttq
+from paged_util import sample64
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("u", [1.0, 2.0, float("inf"), -1.0, float("nan")])
+@pytest.mark.parametrize("v", [7, 1000, 100000])
+def test_random_numbers_outside_their_range(ctx, v, u):
+    """They count as the nearest in [0, 1): every row gets a token that was kept, flat rows of a great total weight too."""
+    logits = torch.zeros(5, v, device="cuda")
+    logits[2, v // 2] = -float("inf")
+    logits[3, v - 1] = -float("inf")
+    clamped = np.float32(0 if u != u else min(max(u, 0.0), 1.0 - 2.0 ** -24))
+    for s in (dict(), dict(top_k=max(1, v // 3)), dict(top_p=0.37), dict(temperature=9.0)):
+        for dtype in (torch.float32, torch.bfloat16):
+            out = torch.full((5,), -7, dtype=torch.int64, device="cuda")
+            ttq.sample(ctx, logits.to(dtype), torch.full((5,), u, device="cuda"), out=out, **s)
+            want = [sample64(logits[r].cpu().numpy(), clamped, np.float32(s.get("temperature", 1.0)), s.get("top_k", 0), np.float32(s.get("top_p", 1.0)), 0.0)
+                    for r in range(5)]
+            assert out.tolist() == want
