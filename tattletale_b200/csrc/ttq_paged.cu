@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
 
     // fragments of the tile's rows: this thread's are g and g + 8
     uint32_t qf[D / 16][4];
-    float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // references of the weights, and their sums
     int pos0 = 0, pos1 = 0, min_row = 0, max_row = 0;
     auto row_of = [&](int r, int &token, int &head) {
         const int x = cw.rt * ROWS_TILE + r, i = paged_div(x, a.G, a.inv_G);
@@ -417,9 +417,10 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                 x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
                 x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
             }
-            // the running maximum follows only when a score exceeds it by 2^8: weights stay below 256, sums are exact in scale
-            if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f)) {
-                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+            // the reference follows the maximum only when a score exceeds it by RISE: weights stay finite in f16
+            constexpr float BELOW = PAGED_BELOW<BF16>, RISE = BF16 ? 8.f : 15.f;
+            if (__any_sync(0xffffffffu, x0 > m0 + RISE || x1 > m1 + RISE)) {
+                const float n0 = fmaxf(m0, x0 - BELOW), n1 = fmaxf(m1, x1 - BELOW);
                 const float c0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), c1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
                 m0 = n0;
                 m1 = n1;

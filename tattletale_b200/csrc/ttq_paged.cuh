@@ -49,6 +49,13 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The softmax weights enter the second product in the 16-bit type, the only operand that the tensor cores take beside 16-bit values: a
+// rounding of half a step of each weight (2^-8 relative in bf16, 2^-11 in f16), where the contiguous step's kernel (ttq_decode.cu)
+// multiplies in 32 bits.  Weights are 2^(score - reference); in f16, whose range ends at 2^-14 (2^-24 in steps), the reference
+// lies 2^9 below the maximum that it was taken from, so that a weight is rounded relative to itself down to 2^-23 of the row's
+// largest and is off by no more than 2^-34 of it below.  Their sum is of the unrounded ones.
+template <bool BF16>
+constexpr float PAGED_BELOW = BF16 ? 0.f : 9.f;
 constexpr int PAGED_BAD_INDEX = 8;  // status bit: page id or position outside the cache
 
 // One sequence's rows and keys (prefix pass: the one group of all rows).  Keys are in the coordinates of its page table.

@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             int pos = -1;
             if (valid) pos = a.prefix_pass ? paged_row_pos(a, g.q0 + tok) : g.pos0 + tok;
             const int min_row = __reduce_min_sync(0xffffffffu, valid ? pos : INT_MAX), max_row = __reduce_max_sync(0xffffffffu, valid ? pos : -1);
-            float mx = valid ? -INFINITY : 0.f, l = 0.f;  // reference for the scores (unscaled) and sum
+            float mx = valid ? -INFINITY : 0.f, l = 0.f;  // maximum that the reference goes by (unscaled), and sum
             const int step = joint ? 2 : 1, first = joint ? st : 0;
             const uint32_t halves0 = halves;
             for (int i = first; i < m; i += step) {
@@ -440,8 +440,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                         for (int kk = 0; kk < TC_HALF; kk++)
                             if (!(kk < end && (kk >= from || kk < sink))) s[kk] = -INFINITY;
                     }
-                    // The weights are taken relative to the row's reference `mx`, which follows the maximum only when they grow too
-                    // large (a sum of 2^15: every weight is finite in fp16): the maximum of 64 scores costs a fifth of their softmax.
+                    // The weights are taken relative to the row's reference (`mx` less PAGED_BELOW), which follows the maximum only when they
+                    // grow too large (by their sum: every weight is finite in f16, where 64 weights of 2^9 are 2^15): the maximum of 64
+                    // scores costs a fifth of their softmax.
                     // The streams' exponentials take turns.  Each alone keeps the special-function unit busy (590 clocks for 64 rows' weights of a
                     // warp, 512 at the unit's rate); both at once take as long as one after the other, and then both wait for
                     // their next scores at once, the unit idle.  The turn passes on half way, which hides the hand-over (prompts of 8116
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                                 }
                             }
                         }
-                        const float off = mx == -INFINITY ? 0.f : -mx * a.scale2;
+                        const float off = mx == -INFINITY ? 0.f : fmaf(-mx, a.scale2, PAGED_BELOW<BF16>);
                         const uint64_t off_2 = f2(off, off);
                         uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                         float x, y;
                         f2_split(add2(sums[0], sums[1]), x, y);
                         sum = x + y;
-                        redo = valid && !(sum <= 32768.f);  // (rows of no token hold anything)
+                        redo = valid && !(sum <= (BF16 ? 32768.f : 61440.f));  // (rows of no token hold anything)
                         if (turn > 0 || !__any_sync(0xffffffffu, redo)) break;
                     }
                     l += sum;
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
             if (first < m && alive) alive = tc_wait(o_full + 8 * st, (halves - 1) & 1, a.status);
             __syncwarp();
             tc_fence_after();
-            const float m2 = mx == -INFINITY ? -INFINITY : mx * a.scale2;
+            const float m2 = mx == -INFINITY ? -INFINITY : -fmaf(-mx, a.scale2, PAGED_BELOW<BF16>);  // the reference in log2
             const bool complete = g.complete;
             const int token = g.q0 + tok, head = g.head * a.G + r_head;
             float M = m2, L = l, f0 = 1.f, f1 = 0.f;

@@ -1,4 +1,6 @@
 """Paged attention and append at their edges: odd numbers of units, faint weights, empty sequences, extreme lengths and windows."""
+import math
+
 import pytest
 import torch
 
@@ -28,3 +30,60 @@ def test_items_of_odd_length_follow_each_other(ctx, units, d):
     check_attention(first, bt)
     for _ in range(20):
         assert torch.equal(run(ctx, bt), first)
+
+
+@pytest.mark.parametrize("new", [1, 12, 40])
+def test_faint_weights_behind_a_dominant_key(ctx, new):
+    """f16: a first key of value zero that outweighs each of 30000 others by 2^25.  The result is theirs: weights that the 16-bit type
+    cannot hold relative to the row's largest still have to count.  320 sequences that share their pages, so that a CTA sees whole
+    rows.  The bound: as in attention64, and weights off by 2^-34 of the largest (half a step of 2^-24 at a largest weight of 2^9),
+    and half a step of 2^-24 of the result."""
+    past, d, hq, seqs, page = 30000, 64, 2, 320, 64
+    bt = Batch([(new, past)], hq, 1, d, page, F16, seed=1)
+    total = past + new
+    pos = torch.arange(total)
+    pages, slots = bt.table_host[0][pos // page].long().cuda(), (pos % page).cuda()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k = torch.zeros(total, d, device="cuda")
+    k[:, 0] = 0.3 * torch.rand(total, generator=g, device="cuda")
+    k[0, 0] = 17.7
+    v = 1.0 + torch.rand(total, d, generator=g, device="cuda")
+    v[0] = 0.0
+    bt.k[pages, 0, slots], bt.v[pages, 0, slots] = k.to(F16), v.to(F16)
+    bt.q.zero_()
+    bt.q[..., 0] = 8.0
+    k64, v64 = bt.keys(0)
+    q = bt.q.double().transpose(0, 1)
+    seen = torch.arange(total, device="cuda")[None] <= torch.arange(past, total, device="cuda")[:, None]
+    w = torch.softmax(torch.where(seen, q @ k64.transpose(1, 2) / 8.0, -math.inf), -1)
+    want = (w @ v64).transpose(0, 1)
+    u, err_s = 2.0 ** -11, d * 2.0 ** -23 * 17.7
+    bound = want * (2 * u + 2 * err_s + 2.0 ** -18) + 2.0 ** -34 * v64.abs().sum(1)[0] + 2.0 ** -25
+    ints = torch.arange(seqs + 1, dtype=torch.int32, device="cuda")
+    batch = ttq.PagedBatch(ints * new, torch.full((seqs,), total, dtype=torch.int32, device="cuda"), bt.table.expand(seqs, -1).contiguous(), max_q=new)
+    plan = ttq.PagedAttention(ctx, hq, 1, d, page, max_seqs=seqs, max_tokens=seqs * new, dtype=F16)
+    got = plan.forward(bt.q.repeat(seqs, 1, 1), bt.k, bt.v, batch).double().view(seqs, new, hq, d)
+    ctx.check_device_status()
+    assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max()
+
+
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("slope", [-0.5, 0.03, 0.5])
+def test_f16_scores_of_great_range(ctx, new, slope):
+    """Scores that grow or fall by up to hundreds along the keys: weights stay finite in f16 and the reference follows."""
+    bt = Batch([(new, 900)], 4, 2, 64, 16, F16, seed=7)
+    pos = torch.arange(900 + new)
+    pages, slots = bt.table_host[0][pos // 16].long().cuda(), (pos % 16).cuda()
+    bt.k[pages, :, slots, 0] = (slope * pos.float()).to(F16).cuda()[:, None]
+    bt.q[..., 0] = 4.0
+    check_attention(run(ctx, bt), bt)
+
+
+@pytest.mark.parametrize("new", [1, 150])
+def test_f16_flat_scores(ctx, new):
+    """Equal scores everywhere: the largest sums of weights that a tile can have."""
+    bt = Batch([(new, 900)], 4, 2, 64, 16, F16, seed=7)
+    bt.q.fill_(0.0)
+    check_attention(run(ctx, bt), bt)
+    bt.k[:], bt.q[:] = 0.5, 0.5
+    check_attention(run(ctx, bt), bt)
