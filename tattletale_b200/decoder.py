@@ -134,6 +134,8 @@ class DecoderStack:
     def step(self, token_ids: torch.Tensor, u: torch.Tensor | None = None, **settings) -> torch.Tensor:
         """One decode step for `batch` sequences at position context-1; returns next token ids: greedy, or drawn with the random numbers
         ``u`` (one GPU) under the settings of ``sample``."""
+        if u is None and settings:
+            raise ValueError(f"{', '.join(settings)}: settings of the sampler need random numbers u")
         if u is not None and self.world > 1:
             raise ValueError("sampling needs the whole vocabulary's logits on one GPU")
         if self.fused_glue:
