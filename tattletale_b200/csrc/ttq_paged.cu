@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
     // fragments of the tile's rows: this thread's are g and g + 8
     uint32_t qf[D / 16][4];
     float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // references of the weights, and their sums
-    int pos0 = 0, pos1 = 0, min_row = 0, max_row = 0;
+    int pos0 = 0, pos1 = 0, min_row = 0, max_row = 0, lo_row = 0;  // lo_row: smallest position of a row that has one
     auto row_of = [&](int r, int &token, int &head) {
         const int x = cw.rt * ROWS_TILE + r, i = paged_div(x, a.G, a.inv_G);
         token = cw.s.q0 + i;
@@ -351,6 +351,9 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             min_row = r == 0 ? lo : min(min_row, lo);
             max_row = r == 0 ? hi : max(max_row, hi);
         }
+        lo_row = min_row;
+        if (a.prefix_pass && min_row < 0)  // (rows of other sequences, which may be padding)
+            lo_row = __reduce_min_sync(0xffffffffu, min(pos0 >= 0 ? pos0 : INT_MAX, pos1 >= 0 ? pos1 : INT_MAX));
 #pragma unroll
         for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
         m0 = m1 = -INFINITY;
@@ -401,7 +404,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
                         if (!v0) s[n][e] = -INFINITY;
                         if (!v1) s[n][2 + e] = -INFINITY;
                         // values that no row sees may be anything: zero them
-                        const bool any = in && j <= max_row && (a.window == 0 || j > min_row - a.window || j < a.sinks);
+                        const bool any = in && j <= max_row && (a.window == 0 || j > lo_row - a.window || j < a.sinks);
                         if (!any) vm[n] &= e == 0 ? 0xffff0000u : 0x0000ffffu;
                     }
                 }

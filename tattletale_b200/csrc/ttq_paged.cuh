@@ -150,7 +150,7 @@ struct PagedShare {
     int64_t seq_u;   // number of the first unit of the sequence that holds u0
     int b;           // that sequence
     int N;           // CTAs that have a share
-    int min_pos;     // prefix pass: smallest position of any token
+    int min_pos;     // prefix pass: smallest position of any token that has one (INT_MAX: none does)
 };
 
 // Number of shares: of at least MIN_SHARE numbers each, at most one per CTA.
@@ -170,8 +170,8 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
     if (a.prefix_pass && a.window > 0) {
         int mp = INT_MAX;
         for (int b = tid; b < a.B; b += THREADS) {
-            const int n = a.q_start[b + 1] - a.q_start[b];
-            if (n > 0) mp = min(mp, a.kv_len[b] - n);
+            const int n = a.q_start[b + 1] - a.q_start[b], L = a.kv_len[b];
+            if (n > 0 && L > 0) mp = min(mp, max(0, L - n));  // (padding, a token of no position, sees nothing)
         }
         mp = __reduce_min_sync(0xffffffffu, mp);
         if (lane == 0) red[warp] = mp;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import tattletale_b200 as ttq
-from paged_util import Batch, check_attention
+from paged_util import Batch, attention64, check_attention
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -87,3 +87,28 @@ def test_f16_flat_scores(ctx, new):
     check_attention(run(ctx, bt), bt)
     bt.k[:], bt.q[:] = 0.5, 0.5
     check_attention(run(ctx, bt), bt)
+
+
+@pytest.mark.parametrize("sinks", [0, 5])
+@pytest.mark.parametrize("new", [1, 40])
+def test_padding_sequences_of_a_batch_with_a_prefix(ctx, new, sinks):
+    """A sequence of length 0 that brings a token (a batch padded for a graph) sees nothing, so it makes nothing visible either: what the
+    prefix holds before everybody's window stays unread, and its pages may have been given away."""
+    window, prefix = 64, 777
+    bt = Batch([(new, 20), (1, 0), (new, 30)], 8, 2, 128, 16, BF16, prefix=prefix, seed=3)
+    bt.kv_len[1] = 0
+    plan = bt.plan(ctx)
+    want = plan.forward(bt.q, bt.k, bt.v, bt.batch(), window=window, sinks=sinks)
+    ctx.check_device_status()
+    rows = torch.arange(bt.rows, device="cuda") != new
+    w64, bound = attention64(bt, window, sinks)
+    assert ((want.double() - w64).abs() <= bound)[rows].all() and (want[new] == 0).all()
+    hidden = slice(1 if sinks else 0, (prefix + 20 - window + 1) // 16)
+    for page in bt.prefix_host[hidden].tolist():
+        bt.k[page], bt.v[page] = float("nan"), float("nan")
+    given_away = bt.prefix_host.clone()
+    given_away[hidden] = -1
+    for table in (bt.prefix_host, given_away):
+        batch = ttq.PagedBatch(bt.q_start, bt.kv_len, bt.table, max_q=new, prefix_len=prefix, prefix_table=table.cuda())
+        assert torch.equal(plan.forward(bt.q, bt.k, bt.v, batch, window=window, sinks=sinks), want)
+        ctx.check_device_status()
