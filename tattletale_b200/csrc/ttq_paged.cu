@@ -71,11 +71,11 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) paged_append_kernel(const _
         const int s = max(a.q_start[b], 0), e = a.q_start[b + 1];
         const int lo = max(s, t0), hi = min(e, t1);
         if (lo < hi) {
-            const int L = a.kv_len[b];
+            const int L = paged_len(a, b);
             for (int t = lo; t < hi; t++) {
-                const int pos = L - (e - t), own = pos - a.prefix_len, idx = own >> a.page_shift;
+                const int pos = L - (e - t), own = pos >= a.prefix_len ? pos - a.prefix_len : 0, idx = own >> a.page_shift;
                 int page = -1;
-                if (own >= 0 && idx < a.table_len && pos < p.n_rope) page = a.block_table[(int64_t)b * a.ld_table + idx];
+                if (pos >= a.prefix_len && idx < a.table_len && pos < p.n_rope) page = a.block_table[(int64_t)b * a.ld_table + idx];
                 if (page >= 0 && page < a.n_pages) {
                     dst_s[t - t0] = (int64_t)page * p.page_stride + (int64_t)(own & ((1 << a.page_shift) - 1)) * p.token_stride;
                     pos_s[t - t0] = pos;

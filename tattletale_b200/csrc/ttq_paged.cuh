@@ -58,6 +58,9 @@ template <bool BF16>
 constexpr float PAGED_BELOW = BF16 ? 0.f : 9.f;
 constexpr int PAGED_BAD_INDEX = 8;  // status bit: page id or position outside the cache
 
+// A sequence of no or negative length has no positions: its tokens count down from -1.
+__device__ __forceinline__ int paged_len(const PagedArgs &a, int b) { return max(0, a.kv_len[b]); }
+
 // One sequence's rows and keys (prefix pass: the one group of all rows).  Keys are in the coordinates of its page table.
 struct PagedSeq {
     int q0, n;      // first row and number of new tokens

@@ -112,3 +112,20 @@ def test_padding_sequences_of_a_batch_with_a_prefix(ctx, new, sinks):
         batch = ttq.PagedBatch(bt.q_start, bt.kv_len, bt.table, max_q=new, prefix_len=prefix, prefix_table=table.cuda())
         assert torch.equal(plan.forward(bt.q, bt.k, bt.v, batch, window=window, sinks=sinks), want)
         ctx.check_device_status()
+
+
+def test_append_at_negative_lengths_of_a_wide_table(ctx):
+    """A position below zero is outside whatever the table's width: nothing is read or written for its token.  (With 2^27 - 1 pages and a
+    prefix, its distance from the prefix passes 32 bits and would be a place in the table.)"""
+    bt = Batch([(1, 20)], 4, 2, 64, 16, BF16, prefix=100, seed=1)
+    wide = torch.zeros(1, (2 ** 31 - 1) // 16, dtype=torch.int32, device="cuda")
+    plan = bt.plan(ctx)
+    k0 = bt.k.clone()
+    for length in (0, 100, -2 ** 31, -2 ** 31 + 50):
+        bt.kv_len[0] = length
+        batch = ttq.PagedBatch(bt.q_start, bt.kv_len, wide, max_q=1, prefix_len=100, prefix_table=bt.prefix_host.cuda())
+        out = torch.full((1, 4, 64), 3.0, dtype=BF16, device="cuda")
+        plan.append(torch.ones(1, 8 * 64, dtype=BF16, device="cuda"), bt.k, bt.v, batch, torch.ones(200, 64, device="cuda"), torch.ones(200, 64, device="cuda"), q_out=out)
+        with pytest.raises(ttq.TtqError) as ei:
+            ctx.check_device_status()
+        assert ei.value.status == 2 and (out == 3).all() and torch.equal(k0.view(torch.int16), bt.k.view(torch.int16))
