@@ -369,7 +369,8 @@ typedef struct ttq_kv_pages {
 
 /* A ragged batch.  The rows q_start[b] .. q_start[b+1]-1 of the call's tokens are the newest of the kv_len[b] tokens of
  * sequence b: its token i is at position kv_len[b] - (q_start[b+1] - q_start[b]) + i.  Rows from q_start[n_seqs] on belong to
- * no sequence (a padded batch) and are left as they were; a sequence may bring no token.  All three arrays are int32 in
+ * no sequence (a padded batch) and are left as they were; a sequence may bring no token.  Lengths reach up to 2^31 - 4096; tokens
+ * before position 0 (kv_len less than the new tokens, 0 or negative) have no position and see nothing.  All three arrays are int32 in
  * device memory, so a captured graph follows their contents.
  * With prefix_len > 0 every sequence begins with the same prefix_len tokens, whose pages are prefix_table[0 ..
  * ceil(prefix_len / page_size) - 1]; kv_len counts them, the sequence's own table starts behind them: position p >= prefix_len is

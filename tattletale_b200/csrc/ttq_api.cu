@@ -1,6 +1,7 @@
 // C-ABI entry points of libttq: argument validation, context and weight lifetime, dispatch.
 // Nothing here touches weights on the host beyond copying the caller's canonical blocks to the
 // device; there is no CPU compute path.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1639,7 +1640,7 @@ ttq_status paged_args(ttq_ctx *ctx, const ttq_paged *p, const ttq_kv_pages *kv, 
         return fail(ctx, TTQ_ERR_INVALID_ARG, "q_start, kv_len or block_table is NULL");
     if (bt->ld_table < bt->table_len) return fail(ctx, TTQ_ERR_SHAPE, "ld_table is smaller than table_len");
     if (bt->prefix_len > 0 && !bt->prefix_table_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "prefix_table is NULL");
-    if (bt->prefix_len > INT32_MAX || bt->table_len > INT32_MAX / p->page_size)
+    if (bt->prefix_len > PAGED_MAX_LEN || bt->table_len > INT32_MAX / p->page_size)
         return fail(ctx, TTQ_ERR_LIMIT, "prefix_len or table_len: positions are 32-bit");
     if (!kv->k_dev || !kv->v_dev) return fail(ctx, TTQ_ERR_INVALID_ARG, "k or v pages pointer is NULL");
     if (!aligned16(kv->k_dev) || !aligned16(kv->v_dev)) return fail(ctx, TTQ_ERR_INVALID_ARG, "the pages must be 16-byte aligned");
@@ -1771,7 +1772,8 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
     DeviceScope dev(ctx->device);
     if (dev.err != cudaSuccess) return cuda_fail(ctx, dev.err, "cudaSetDevice");
     a.q = q_dev; a.ld_q = ld_q; a.out = out_dev; a.ld_out = ld_out;
-    a.window = window > INT32_MAX ? 0 : (int)window;
+    // a window of all positions that the tables hold hides nothing
+    a.window = window >= std::min<int64_t>(INT32_MAX, bt->prefix_len + bt->table_len * p->page_size) ? 0 : (int)window;
     a.sinks = sinks > INT32_MAX ? INT32_MAX : (int)sinks;
     a.scale2 = scale * 1.4426950408889634f;
     a.part = p->part;

@@ -58,8 +58,15 @@ template <bool BF16>
 constexpr float PAGED_BELOW = BF16 ? 0.f : 9.f;
 constexpr int PAGED_BAD_INDEX = 8;  // status bit: page id or position outside the cache
 
-// A sequence of no or negative length has no positions: its tokens count down from -1.
+// Lengths and positions are 32-bit.  A sequence of no or negative length has no positions: its tokens count down from -1.  Positions end
+// a few units before 2^31, so that the first key behind a unit is still a number.
+constexpr int PAGED_MAX_LEN = INT_MAX - 4095;
 __device__ __forceinline__ int paged_len(const PagedArgs &a, int b) { return max(0, a.kv_len[b]); }
+// First key (of `end`; in the coordinates of a table that begins at position `base`) that the window of a token at `pos` holds.
+__device__ __forceinline__ int paged_window_start(const PagedArgs &a, int pos, int base, int end) {
+    const int64_t first = (int64_t)pos - a.window + 1 - base;
+    return (int)max((int64_t)0, min((int64_t)end, first));
+}
 
 // One sequence's rows and keys (prefix pass: the one group of all rows).  Keys are in the coordinates of its page table.
 struct PagedSeq {
@@ -83,9 +90,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, int b, int min
     } else {
         s.q0 = max(0, min(a.q_start[b], T));
         s.n = max(0, min(a.q_start[b + 1], T) - s.q0);
-        const int L = a.kv_len[b];
+        const int L = paged_len(a, b);
         s.pos0 = L - s.n;
-        const int64_t cap = (int64_t)a.table_len << a.page_shift;
+        const int64_t cap = min((int64_t)a.table_len << a.page_shift, max((int64_t)0, PAGED_MAX_LEN - (int64_t)a.prefix_len));
         end = max(0, L - a.prefix_len);
         if (end > cap) {
             if (s.n > 0) atomicOr(a.status, PAGED_BAD_INDEX);
@@ -98,7 +105,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs &a, int b, int min
     s.lo = 0;
     s.sink = 0;
     if (a.window > 0) {
-        s.lo = max(0, min(end, pmin - a.window + 1 - base));
+        s.lo = paged_window_start(a, pmin, base, end);
         s.sink = max(0, min(s.lo, a.sinks - base));
     }
     return s;
@@ -127,7 +134,7 @@ __device__ __forceinline__ int paged_row_pos(const PagedArgs &a, int token) {
         if (a.q_start[mid] <= token) lo = mid;
         else hi = mid;
     }
-    return a.kv_len[lo] - (a.q_start[lo + 1] - token);
+    return paged_len(a, lo) - (a.q_start[lo + 1] - token);
 }
 
 // Quotients.  The compiler's 64-bit division is several hundred clocks of a warp's time, its 32-bit one a hundred and more, and a CTA
@@ -173,7 +180,7 @@ __device__ __forceinline__ PagedShare paged_share(const PagedArgs &a, int64_t *r
     if (a.prefix_pass && a.window > 0) {
         int mp = INT_MAX;
         for (int b = tid; b < a.B; b += THREADS) {
-            const int n = a.q_start[b + 1] - a.q_start[b], L = a.kv_len[b];
+            const int n = a.q_start[b + 1] - a.q_start[b], L = paged_len(a, b);
             if (n > 0 && L > 0) mp = min(mp, max(0, L - n));  // (padding, a token of no position, sees nothing)
         }
         mp = __reduce_min_sync(0xffffffffu, mp);

@@ -209,7 +209,7 @@ __device__ __forceinline__ TcItem tc_item(const PagedArgs &a, const PagedSeq &s,
         it.k.key_end = max(0, min(s.key_end, s.pos0 + it.tok0 + it.tokens - a.prefix_len));
         it.k.lo = it.k.sink = 0;
         if (a.window > 0) {
-            it.k.lo = max(0, min(it.k.key_end, s.pos0 + it.tok0 - a.window + 1 - a.prefix_len));
+            it.k.lo = paged_window_start(a, s.pos0 + it.tok0, a.prefix_len, it.k.key_end);
             it.k.sink = max(0, min(it.k.lo, a.sinks - a.prefix_len));
         }
     }

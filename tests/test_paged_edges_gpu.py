@@ -114,6 +114,38 @@ def test_padding_sequences_of_a_batch_with_a_prefix(ctx, new, sinks):
         ctx.check_device_status()
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 62])
+@pytest.mark.parametrize("new,kv", [(10, 4), (300, 200), (2, 900)])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_windows_beyond_every_position(ctx, new, kv, window, prefix):
+    """As no window at all, with tokens before position 0 too."""
+    bt = Batch([(new, 1000)], 8, 2, 128, 16, BF16, prefix=prefix, seed=4)
+    bt.kv_len[0] = kv
+    want = run(ctx, bt)
+    assert torch.equal(run(ctx, bt, window=window), want)
+    assert torch.isfinite(want).all() and (want[:max(0, new - kv)] == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("window", [0, 50])
+def test_lengths_at_the_ends_of_their_type(ctx, new, window):
+    """Negative lengths are no length; a length beyond the table is reported.  The other sequence is as it was."""
+    bt = Batch([(new, 90), (new, 70)], 8, 2, 128, 16, BF16, prefix=33, seed=5)
+    want, bound = attention64(bt, window)
+    plan = bt.plan(ctx)
+    for length in (0, -1, -5000, -2 ** 31, -2 ** 31 + 40):
+        bt.kv_len[0] = length
+        out = plan.forward(bt.q, bt.k, bt.v, bt.batch(), window=window)
+        ctx.check_device_status()
+        assert (out[:new] == 0).all()
+        assert ((out.double() - want).abs() <= bound)[new:].all()
+    bt.kv_len[0] = 2 ** 31 - 1
+    plan.forward(bt.q, bt.k, bt.v, bt.batch(), window=window)
+    with pytest.raises(ttq.TtqError) as ei:
+        ctx.check_device_status()
+    assert ei.value.status == 2
+
+
 def test_append_at_negative_lengths_of_a_wide_table(ctx):
     """A position below zero is outside whatever the table's width: nothing is read or written for its token.  (With 2^27 - 1 pages and a
     prefix, its distance from the prefix passes 32 bits and would be a place in the table.)"""
