@@ -80,6 +80,7 @@ struct ttq_moe {
 // Paged attention: head geometry and the workspace of one call.
 struct ttq_paged {
     ttq_ctx *ctx;
+    int device;          // (a plan may be destroyed after its context)
     int dt, hq, hkv, d, page_size, page_shift;
     int64_t max_seqs, max_tokens, max_prefix_tokens;
     void *ws;            // one allocation: arrival counters, records of cut items, partial results, the shared prefix's results
@@ -1693,7 +1694,7 @@ ttq_status ttq_paged_create(ttq_ctx *ctx, ttq_dtype dt, int32_t hq, int32_t hkv,
     if (dev.err != cudaSuccess) return cuda_fail(ctx, dev.err, "cudaSetDevice");
     ttq_paged *p = new (std::nothrow) ttq_paged();
     if (!p) return fail(ctx, TTQ_ERR_OOM, "host allocation failed");
-    p->ctx = ctx; p->dt = dt; p->hq = hq; p->hkv = hkv; p->d = d; p->page_size = page_size;
+    p->ctx = ctx; p->device = ctx->device; p->dt = dt; p->hq = hq; p->hkv = hkv; p->d = d; p->page_size = page_size;
     p->max_seqs = max_seqs; p->max_tokens = max_tokens; p->max_prefix_tokens = max_prefix_tokens;
     while ((1 << p->page_shift) < page_size) p->page_shift++;
     auto up256 = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -1720,7 +1721,7 @@ ttq_status ttq_paged_create(ttq_ctx *ctx, ttq_dtype dt, int32_t hq, int32_t hkv,
 
 ttq_status ttq_paged_destroy(ttq_paged *p) {
     if (!p) return TTQ_OK;
-    DeviceScope dev(p->ctx->device);
+    DeviceScope dev(p->device);
     cudaFree(p->ws);
     delete p;
     return TTQ_OK;

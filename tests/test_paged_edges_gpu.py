@@ -161,3 +161,16 @@ def test_append_at_negative_lengths_of_a_wide_table(ctx):
         with pytest.raises(ttq.TtqError) as ei:
             ctx.check_device_status()
         assert ei.value.status == 2 and (out == 3).all() and torch.equal(k0.view(torch.int16), bt.k.view(torch.int16))
+
+
+def test_a_plan_outlives_its_context():
+    """Contexts are closed and collected in any order: a plan that goes later asks nothing of its context."""
+    ctx = ttq.Context(0)
+    plans = [ttq.PagedAttention(ctx, 8, 2, 64, 16, max_seqs=4, max_tokens=4) for _ in range(2)]
+    ctx.close()
+    held = torch.cuda.mem_get_info()[0]
+    for plan in plans:
+        plan.close()
+    assert torch.cuda.mem_get_info()[0] >= held and torch.cuda.current_device() == 0
+    with pytest.raises(ttq.TtqError):
+        ttq.PagedAttention(ctx, 8, 2, 64, 16, max_seqs=4, max_tokens=4)
