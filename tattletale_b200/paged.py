@@ -60,8 +60,12 @@ class PagedBatch:
         page_size = plan.page_size
         if self.prefix_len > self._page_entries * page_size:
             raise TtqError(2, f"prefix_table has {self._page_entries} pages of {page_size}, prefix_len is {self.prefix_len}")
-        self._args.n_tokens = n_tokens
-        return self._args
+        args = self._args
+        if args.n_tokens != n_tokens:  # (a copy: another thread's call may hold the present ones)
+            args = PagedBatchArgs.from_buffer_copy(args)
+            args.n_tokens = n_tokens
+            self._args = args
+        return args
 
 
 class PagedAttention:

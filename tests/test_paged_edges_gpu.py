@@ -174,3 +174,13 @@ def test_a_plan_outlives_its_context():
     assert torch.cuda.mem_get_info()[0] >= held and torch.cuda.current_device() == 0
     with pytest.raises(ttq.TtqError):
         ttq.PagedAttention(ctx, 8, 2, 64, 16, max_seqs=4, max_tokens=4)
+
+
+def test_a_batch_shared_by_plans(ctx):
+    """Two threads with contexts of their own may use one batch: a call's arguments stay as they were handed over."""
+    bt = Batch([(1, 20), (2, 20)], 8, 2, 128, 16, BF16)
+    plan, batch = bt.plan(ctx), bt.batch()
+    first = batch._for(plan, 3)
+    second = batch._for(plan, 2)
+    assert (first.n_tokens, second.n_tokens) == (3, 2) and second.kv_len_dev == first.kv_len_dev == bt.kv_len.data_ptr()
+    check_attention(plan.forward(bt.q, bt.k, bt.v, batch), bt)
