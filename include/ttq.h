@@ -428,7 +428,7 @@ typedef struct ttq_sampling {
     int32_t top_k;
 } ttq_sampling;
 
-/* ids[m] = the next token of logits row m [V] (f32, bf16 or f16), drawn with the random number u[m] in [0, 1).
+/* ids[m] = the next token of logits row m [V] (f32, bf16 or f16; rows ld apart, 0: one row for all), drawn with the random number u[m] in [0, 1).
  * With w_i = exp((x_i - max x) / temperature) the tokens in descending order of x (equal logits: lowest index first) are cut to
  * the first top_k (0 or less: all), of those to the shortest run that holds top_p of their weight (1 or more: all; at least
  * one token stays), of those to w_i >= min_p (the largest logit always stays).  The result is the first token, in the order of the vocabulary, at which the

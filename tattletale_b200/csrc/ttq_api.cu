@@ -1806,7 +1806,7 @@ ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *p, const ttq_kv_pages *k
 ttq_status ttq_sample(ttq_ctx *ctx, const void *logits_dev, ttq_dtype dt, int64_t M, int64_t V, int64_t ld, const ttq_sampling *sp,
                       const float *u_dev, int64_t *ids_dev, void *stream) {
     if (!ctx) return TTQ_ERR_INVALID_ARG;
-    if (M < 0 || V <= 0 || ld < V) return fail(ctx, TTQ_ERR_SHAPE, "bad size (M=%lld V=%lld ld=%lld)", (long long)M, (long long)V, (long long)ld);
+    if (M < 0 || V <= 0 || (ld < V && ld != 0)) return fail(ctx, TTQ_ERR_SHAPE, "bad size (M=%lld V=%lld ld=%lld)", (long long)M, (long long)V, (long long)ld);
     if (V > (1 << 18)) return fail(ctx, TTQ_ERR_LIMIT, "V=%lld exceeds 2^18", (long long)V);
     if (M > INT32_MAX / 16) return fail(ctx, TTQ_ERR_LIMIT, "M=%lld exceeds the grid", (long long)M);
     if (!sp) return fail(ctx, TTQ_ERR_INVALID_ARG, "sampling settings are NULL");

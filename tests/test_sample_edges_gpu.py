@@ -1,4 +1,4 @@
-"""The sampler at its edges: random numbers outside their range."""
+"""The sampler at its edges: random numbers outside their range, one row for all, settings beyond their type."""
 import numpy as np
 import pytest
 import torch
@@ -24,3 +24,19 @@ def test_random_numbers_outside_their_range(ctx, v, u):
             want = [sample64(logits[r].cpu().numpy(), clamped, np.float32(s.get("temperature", 1.0)), s.get("top_k", 0), np.float32(s.get("top_p", 1.0)), 0.0)
                     for r in range(5)]
             assert out.tolist() == want
+
+
+@pytest.mark.parametrize("v", [1, 5000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_draws_from_one_row(ctx, v, dtype):
+    """Rows of pitch 0: an expanded row is as good as copies of it."""
+    g = torch.Generator().manual_seed(v)
+    x, u = torch.randn(v, generator=g).to(dtype).cuda(), torch.rand(300, generator=g).cuda()
+    for s in (dict(), dict(top_k=40, top_p=0.9), dict(temperature=0.0)):
+        assert torch.equal(ttq.sample(ctx, x.expand(300, -1), u, **s), ttq.sample(ctx, x.repeat(300, 1), u, **s))
+
+
+def test_overlapping_rows_are_refused(ctx):
+    with pytest.raises(ttq.TtqError) as ei:
+        ttq.sample(ctx, torch.zeros(150, device="cuda").as_strided((2, 100), (50, 1)), torch.zeros(2, device="cuda"))
+    assert ei.value.status == 2
