@@ -197,7 +197,7 @@ def sample(ctx: Context, logits: torch.Tensor, u: torch.Tensor, temperature: Uni
             keep.append(_on(ctx, value, name))
             setattr(s, name + "_dev", value.data_ptr())
         else:
-            setattr(s, name, value)
+            setattr(s, name, max(0, min(value, 2 ** 31 - 1)) if name == "top_k" else value)  # (ctypes would wrap it)
     if u.numel() != m or u.dtype != torch.float32 or not u.is_contiguous():
         raise TtqError(2, f"u must be {m} contiguous values of float32")
     _on(ctx, u, "u")

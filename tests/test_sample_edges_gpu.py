@@ -40,3 +40,12 @@ def test_overlapping_rows_are_refused(ctx):
     with pytest.raises(ttq.TtqError) as ei:
         ttq.sample(ctx, torch.zeros(150, device="cuda").as_strided((2, 100), (50, 1)), torch.zeros(2, device="cuda"))
     assert ei.value.status == 2
+
+
+def test_top_k_beyond_32_bits(ctx):
+    """More than the vocabulary, or 0 and less: no cut."""
+    g = torch.Generator().manual_seed(1)
+    x, u = torch.randn(64, 5000, generator=g).cuda(), torch.rand(64, generator=g).cuda()
+    want = ttq.sample(ctx, x, u)
+    for k in (5000, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 2 ** 40, -1, -2 ** 32 + 5):
+        assert torch.equal(ttq.sample(ctx, x, u, top_k=k), want), k
