@@ -862,7 +862,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
 // Joins the parts of the items that share borders have cut: CTA (c, y) takes 256 groups of eight results of the item that begins in
 // share c, one thread each.  A launch of its own, since a single CTA reads the parts of a widely cut item (two hundred rows against a
 // long prefix: 2 MB) at a hundred GB/s: 95 us of 187 us when the last CTA to arrive did it (48 decode rows, prefix of 12345).
-constexpr int TC_JOIN_THREADS = 256, TC_JOIN_PARTS = 160;
+constexpr int TC_JOIN_THREADS = 256, TC_JOIN_PARTS = 160;  // (a grid has no more CTAs than an item may have parts; the card: 148)
 template <int D, bool BF16>
 __global__ void __launch_bounds__(TC_JOIN_THREADS) paged_tc_join_kernel(const __grid_constant__ PagedArgs a) {
     grid_launch_dependents();
@@ -878,44 +878,38 @@ __global__ void __launch_bounds__(TC_JOIN_THREADS) paged_tc_join_kernel(const __
     auto part_of = [&](int i) { return (int64_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * pitch; };
     const int rr = r % TC_ROWS, t = paged_div(rr, a.G, a.inv_G), tok = sp.tok0 + r / TC_ROWS * tc_tokens(a) + t;
     const bool valid = t < tc_tokens(a) && tok < sp.n;
-    float m, l, v[8];
-    if (parts <= TC_JOIN_PARTS) {
-        // the threads of a row share the parts' maxima and sums, then every thread adds its columns with all loads in flight
-        const float *ml = a.part + (int64_t)TC_ITEM_ROWS * D + 2 * r;
-        const unsigned group = __activemask();  // (whole warps)
-        m = -INFINITY;
-        if (valid)
-            for (int i = lane; i < parts; i += PER_ROW) {
-                const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + part_of(i)));
-                w_s[i][lr] = x;
-                m = fmaxf(m, x.x);
-            }
-#pragma unroll
-        for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(group, m, o));
-        l = 0.f;
-        if (valid)
-            for (int i = lane; i < parts; i += PER_ROW) {
-                const float2 x = w_s[i][lr];
-                const float w = x.x == -INFINITY ? 0.f : ex2(x.x - m);
-                w_s[i][lr].x = w;
-                w_s[i][lr].y = x.y * w;
-            }
-        __syncwarp();
-#pragma unroll
-        for (int x = 0; x < 8; x++) v[x] = 0.f;
-        if (!valid) return;
-        const float *o = a.part + (int64_t)r * D + col;
-#pragma unroll 8
-        for (int i = 0; i < parts; i++) {
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(o + part_of(i))), y = __ldcg(reinterpret_cast<const float4 *>(o + part_of(i) + 4));
-            const float w = w_s[i][lr].x;
-            l += w_s[i][lr].y;
-            v[0] = fmaf(w, x.x, v[0]); v[1] = fmaf(w, x.y, v[1]); v[2] = fmaf(w, x.z, v[2]); v[3] = fmaf(w, x.w, v[3]);
-            v[4] = fmaf(w, y.x, v[4]); v[5] = fmaf(w, y.y, v[5]); v[6] = fmaf(w, y.z, v[6]); v[7] = fmaf(w, y.w, v[7]);
+    float m, l = 0.f, v[8];
+    // the threads of a row share the parts' maxima and sums, then every thread adds its columns with all loads in flight
+    const float *ml = a.part + (int64_t)TC_ITEM_ROWS * D + 2 * r;
+    const unsigned group = __activemask();  // (whole warps)
+    m = -INFINITY;
+    if (valid)
+        for (int i = lane; i < parts; i += PER_ROW) {
+            const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + part_of(i)));
+            w_s[i][lr] = x;
+            m = fmaxf(m, x.x);
         }
-    } else {
-        if (!valid) return;
-        paged_gather8<TC_ITEM_ROWS>(a, D, c0, sp.c1, r, col, m, l, v);
+#pragma unroll
+    for (int o = PER_ROW / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(group, m, o));
+    if (valid)
+        for (int i = lane; i < parts; i += PER_ROW) {
+            const float2 x = w_s[i][lr];
+            const float w = x.x == -INFINITY ? 0.f : ex2(x.x - m);
+            w_s[i][lr].x = w;
+            w_s[i][lr].y = x.y * w;
+        }
+    __syncwarp();
+#pragma unroll
+    for (int x = 0; x < 8; x++) v[x] = 0.f;
+    if (!valid) return;
+    const float *o = a.part + (int64_t)r * D + col;
+#pragma unroll 8
+    for (int i = 0; i < parts; i++) {
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(o + part_of(i))), y = __ldcg(reinterpret_cast<const float4 *>(o + part_of(i) + 4));
+        const float w = w_s[i][lr].x;
+        l += w_s[i][lr].y;
+        v[0] = fmaf(w, x.x, v[0]); v[1] = fmaf(w, x.y, v[1]); v[2] = fmaf(w, x.z, v[2]); v[3] = fmaf(w, x.w, v[3]);
+        v[4] = fmaf(w, y.x, v[4]); v[5] = fmaf(w, y.y, v[5]); v[6] = fmaf(w, y.z, v[6]); v[7] = fmaf(w, y.w, v[7]);
     }
     paged_finish8<BF16>(a, D, sp.q0 + tok, sp.head * a.G + (rr - t * a.G), col, m, l, v);
 }
@@ -928,9 +922,10 @@ cudaError_t launch_tc_t(const PagedArgs &a, const PagedMaps &maps, int box_rows,
     static OncePerDevice once;
     const cudaError_t e = once([&]() { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM); });
     if (e != cudaSuccess) return e;
-    const cudaError_t r = launch_pdl(kernel, dim3((unsigned)a.sms), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, maps.q, box_rows);
+    const unsigned ctas = (unsigned)(a.sms < TC_JOIN_PARTS ? a.sms : TC_JOIN_PARTS);
+    const cudaError_t r = launch_pdl(kernel, dim3(ctas), dim3(TC_THREADS), C::SMEM, st, a, maps.k, maps.v, maps.q, box_rows);
     if (r != cudaSuccess) return r;
-    return launch_pdl(paged_tc_join_kernel<D, BF16>, dim3((unsigned)a.sms, TC_ITEM_ROWS * D / 8 / TC_JOIN_THREADS), dim3(TC_JOIN_THREADS), 0, st, a);
+    return launch_pdl(paged_tc_join_kernel<D, BF16>, dim3(ctas, TC_ITEM_ROWS * D / 8 / TC_JOIN_THREADS), dim3(TC_JOIN_THREADS), 0, st, a);
 }
 
 }  // namespace

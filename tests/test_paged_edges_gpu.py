@@ -184,3 +184,12 @@ def test_a_batch_shared_by_plans(ctx):
     second = batch._for(plan, 2)
     assert (first.n_tokens, second.n_tokens) == (3, 2) and second.kv_len_dev == first.kv_len_dev == bt.kv_len.data_ptr()
     check_attention(plan.forward(bt.q, bt.k, bt.v, batch), bt)
+
+
+@pytest.mark.parametrize("d,new,prefix", [(128, 40, 0), (64, 100, 0), (128, 25, 59000)])
+def test_one_item_cut_into_as_many_parts_as_there_are_ctas(ctx, d, new, prefix):
+    """One row tile against 60000 keys: every multiprocessor has a part of it."""
+    bt = Batch([(new, 60000 - prefix)], 4, 1, d, 64, BF16, prefix=prefix, seed=d)
+    first = run(ctx, bt)
+    check_attention(first, bt)
+    assert torch.equal(run(ctx, bt), first)
