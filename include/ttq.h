@@ -380,7 +380,7 @@ typedef struct ttq_kv_pages {
  * memory; the call's results are then invalid and ttq_device_status reports TTQ_ERR_SHAPE. */
 typedef struct ttq_paged_batch {
     int64_t n_seqs, n_tokens;   /* n_tokens: rows of qkv, q and out (at least q_start[n_seqs]) */
-    int64_t max_q;              /* most new tokens of any sequence: selects the kernel, results do not depend on it (0: unknown) */
+    int64_t max_q;              /* most new tokens of any sequence: selects the kernel, results do not depend on it (0: unknown, taken for n_tokens: slow for many short ones) */
     const int32_t *q_start_dev;     /* [n_seqs + 1], ascending from 0 */
     const int32_t *kv_len_dev;      /* [n_seqs] */
     const int32_t *block_table_dev; /* [n_seqs][ld_table], the first table_len entries of a row are used */
@@ -413,7 +413,8 @@ TTQ_API ttq_status ttq_paged_append(ttq_ctx *ctx, ttq_paged *plan, const ttq_kv_
  * q and out: [n_tokens][ld], hq x d used, 16-byte aligned rows of the plan's dtype.  Scores, softmax statistics and sums in
  * fp32; the softmax weights enter the second product in the plan's dtype (each rounded to it, in f16 to no less than 2^-34 of the
  * row's largest).  What the cache holds at positions that no token
- * of a sequence sees is ignored, NaN included; keys and values that some token sees must be finite. */
+ * of a sequence sees is ignored, NaN included; keys and values that some token sees must be finite (with a window: those of the
+ * shared prefix from the earliest window of any token on). */
 TTQ_API ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *plan, const ttq_kv_pages *kv, const ttq_paged_batch *batch,
                                        const void *q_dev, int64_t ld_q, float scale, int64_t window, int64_t sinks,
                                        void *out_dev, int64_t ld_out, void *stream);

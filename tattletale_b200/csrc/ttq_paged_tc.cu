@@ -22,8 +22,9 @@
 // place, which they do only when the weights outgrow their reference and once the last product that they asked for is complete.
 //
 // Bound: 4 d flops and one exponential per key and row; at d = 128 the special-function unit (16 a clock and SM) takes as long for a
-// unit's exponentials as the tensor core for its products, 2048 clocks for both streams.  Measured: 780 TFLOP/s on prompts of
-// 1111 to 4300 tokens (284 us, 47 % of the measured bf16 rate), 850 on 24000 shared keys.
+// unit's exponentials as the tensor core for its products, 2048 clocks for both streams.  Measured: prompts of 1111 to 4300
+// tokens 301 us among other passes on changing inputs (737 TFLOP/s, 44 % of the measured bf16 rate), 285 back to back on the same ones; 24000
+// shared keys 172 and 157 us (774 and 847 TFLOP/s).
 #include <climits>
 
 #include "ttq_devutil.cuh"
@@ -445,8 +446,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_tc_kernel(const __grid_co
                     // scores costs a fifth of their softmax.
                     // The streams' exponentials take turns.  Each alone keeps the special-function unit busy (590 clocks for 64 rows' weights of a
                     // warp, 512 at the unit's rate); both at once take as long as one after the other, and then both wait for
-                    // their next scores at once, the unit idle.  The turn passes on half way, which hides the hand-over (prompts of 8116
-                    // tokens: 308 us without turns, 291 with, 284 passing on half way; 24000 shared keys: 176, 170, 158).
+                    // their next scores at once, the unit idle.  The turn passes on half way, which hides the hand-over (back to
+                    // back, prompts of 8116 tokens: 308 us without turns, 291 with, 284 passing on half way; 24000 shared keys: 176, 170, 158).
                     if (!joint) pair_sync(TC_TURN_BAR + 2 * (warp & 3) + st);
                     float sum;
                     bool redo = mx == -INFINITY;

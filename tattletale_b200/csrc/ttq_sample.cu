@@ -10,8 +10,8 @@
 // first over 2048 equal parts of the range that has weight (max - 32 T to max: evenly spread logits, few collisions).  The tokens of the
 // part with the cut, a few hundred, go to the first CTA, which goes on alone: each against each, or, above 512, histograms over the
 // order-preserving keys, 2048 at a time, until a bin is one key.  (Only where a part holds more than LIST tokens do all CTAs go on, adding into the first
-// one's histogram.)  Bound: one reading of the logits; in practice the 64-bit exponentials (11 instructions each, half the
-// rate of 32-bit ones) for large batches, the chain of cluster barriers for small ones.
+// one's histogram.)  Bound: one reading of the logits; in practice the 64-bit exponentials (58 clocks per 32 weights and
+// scheduler, 22 of them for eleven 64-bit instructions at half the 32-bit rate) for large batches, the chain of cluster barriers for small ones.
 #include <cooperative_groups.h>
 
 #include "ttq_internal.cuh"
@@ -94,7 +94,7 @@ __device__ __forceinline__ void add_u64(uint32_t *lo, uint32_t *hi, u64 v) {
 }
 
 // exp((x - max) / T) in 2^-44 fixed point.  2^y with y = 512ths + r: a table and the series of 2^r to r^3 (|r| <= 2^-10: 9e-15 of the
-// weight).  64-bit instructions are what the sampler spends its time on (a quarter of the 32-bit rate and less), so the
+// weight).  64-bit instructions run at half the rate of 32-bit ones and conversions slower, so the
 // logit is widened by integer instructions and the range is checked in 32 bits: beyond -46 the weight is zero either way.
 constexpr int TABLE = 512;
 struct Weigher {

@@ -29,7 +29,8 @@ def _on(ctx: Context, t: torch.Tensor, name: str) -> torch.Tensor:
 class PagedBatch:
     """A ragged batch (``ttq_paged_batch``): rows ``q_start[b] .. q_start[b+1]-1`` are the newest of the ``kv_len[b]`` tokens of
     sequence b, whose pages are ``block_table[b]``.  int32 tensors on the device; their contents may change between calls (a
-    captured graph follows them), ``max_q`` is the most new tokens of any sequence (0: unknown; it selects the kernel only).
+    captured graph follows them), ``max_q`` is the most new tokens of any sequence (it selects the kernel only; 0: unknown, slow for
+    many short ones).
     With ``prefix_len`` all sequences begin with the tokens of ``prefix_table``'s pages; ``kv_len`` counts them, the
     block tables start behind them."""
 
@@ -70,7 +71,8 @@ class PagedBatch:
 
 class PagedAttention:
     """Head geometry and workspace of paged attention (``ttq_paged_create``); one object serves all layers of a model, its calls
-    follow each other on one stream.  A layer's cache is a pair of tensors ``[n_pages, n_kv_heads, page_size, head_dim]`` (any
+    follow each other on one stream.  ``max_prefix_tokens`` (default: ``max_tokens``) makes room for calls with a
+    shared prefix, (head_dim + 1) * 4 bytes per token and query head; 0 where no batch has one.  A layer's cache is a pair of tensors ``[n_pages, n_kv_heads, page_size, head_dim]`` (any
     strides with a contiguous head dimension, so a permuted view of another layout will do)."""
 
     def __init__(self, ctx: Context, n_q_heads: int, n_kv_heads: int, head_dim: int, page_size: int, max_seqs: int, max_tokens: int,
@@ -179,7 +181,7 @@ class PagedAttention:
 def sample(ctx: Context, logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0,
            top_p: Union[float, torch.Tensor] = 1.0, min_p: Union[float, torch.Tensor] = 0.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The next token (int64) of every row of ``logits`` ``[rows, vocabulary]``, drawn with the random numbers ``u`` ``[rows]`` (f32 in
-    [0, 1)).  Settings are one value for all rows or a tensor of one per row; top-k, then top-p, then min-p, as ``ttq_sample`` defines
+    [0, 1); others count as the nearest, NaN as 0).  ``logits`` may be one row expanded to many.  Settings are one value for all rows or a tensor of one per row; top-k, then top-p, then min-p, as ``ttq_sample`` defines
     them.  A temperature of 0 takes the largest logit, the lowest index among equals; a row with nothing but -inf (or NaN) gives -1."""
     if logits.dim() != 2:
         raise TtqError(2, "logits must be [rows, vocabulary]")
