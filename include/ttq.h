@@ -411,8 +411,8 @@ TTQ_API ttq_status ttq_paged_append(ttq_ctx *ctx, ttq_paged *plan, const ttq_kv_
  * out[t][h] = softmax_j(scale * q[t][h] . k[j][h / (hq/hkv)]) . v over the keys j <= p of a token at position p and, with
  * window > 0, of those only j > p - window or j < sinks (the first tokens stay visible).  A row that sees no key gives zeros.
  * q and out: [n_tokens][ld], hq x d used, 16-byte aligned rows of the plan's dtype.  Scores, softmax statistics and sums in
- * fp32; the softmax weights enter the second product in the plan's dtype (each rounded to it, in f16 to no less than 2^-34 of the
- * row's largest).  What the cache holds at positions that no token
+ * fp32; the softmax weights enter the second product in the plan's dtype (each rounded to it; in f16, whose steps
+ * end, to within 2^-34 of the row's largest).  What the cache holds at positions that no token
  * of a sequence sees is ignored, NaN included; keys and values that some token sees must be finite (with a window: those of the
  * shared prefix from the earliest window of any token on). */
 TTQ_API ttq_status ttq_paged_attention(ttq_ctx *ctx, ttq_paged *plan, const ttq_kv_pages *kv, const ttq_paged_batch *batch,

@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(ROWS_THREADS, PAGED_ROWS16_CTAS) paged_rows_ke
             min_row = r == 0 ? lo : min(min_row, lo);
             max_row = r == 0 ? hi : max(max_row, hi);
         }
-        lo_row = min_row;
+        lo_row = max(min_row, 0);
         if (a.prefix_pass && min_row < 0)  // (rows of other sequences, which may be padding)
             lo_row = __reduce_min_sync(0xffffffffu, min(pos0 >= 0 ? pos0 : INT_MAX, pos1 >= 0 ? pos1 : INT_MAX));
 #pragma unroll
