@@ -476,7 +476,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         cluster_sync();
         for (int c = 0; c < rank; c++) ties_before += (u64)cluster.map_shared_rank(&sh, c)->ties;
     }
-    const u64 floor_w = min_p > 0.f ? (u64)ceil(fmin((double)min_p, 2.0) * FIXED_ONE) : 0;
+    // (1 and more: nothing but the largest logit, whose weight a fixed-point one may equal by its rounding)
+    const u64 floor_w = min_p >= 1.f ? (u64)FIXED_ONE + 1 : (min_p > 0.f ? (u64)ceil((double)min_p * FIXED_ONE) : 0);
     const float cut_x = cut_key > 0 ? of_key(cut_key) : -INFINITY;
     auto walk = [&](auto &&visit) {  // visit(i, kept weight) over this warp's run, 32 tokens at a time; false ends it
         u64 tie = ties_before;

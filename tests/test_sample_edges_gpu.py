@@ -49,3 +49,17 @@ def test_top_k_beyond_32_bits(ctx):
     want = ttq.sample(ctx, x, u)
     for k in (5000, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 2 ** 40, -1, -2 ** 32 + 5):
         assert torch.equal(ttq.sample(ctx, x, u, top_k=k), want), k
+
+
+@pytest.mark.parametrize("min_p", [1.0, 1.5, float("inf")])
+def test_min_p_of_one_keeps_the_largest_logit_alone(ctx, min_p):
+    """A weight of 1 - 10^-14 is less than 1, though not as 2^-44 fixed point; equal logits are all the largest."""
+    x = torch.zeros(4, 600, device="cuda")
+    x[:, ::2] = -1e-10
+    x[1:, 11:] = -1e-10
+    x[2:, 3] = -1e-10
+    for u in (0.0, 0.3, 0.7, 0.9999):
+        got = ttq.sample(ctx, x, torch.full((4,), u, device="cuda"), temperature=1e4, min_p=min_p)
+        u = float(np.float32(u))
+        want = [1 + 2 * int(u * 300), 1 + 2 * int(u * 5), [1, 5, 7, 9][int(u * 4)], [1, 5, 7, 9][int(u * 4)]]
+        assert got.tolist() == want
